@@ -381,6 +381,97 @@ int rw_gemm_bf16(const void* A, long long lda, const void* B, long long ldb, con
  * the tiles fill whole rounds). */
 long long rw_gemm_workspace_bytes(int M, int N, int K);
 
+/* ---- paged KV cache ---------------------------------------------------------
+ * Many sessions' keys and values in pages of one pool, for a ragged batch of
+ * sequences.  The reference keeps one contiguous cache per session
+ * (pipeline/causal_diffusion_inference.py:372-414); these calls are the paged
+ * form of its cache write (wan_5b/modules/action_model.py:265-292), of the
+ * attention that reads it (:302) and of a bounded cache's eviction.
+ *
+ * k, v: pools [num_pages, page_size, Hkv, D] with the element strides of page,
+ * row and head (multiples of 8; the channels are contiguous), 16-byte aligned,
+ * D 64 or 128, page_size a power of two >= 8.  Row r of sequence b lies in page
+ * block_table[b * table_stride + r / page_size] at row r % page_size.
+ * q_starts [B + 1]: sequence b's new tokens are q_starts[b] .. q_starts[b + 1] - 1
+ * of the call's packed tokens; kv_lens [B]: cached rows, the new tokens'
+ * included (they are the last ones).  block_table, q_starts and kv_lens are
+ * DEVICE memory, read when the kernels run.  A value out of range (a page
+ * outside the pool, a length beyond the table, starts that fall or pass T) is
+ * brought into range and RW_STATUS_BAD_SLOT is reported; no address leaves the
+ * pools and the tensors.  table_width * page_size <= 2^30. */
+#define RW_DTYPE_BF16 0
+#define RW_DTYPE_FP16 1
+typedef struct rw_paged {
+  void* k;
+  void* v;
+  long long k_sp, k_sl, k_sh, v_sp, v_sl, v_sh;
+  int num_pages, page_size, Hkv, D, dtype, B, table_width, pad;
+  const int* block_table;
+  long long table_stride;
+  const int* q_starts;
+  const int* kv_lens;
+} rw_paged_t;
+
+/* Rotary positions: out[t, h] = x[t, h] with the pairs of its first `rot`
+ * channels turned by table[positions[t]] (fp32 (cos, sin) pairs [max_pos][rot /
+ * 2], 16-byte aligned); the pairs are channels (2i, 2i + 1) when interleaved != 0,
+ * else (i, i + rot / 2); channels behind `rot` are copied.  rot a multiple of 16.
+ * fp32 arithmetic, one rounding.  out may be x (same strides).  A position
+ * outside the table takes its nearest row and RW_STATUS_BAD_SLOT is reported.
+ * The 1-D, table-per-position counterpart of causal_rope_apply
+ * (wan_5b/modules/causal_model.py:156-184). */
+int rw_rotary(const void* x, void* out, int T, int H, int D, int dtype, long long x_sl, long long x_sh,
+              long long o_sl, long long o_sh, const float* table, int max_pos, int rot, int interleaved,
+              const int* positions, int* status, void* stream);
+
+/* The new tokens' keys, rotated, and values into their sequences' pages (token i
+ * of sequence b is row kv_lens[b] - lq + i), and q_out = rotated q when q != NULL,
+ * in one launch.  k, v: [T, Hkv, D], q, q_out: [T, Hq, D] (q_out may be q).
+ * positions [T] or NULL (then a token's row is its position); table NULL: no
+ * rotation.  Tokens behind the last sequence, and rows of the pools that no new
+ * token has, stay as they were. */
+int rw_paged_rotary_store(const rw_paged_t* cache, const void* k, const void* v, const void* q, void* q_out, int T,
+                          int Hq, long long k_sl, long long k_sh, long long v_sl, long long v_sh, long long q_sl,
+                          long long q_sh, long long qo_sl, long long qo_sh, const float* table, int max_pos, int rot,
+                          int interleaved, const int* positions, int* status, void* stream);
+
+/* Attention of the new tokens over their sequences' cached rows: out[t, h] =
+ * softmax(q[t, h] k^T * softmax_scale) v over key head h / (Hq / Hkv), fp32
+ * statistics and accumulation, one rounding of the output.  causal != 0: token i
+ * of a sequence with lq new tokens sees rows 0 .. kv - lq + i, otherwise all kv.
+ * A row that sees nothing gets zeros and lse -inf.  What lies in a page behind
+ * the rows that a token sees has no effect, NaN included.  lse ([T, Hq] fp32,
+ * may be NULL): natural logarithm of the sum of exp(score).  Hq / Hkv <= 128.
+ * max_q_len: no sequence has more new tokens (rows of a longer one are not
+ * computed).  Rows of out and lse behind the last sequence stay as they were.
+ * sums (may be NULL): fp32 [B, Hkv, >= table_width * page_size] with element strides
+ * sums_sb, sums_sh; sums[b, g, j] += the weights that the rows of key head g's group
+ * gave to cached row j.  The order of the additions is fixed.
+ * counters: n_counters ints of device memory, zeroed once; every call leaves them
+ * zero.  workspace: 16-byte aligned, rw_paged_attn_workspace_bytes(...) bytes,
+ * which also tells the counters needed.  Calls that overlap on the GPU need
+ * counters and workspaces of their own. */
+int rw_paged_attn(const rw_paged_t* cache, const void* q, void* out, float* lse, int T, int Hq, int max_q_len,
+                  long long q_sl, long long q_sh, long long o_sl, long long o_sh, int causal, float softmax_scale,
+                  float* sums, long long sums_sb, long long sums_sh, int* counters, long long n_counters,
+                  void* workspace, long long workspace_bytes, int* status, void* stream);
+long long rw_paged_attn_workspace_bytes(int T, int Hq, int Hkv, int D, int B, int max_q_len, long long cache_rows,
+                                        int with_sums, long long* n_counters);
+
+/* Eviction by accumulated attention weight.  Of the kv rows of every sequence and
+ * key head, the first n_sink and the last n_recent are kept and, of the others,
+ * those with the largest sums (equal: the lower row; NaN: below everything), keep
+ * rows in all (all kv where kv <= keep), in their order.  Row j of the result goes
+ * to page dst_table[b * dst_stride + j / page_size] of the same pools; the pages of
+ * the two tables must be apart.  kept [B, Hkv, keep]: the kept rows, -1 behind the
+ * last; new_sums [B, Hkv, new_cap], new_cap >= keep: their sums, 0 behind the last;
+ * new_lens [B] = min(kv, keep).  new_sums must not overlap sums.  q_starts is not
+ * read.  The weight-ranked counterpart of the landmark bank's pose-ranked eviction
+ * (longctx/inference/landmark_cache_v2.py:465-479). */
+int rw_paged_evict(const rw_paged_t* cache, const float* sums, long long sums_sb, long long sums_sh, float* new_sums,
+                   long long new_cap, int* kept, int* new_lens, int keep, int n_sink, int n_recent,
+                   const int* dst_table, long long dst_stride, int dst_width, int* status, void* stream);
+
 /* Human-readable text of an RW_ERR_* code. */
 const char* rw_error_string(int code);
 

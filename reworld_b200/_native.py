@@ -52,6 +52,14 @@ class RwCopyDesc(ctypes.Structure):
     _fields_ = [("src", c_vp), ("dst", c_vp), ("nbytes", c_ll)]
 
 
+class RwPaged(ctypes.Structure):
+    """rw_paged_t: the pools of a paged cache and the batch that uses them."""
+    _fields_ = [("k", c_vp), ("v", c_vp), ("k_sp", c_ll), ("k_sl", c_ll), ("k_sh", c_ll), ("v_sp", c_ll),
+                ("v_sl", c_ll), ("v_sh", c_ll), ("num_pages", c_int), ("page_size", c_int), ("Hkv", c_int),
+                ("D", c_int), ("dtype", c_int), ("B", c_int), ("table_width", c_int), ("pad", c_int),
+                ("block_table", c_vp), ("table_stride", c_ll), ("q_starts", c_vp), ("kv_lens", c_vp)]
+
+
 # name -> (restype, argtypes)
 _SIGNATURES = {
     "rw_attn_fwd": (c_int, [c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int] + [c_ll] * 12
@@ -80,11 +88,19 @@ _SIGNATURES = {
     "rw_gemm_bf16": (c_int, [c_vp, c_ll, c_vp, c_ll, c_vp, c_vp, c_ll, c_vp, c_ll, c_int, c_int, c_int, c_int, c_vp,
                              c_ll, c_vp, c_vp]),
     "rw_gemm_workspace_bytes": (c_ll, [c_int, c_int, c_int]),
+    "rw_rotary": (c_int, [c_vp, c_vp] + [c_int] * 4 + [c_ll] * 4 + [c_vp] + [c_int] * 3 + [c_vp] * 3),
+    "rw_paged_rotary_store": (c_int, [ctypes.POINTER(RwPaged)] + [c_vp] * 4 + [c_int] * 2 + [c_ll] * 8 + [c_vp]
+                              + [c_int] * 3 + [c_vp] * 3),
+    "rw_paged_attn": (c_int, [ctypes.POINTER(RwPaged)] + [c_vp] * 3 + [c_int] * 3 + [c_ll] * 4 + [c_int, c_float, c_vp]
+                      + [c_ll] * 2 + [c_vp, c_ll, c_vp, c_ll, c_vp, c_vp]),
+    "rw_paged_attn_workspace_bytes": (c_ll, [c_int] * 6 + [c_ll, c_int, ctypes.POINTER(c_ll)]),
+    "rw_paged_evict": (c_int, [ctypes.POINTER(RwPaged), c_vp, c_ll, c_ll, c_vp, c_ll, c_vp, c_vp] + [c_int] * 3
+                       + [c_vp, c_ll, c_int, c_vp, c_vp]),
     "rw_error_string": (ctypes.c_char_p, [c_int]),
     "rw_abi_version": (c_int, []),
 }
 
-ABI_VERSION = 4
+ABI_VERSION = 5
 _lib = None
 
 

@@ -1,0 +1,116 @@
+// What the kernels over a paged KV cache share: the pools and the batch as they
+// travel to a kernel, the bounds that every kernel puts on what it reads from
+// device memory (page indices, lengths, starts), and the 16-bit types.
+//
+// The pools are [num_pages, page_size, Hkv, D] with free strides of page, row and
+// head.  Row r of sequence b lies in page block_table[b][r / page_size] at row
+// r % page_size.  Lengths and starts are device data, so a call needs no
+// synchronisation and can be captured and replayed with new values; a value out of
+// range is brought into range, and RW_STATUS_BAD_SLOT is reported.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "host_util.h"
+
+namespace rw {
+namespace paged {
+
+struct Pool {
+  const uint8_t* k;
+  const uint8_t* v;
+  long long k_sp, k_sl, k_sh, v_sp, v_sl, v_sh;  // byte strides: page, row, head
+  int num_pages, page_shift, Hkv, B, width;
+  const int* table;
+  long long table_stride;
+  const int* q_starts;
+  const int* kv_lens;
+};
+
+__device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }
+
+// Tokens [s0, s0 + lq) and cached rows of a sequence, within the call's T tokens and
+// the table's width.
+struct Seq {
+  int s0, lq, kv;
+};
+
+__device__ __forceinline__ Seq load_seq(const Pool& p, int b, int T, int* status) {
+  const int a = __ldg(p.q_starts + b), e = __ldg(p.q_starts + b + 1), n = __ldg(p.kv_lens + b);
+  Seq s;
+  s.s0 = clampi(a, 0, T);
+  s.lq = clampi(e, s.s0, T) - s.s0;
+  s.kv = (int)min((long long)max(n, 0), (long long)p.width << p.page_shift);
+  if (s.s0 != a || s.s0 + s.lq != e || s.kv != n) report_status(status, RW_STATUS_BAD_SLOT);
+  return s;
+}
+
+// Page of a sequence's row; a page outside the pool becomes page 0 (its rows are
+// then wrong, and said to be) so that no address leaves the pool.
+__device__ __forceinline__ int page_of(const Pool& p, int b, int row, int* status) {
+  const int pg = __ldg(p.table + b * p.table_stride + (row >> p.page_shift));
+  if ((unsigned)pg >= (unsigned)p.num_pages) {
+    report_status(status, RW_STATUS_BAD_SLOT);
+    return 0;
+  }
+  return pg;
+}
+
+// The two 16-bit types.  Values are widened to fp32 exactly and rounded once, to
+// nearest, when they are stored.
+template <bool HALF>
+struct Num;
+
+template <>
+struct Num<false> {
+  static __device__ __forceinline__ float2 wide(uint32_t v) { return make_float2(bf16_lo(v), bf16_hi(v)); }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
+};
+
+template <>
+struct Num<true> {
+  static __device__ __forceinline__ float2 wide(uint32_t v) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&v));
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+  }
+};
+
+// Host: checks a rw_paged_t and makes the kernels' form of it.  RW_OK, or what is wrong.
+inline int make_pool(const rw_paged_t* a, Pool* p) {
+  if (!a) return RW_ERR_INVALID_ARG;
+  if ((a->D != 64 && a->D != 128) || (a->dtype != RW_DTYPE_BF16 && a->dtype != RW_DTYPE_FP16))
+    return RW_ERR_UNSUPPORTED;
+  if (!a->k || !a->v || !a->block_table || !a->kv_lens || !aligned16(a->k) || !aligned16(a->v))
+    return RW_ERR_INVALID_ARG;
+  if (a->num_pages < 1 || a->Hkv < 1 || a->Hkv > 65535 || a->B < 0 || a->B > 65535 || a->table_width < 0 ||
+      a->table_stride < a->table_width)
+    return RW_ERR_INVALID_ARG;
+  if (a->page_size < 8 || a->page_size > (1 << 20) || (a->page_size & (a->page_size - 1))) return RW_ERR_UNSUPPORTED;
+  // rows are counted in 32 bits, with room for a tile behind the last one
+  if ((long long)a->table_width * a->page_size > (1ll << 30)) return RW_ERR_CAPACITY;
+  const long long st[6] = {a->k_sp, a->k_sl, a->k_sh, a->v_sp, a->v_sl, a->v_sh};
+  for (long long s : st)
+    if (!stride_ok(s)) return RW_ERR_INVALID_ARG;
+  p->k = static_cast<const uint8_t*>(a->k);
+  p->v = static_cast<const uint8_t*>(a->v);
+  p->k_sp = 2 * a->k_sp; p->k_sl = 2 * a->k_sl; p->k_sh = 2 * a->k_sh;
+  p->v_sp = 2 * a->v_sp; p->v_sl = 2 * a->v_sl; p->v_sh = 2 * a->v_sh;
+  p->num_pages = a->num_pages;
+  p->page_shift = __builtin_ctz((unsigned)a->page_size);
+  p->Hkv = a->Hkv;
+  p->B = a->B;
+  p->width = a->table_width;
+  p->table = a->block_table;
+  p->table_stride = a->table_stride;
+  p->q_starts = a->q_starts;
+  p->kv_lens = a->kv_lens;
+  return RW_OK;
+}
+
+}  // namespace paged
+}  // namespace rw

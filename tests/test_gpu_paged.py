@@ -1,0 +1,484 @@
+"""The paged-cache operators on the GPU against their definitions in 64 bits.
+
+Error bounds (all relative to sums of magnitudes that the oracle gives):
+  a score is a sum of D products, exact in fp32, added in fp32: off by at most ds = (D + 2) 2^-24 * sum |q_d k_d| scale;
+  a weight exp(s - m) is off by ds and by the exponential's 2^-22, relative; so is the total l, whose n terms add n 2^-24;
+  the weights enter the second product rounded to the 16-bit type (half a step, eps / 2 of each), the output is rounded once more.
+"""
+import math
+
+import pytest
+import torch
+
+from oracle import paged as op
+
+pytestmark = pytest.mark.gpu
+BF, FP = torch.bfloat16, torch.float16
+
+
+def _status_clean():
+    from reworld_b200 import _native
+    _native.check_status()
+
+
+def _cache(cuda, lens, page, hkv, D, dtype, seed=0, layout="rows", spare=3, width=None, fill=None):
+    """Pools in which every row that no sequence has holds NaN, and a shuffled block table."""
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    need = [-(-n // page) for n in lens]
+    width = max(need + [1]) if width is None else width
+    total = sum(need) + spare
+    shape = (total, page, hkv, D) if layout == "rows" else (total, hkv, page, D)
+
+    def pool():
+        t = torch.full(shape, float("nan"), dtype=dtype, device=cuda)
+        return t if layout == "rows" else t.transpose(1, 2)
+
+    k, v = pool(), pool()
+    order = torch.randperm(total, generator=g, device=cuda).tolist()
+    table = torch.zeros(len(lens), width, dtype=torch.int32)
+    for b, n in enumerate(lens):
+        for i in range(need[b]):
+            pg = order.pop()
+            table[b, i] = pg
+            rows = min(page, n - i * page)
+            k[pg, :rows] = torch.randn(rows, hkv, D, generator=g, device=cuda).to(dtype)
+            v[pg, :rows] = torch.randn(rows, hkv, D, generator=g, device=cuda).to(dtype)
+    return k, v, table.to(cuda), torch.tensor(lens, dtype=torch.int32, device=cuda), g
+
+
+def _starts(cuda, lqs):
+    s = [0]
+    for n in lqs:
+        s.append(s[-1] + n)
+    return torch.tensor(s, dtype=torch.int32, device=cuda)
+
+
+def _check(out, lse, sums, want, dtype, D, n, before=0.0):
+    o, ls, sm, wv, qk = want
+    half = torch.finfo(dtype).eps / 2
+    ds = (D + 2) * 2.0 ** -24 * qk
+    rel = 2 * (ds + 2.0 ** -22 + n * 2.0 ** -24)
+    # one more half step of the smallest subnormal where fp16 weights or outputs fall below the normal range
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    tol = (half + rel) * wv + half * (o.abs() + (half + rel) * wv) + tiny * (1 + n)
+    bad = (out.double() - o).abs() > tol
+    assert not bad.any(), ((out.double() - o).abs() - tol).max().item()
+    assert torch.isfinite(out.float()).all()
+    if lse is not None:
+        fin = torch.isfinite(ls)
+        assert torch.equal(fin, torch.isfinite(lse)) and (lse[~fin] == -math.inf).all()
+        err = (lse.double() - ls)[fin].abs()
+        assert (err <= rel + 2.0 ** -22 * (1 + ls[fin].abs())).all(), err.max().item()
+    if sums is not None:
+        # a row's weights are taken against its rounded maximum or total: 2^-22 of their size
+        top = ls[torch.isfinite(ls)].abs().max().item() if torch.isfinite(ls).any() else 0.0
+        r = rel + 2.0 ** -22 * (2 + 2 * top) + n * 2.0 ** -24
+        err = (sums.double() - before - sm).abs()
+        assert (err <= r * sm + 2.0 ** -23 * (abs(before) + sm) + 1e-37).all(), err.max().item()
+
+
+def _run(cuda, lqs, lens, hq, hkv, D, dtype, page=16, causal=True, layout="rows", max_q=None, seed=0, sums=True,
+         width=None, tail=2):
+    from reworld_b200 import paged_attention
+    k, v, table, kv, g = _cache(cuda, lens, page, hkv, D, dtype, seed, layout, width=width)
+    starts = _starts(cuda, lqs)
+    T = sum(lqs) + tail
+    q = (1.5 * torch.randn(T, hq, D, generator=g, device=cuda)).to(dtype)
+    scale = 1 / math.sqrt(D)
+    out = torch.full_like(q, 7.0)
+    w = torch.full((len(lens), hkv, table.shape[1] * page + 5), 0.5, device=cuda) if sums else None
+    got, lse = paged_attention(q, k, v, table, starts, kv, max_q_len=max(lqs) if max_q is None else max_q,
+                               causal=causal, weight_sums=w, return_lse=True, out=out)
+    torch.cuda.synchronize()
+    _status_clean()
+    assert got is out
+    n = T - tail
+    assert (out[n:] == 7.0).all()                       # behind the last sequence
+    want = op.attention(q[:n], k, v, table, starts, kv, causal, scale)
+    _check(out[:n], lse[:n], w[..., :-5] if sums else None, want, dtype, D, max(lens + [1]), 0.5)
+    if sums:
+        assert (w[..., -5:] == 0.5).all()
+    # the same call again gives the same bits
+    if sums:
+        w2 = torch.full_like(w, 0.5)
+        again, lse2 = paged_attention(q, k, v, table, starts, kv, max_q_len=max(lqs) if max_q is None else max_q,
+                                      causal=causal, weight_sums=w2, return_lse=True)
+        assert torch.equal(again[:n], out[:n]) and torch.equal(lse2[:n], lse[:n]) and torch.equal(w, w2)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("hq,hkv,D", [(8, 2, 128), (4, 4, 64), (7, 1, 128), (15, 5, 64), (16, 1, 128)])
+def test_single_tokens(cuda, dtype, hq, hkv, D):
+    _run(cuda, [1] * 6, [1, 17, 64, 65, 777, 3000], hq, hkv, D, dtype)
+
+
+@pytest.mark.parametrize("page,layout", [(8, "rows"), (32, "heads"), (64, "rows"), (128, "heads"), (256, "rows")])
+def test_single_tokens_pages_and_layouts(cuda, page, layout):
+    _run(cuda, [1, 1, 1], [5, 600, 257], 8, 2, 128, BF, page=page, layout=layout)
+
+
+def test_single_tokens_with_empty_sequences(cuda):
+    """No new token, no cached row, both; the block table wider than any sequence."""
+    _run(cuda, [1, 0, 1, 0, 1], [40, 30, 0, 0, 129], 8, 2, 128, BF, width=40)
+
+
+@pytest.mark.parametrize("batch", [1, 2, 150, 700])
+def test_single_tokens_batches(cuda, batch):
+    _run(cuda, [1] * batch, [(37 * i) % 211 + 1 for i in range(batch)], 4, 2, 64, FP, sums=batch < 200)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lqs,lens,hq,hkv,D", [
+    ([2, 5, 16], [2, 70, 400], 8, 2, 128),               # few tokens
+    ([130, 1, 257], [130, 300, 1000], 4, 2, 128),        # chunks over what is cached, one token among them
+    ([65, 40, 129], [65, 40, 129], 3, 1, 64),            # prompts, groups of three
+    ([64, 128, 100], [64, 256, 228], 6, 6, 128),         # whole tiles, a head of its own each
+    ([50], [700], 24, 1, 64),                            # a group of 24
+    ([33, 20], [33, 300], 40, 1, 128),                   # a group of 40
+    ([9, 3], [300, 20], 128, 1, 64),                     # the largest group
+])
+def test_chunks(cuda, dtype, causal, lqs, lens, hq, hkv, D):
+    _run(cuda, lqs, lens, hq, hkv, D, dtype, causal=causal)
+
+
+@pytest.mark.parametrize("page,layout", [(8, "heads"), (16, "heads"), (32, "rows"), (64, "heads"), (128, "rows"),
+                                         (256, "heads")])
+def test_chunks_pages_and_layouts(cuda, page, layout):
+    _run(cuda, [150, 31], [333, 500], 4, 2, 128, BF, page=page, layout=layout)
+
+
+def test_chunk_rows_that_see_nothing(cuda):
+    """More new tokens than rows: the first ones see none; sequences without rows or tokens."""
+    _run(cuda, [40, 10, 0, 200], [25, 0, 100, 60], 4, 2, 128, BF)
+    _run(cuda, [3, 2], [1, 0], 4, 2, 64, FP)
+
+
+def test_max_q_len_is_a_bound_and_may_be_left_out(cuda):
+    _run(cuda, [3, 90], [60, 200], 4, 2, 128, BF, max_q=5000)
+    from reworld_b200 import paged_attention
+    k, v, table, kv, g = _cache(cuda, [60, 200], 16, 2, 128, BF)
+    q = torch.randn(93, 4, 128, generator=g, device=cuda).to(BF)
+    s = _starts(cuda, [3, 90])
+    a = paged_attention(q, k, v, table, s, kv)
+    b = paged_attention(q, k, v, table, s, kv, max_q_len=93)
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("lq", [1, 40])
+def test_large_and_infinite_scores(cuda, lq):
+    """Scores far apart (one weight is 1), masked rows of the largest finite values."""
+    from reworld_b200 import paged_attention
+    k, v, table, kv, g = _cache(cuda, [300], 16, 2, 128, BF, 3)
+    pages = table[0].tolist()
+    big = torch.finfo(BF).max
+    k[pages[-1], 300 % 16:], v[pages[-1], 300 % 16:] = big, -big     # behind the last row
+    q = (100 * torch.randn(lq, 4, 128, generator=g, device=cuda)).to(BF)
+    s = _starts(cuda, [lq])
+    out, lse = paged_attention(q, k, v, table, s, kv, max_q_len=lq, return_lse=True)
+    want = op.attention(q, k, v, table, s, kv, True, 1 / math.sqrt(128))
+    _check(out, lse, None, want, BF, 128, 300)
+    assert torch.isfinite(out.float()).all()
+
+
+def test_strided_inputs_and_output(cuda):
+    from reworld_b200 import paged_attention
+    k, v, table, kv, g = _cache(cuda, [100, 50], 16, 2, 128, BF, 4)
+    wide = torch.randn(20, 12, 128, generator=g, device=cuda).to(BF)
+    q = wide[:, 2:6]                                     # heads of a packed row
+    s = _starts(cuda, [12, 8])
+    odd = torch.randn(20 * 4 * 128 + 1, generator=g, device=cuda).to(BF)[1:].view(20, 4, 128)   # off by 2 bytes
+    out = torch.zeros(20, 9, 128, dtype=BF, device=cuda)[:, 3:7]
+    got = paged_attention(q, k, v, table[:, :], s, kv, out=out)
+    assert torch.equal(got, paged_attention(q.contiguous(), k, v, table, s, kv))
+    assert torch.equal(paged_attention(odd, k, v, table, s, kv), paged_attention(odd.clone(), k, v, table, s, kv))
+
+
+def test_another_stream_and_two_graphs(cuda):
+    """Calls on two streams at once, and two captured graphs replayed at once with new lengths."""
+    from reworld_b200 import paged_attention
+    lens = [3000, 4000]
+    k, v, table, kv, g = _cache(cuda, lens, 16, 2, 128, BF, 5)
+    s = _starts(cuda, [1, 1])
+    qs = [torch.randn(2, 8, 128, generator=g, device=cuda).to(BF) for _ in range(2)]
+    ws = [torch.zeros(2, 2, table.shape[1] * 16, device=cuda) for _ in range(2)]
+    ref = [paged_attention(q, k, v, table, s, kv, max_q_len=1) for q in qs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = [torch.zeros_like(qs[0]) for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                paged_attention(qs[i], k, v, table, s, kv, max_q_len=1, out=outs[i])
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, r) for o, r in zip(outs, ref))
+    graphs, cap = [], []
+    for i in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            o = paged_attention(qs[i], k, v, table, s, kv, max_q_len=1, weight_sums=ws[i])
+        graphs.append(gr)
+        cap.append(o)
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, r) for o, r in zip(cap, ref))
+    kv.copy_(torch.tensor([70, 1], dtype=torch.int32))   # other lengths, same graph
+    new = [paged_attention(q, k, v, table, s, kv, max_q_len=1) for q in qs]
+    for i in range(2):
+        graphs[i].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, r) for o, r in zip(cap, new))
+    _status_clean()
+
+
+def test_bad_pages_and_lengths_are_reported_and_stay_in_bounds(cuda):
+    from reworld_b200 import _native, paged_attention, paged_rotary_store
+    k, v, table, kv, g = _cache(cuda, [60], 16, 2, 128, BF, 6)
+    q = torch.randn(1, 4, 128, generator=g, device=cuda).to(BF)
+    s = _starts(cuda, [1])
+    for bad_table, bad_kv, bad_s in ((table + 100000, kv, s), (table - 100000, kv, s), (table, kv + 100000, s),
+                                     (table, kv - 100000, s), (table, kv, s + 50), (table, kv, -s)):
+        paged_attention(q, k, v, bad_table, bad_s, bad_kv, max_q_len=1)
+        with pytest.raises(RuntimeError):
+            _native.check_status(cuda)
+        paged_rotary_store(q[:, :2], q[:, 2:], k.clone(), v.clone(), bad_table, bad_s, bad_kv)
+        torch.cuda.synchronize()
+        try:
+            _native.check_status(cuda)                   # a start behind the tokens just leaves no token
+        except RuntimeError:
+            pass
+    _status_clean()
+
+
+# ------------------------------------------------------------------ rotary positions and the page write
+
+def _freq(rot, theta=10000.0):
+    return theta ** (-torch.arange(0, rot, 2, dtype=torch.float64) / rot)
+
+
+def _rot_tol(y, dtype):
+    """One rounding to the type; two products and a sum in fp32 of values the size of the pair, with a table off by 2^-25."""
+    return torch.finfo(dtype).eps / 2 * y.abs() + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("D,rot", [(128, 128), (128, 64), (128, 48), (64, 64), (64, 16)])
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_rotary(cuda, dtype, D, rot, interleaved):
+    from reworld_b200 import rotary, rotary_table
+    g = torch.Generator(device=cuda).manual_seed(1)
+    x = torch.randn(37, 5, D, generator=g, device=cuda).to(dtype)
+    pos = torch.randint(0, 100000, (37,), generator=g, device=cuda, dtype=torch.int32)
+    tab = rotary_table(100000, rot, device=cuda)
+    y = rotary(x, tab, pos, interleaved)
+    want = op.rotary(x, _freq(rot).to(cuda), pos, rot, interleaved)
+    pair = 4 * x.double().abs().max() * 2.0 ** -24
+    assert ((y.double() - want).abs() <= _rot_tol(want, dtype) * 1.0001 + pair).all()
+    assert torch.equal(y[..., rot:], x[..., rot:])
+    z = x.clone()
+    assert rotary(z, tab, pos, interleaved, out=z) is z and torch.equal(z, y)      # in place
+    packed = torch.zeros(37, 11, D, dtype=dtype, device=cuda)
+    packed[:, 3:8] = x
+    rotary(packed[:, 3:8], tab, pos, interleaved, out=packed[:, 3:8])
+    assert torch.equal(packed[:, 3:8], y) and not packed[:, :3].any() and not packed[:, 8:].any()
+    _status_clean()
+
+
+def test_rotary_position_outside_the_table(cuda):
+    from reworld_b200 import _native, rotary, rotary_table
+    tab = rotary_table(10, 64, device=cuda)
+    x = torch.randn(2, 1, 64, device=cuda).to(BF)
+    rotary(x, tab, torch.tensor([3, 10], dtype=torch.int32, device=cuda))
+    with pytest.raises(RuntimeError):
+        _native.check_status(cuda)
+    rotary(x, tab, torch.tensor([-1, 9], dtype=torch.int32, device=cuda))
+    with pytest.raises(RuntimeError):
+        _native.check_status(cuda)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("lqs,lens,hq,hkv,D,page,layout", [
+    ([1] * 5, [1, 16, 17, 100, 33], 8, 2, 128, 16, "rows"),
+    ([1, 0, 40, 7], [9, 30, 40, 300], 6, 3, 64, 32, "heads"),
+    ([700, 1500], [900, 1500], 24, 24, 128, 64, "rows"),
+    ([2, 3], [20, 30], 0, 1, 128, 8, "rows"),
+])
+@pytest.mark.parametrize("with_positions", [True, False])
+def test_store(cuda, dtype, lqs, lens, hq, hkv, D, page, layout, with_positions):
+    from reworld_b200 import paged_rotary_store, rotary_table
+    kp, vp, table, kv, g = _cache(cuda, lens, page, hkv, D, dtype, 7, layout)
+    k0, v0 = kp.clone(), vp.clone()
+    T = sum(lqs) + 3                                     # three tokens behind the last sequence
+    k, v = (torch.randn(T, hkv, D, generator=g, device=cuda).to(dtype) for _ in range(2))
+    q = torch.randn(T, hq, D, generator=g, device=cuda).to(dtype) if hq else None
+    q_out = torch.full_like(q, 9.0) if hq else None
+    rows = torch.tensor([n - lq + i for lq, n in zip(lqs, lens) for i in range(lq)] + [0] * 3, device=cuda)
+    pos = (rows + 1000).to(torch.int32) if with_positions else None
+    tab = rotary_table(4000, D, device=cuda)
+    got = paged_rotary_store(k, v, kp, vp, table, _starts(cuda, lqs), kv, table=tab, positions=pos, q=q, q_out=q_out)
+    torch.cuda.synchronize()
+    _status_clean()
+    n = T - 3
+    at = rows + 1000 if with_positions else rows
+    wk = op.rotary(k, _freq(D).to(cuda), at, D, False)[:n]
+    seq = torch.tensor([b for b, lq in enumerate(lqs) for _ in range(lq)], device=cuda)
+    r = rows[:n]
+    pg, slot = table.long()[seq, r // page], r % page
+    pair = 4 * 6.0 * 2.0 ** -24
+    assert ((kp[pg, slot].double() - wk).abs() <= _rot_tol(wk, dtype) * 1.0001 + pair).all()
+    assert torch.equal(vp[pg, slot], v[:n])
+    k0[pg, slot], v0[pg, slot] = kp[pg, slot], vp[pg, slot]         # every other row as it was
+    assert torch.equal(torch.nan_to_num(kp, 77.0), torch.nan_to_num(k0, 77.0))
+    assert torch.equal(torch.nan_to_num(vp, 77.0), torch.nan_to_num(v0, 77.0))
+    if hq:
+        wq = op.rotary(q, _freq(D).to(cuda), at, D, False)[:n]
+        assert got is q_out and (q_out[n:] == 9.0).all()
+        assert ((q_out[:n].double() - wq).abs() <= _rot_tol(wq, dtype) * 1.0001 + pair).all()
+
+
+def test_store_without_rotation_and_packed_projections(cuda):
+    """Slices of one packed q|k|v projection, rotated in place where they are."""
+    from reworld_b200 import paged_rotary_store, rotary, rotary_table
+    kp, vp, table, kv, g = _cache(cuda, [50, 20], 16, 2, 64, BF, 8)
+    qkv = torch.randn(15, 8, 64, generator=g, device=cuda).to(BF)
+    ref = qkv.clone()
+    q, k, v = qkv[:, :4], qkv[:, 4:6], qkv[:, 6:]
+    s = _starts(cuda, [10, 5])
+    assert paged_rotary_store(k, v, kp, vp, table, s, kv) is None
+    rows = torch.cat([torch.arange(40, 50), torch.arange(15, 20)]).to(cuda)
+    seq = torch.tensor([0] * 10 + [1] * 5, device=cuda)
+    at = (table.long()[seq, rows // 16], rows % 16)
+    assert torch.equal(kp[at], k) and torch.equal(vp[at], v)
+    tab = rotary_table(64, 32, device=cuda)
+    paged_rotary_store(k, v, kp, vp, table, s, kv, table=tab, q=q, q_out=q, interleaved=True)
+    pos = rows.to(torch.int32)
+    assert torch.equal(q, rotary(ref[:, :4].contiguous(), tab, pos, True))
+    assert torch.equal(kp[at], rotary(ref[:, 4:6].contiguous(), tab, pos, True)) and torch.equal(qkv[:, 4:], ref[:, 4:])
+    _status_clean()
+
+
+# ------------------------------------------------------------------ eviction
+
+def _evict_case(cuda, lens, page, hkv, D, keep, sink, recent, dtype=BF, sums=None, layout="rows", seed=0):
+    from reworld_b200 import paged_evict
+    k, v, table, kv, g = _cache(cuda, lens, page, hkv, D, dtype, seed, layout, spare=len(lens) * -(-keep // page) + 2)
+    cap = max(table.shape[1] * page, keep) + 3
+    w = torch.exp(torch.randn(len(lens), hkv, cap, generator=g, device=cuda)) if sums is None else sums(cap, g)
+    used = set(table.flatten().tolist()) if max(lens) else set()
+    free = [i for i in range(k.shape[0]) if i not in used]
+    dw = -(-keep // page)
+    dst = torch.tensor(free[:len(lens) * dw], dtype=torch.int32, device=cuda).view(len(lens), dw)
+    k0, v0, w0 = k.clone(), v.clone(), w.clone()
+    kept, new_lens, new = paged_evict(k, v, table, kv, w, keep, dst, n_sink=sink, n_recent=recent)
+    torch.cuda.synchronize()
+    _status_clean()
+    assert torch.equal(torch.nan_to_num(w, -1.0), torch.nan_to_num(w0, -1.0))
+    for b, n in enumerate(lens):
+        assert int(new_lens[b]) == min(n, keep)
+        for h in range(hkv):
+            want = op.evict(w0[b, h].cpu(), n, keep, sink, recent)
+            m = len(want)
+            assert kept[b, h].tolist() == want + [-1] * (keep - m)
+            at = torch.tensor(want, dtype=torch.int64, device=cuda)
+            assert torch.equal(torch.nan_to_num(new[b, h, :m], -1.0), torch.nan_to_num(w0[b, h, at], -1.0))
+            assert not new[b, h, m:].any()
+            j = torch.arange(m, device=cuda)
+            for pool, old in ((k, k0), (v, v0)):
+                src = old[table.long()[b, at // page], at % page, h]
+                assert torch.equal(pool[dst.long()[b, j // page], j % page, h], src)
+                pool[dst.long()[b, j // page], j % page, h] = old[dst.long()[b, j // page], j % page, h]
+    assert torch.equal(torch.nan_to_num(k, 77.0), torch.nan_to_num(k0, 77.0))       # nothing else was written
+    assert torch.equal(torch.nan_to_num(v, 77.0), torch.nan_to_num(v0, 77.0))
+
+
+@pytest.mark.parametrize("lens,page,hkv,D,keep,sink,recent", [
+    ([1000, 300, 512], 16, 2, 128, 512, 4, 100),
+    ([40, 41, 39, 0, 1], 8, 3, 64, 40, 0, 0),
+    ([5000, 9000], 64, 1, 128, 2049, 1, 2048),           # nothing left to choose
+    ([100], 16, 2, 64, 1, 0, 0),
+    ([100], 16, 2, 64, 1, 1, 0),
+    ([100, 77], 32, 2, 64, 50, 0, 50),
+    ([8192, 8193, 4096], 256, 2, 64, 4095, 3, 5),
+])
+@pytest.mark.parametrize("layout", ["rows", "heads"])
+def test_evict(cuda, lens, page, hkv, D, keep, sink, recent, layout):
+    _evict_case(cuda, lens, page, hkv, D, keep, sink, recent, layout=layout)
+
+
+@pytest.mark.parametrize("kind", ["equal", "zeros", "few values", "signs and specials", "close"])
+def test_evict_ties_and_special_sums(cuda, kind):
+    def sums(cap, g):
+        x = torch.randn(2, 2, cap, generator=g, device=cuda)
+        if kind == "equal":
+            return torch.ones_like(x)
+        if kind == "zeros":
+            return torch.where(x > 0, 0.0, -0.0)         # one value, whatever its sign
+        if kind == "few values":
+            return torch.round(x)+0.0
+        if kind == "close":
+            return 1 + (x * 4).round() * 2.0 ** -23      # differ in the last bits only
+        x[..., ::7] = float("inf")
+        x[..., 1::7] = -float("inf")
+        x[..., 2::7] = float("nan")
+        return x
+    _evict_case(cuda, [5000, 700], 16, 2, 64, 600, 2, 10, sums=sums)
+
+
+# ------------------------------------------------------------------ together
+
+@pytest.mark.parametrize("D,dtype", [(128, BF), (64, FP)])
+def test_sessions_prompt_decode_evict_decode(cuda, D, dtype):
+    """Prompts, decoding with weights kept, eviction to fresh pages, decoding from there: the caches
+    hold what a dense restatement holds, and each attention matches the oracle over those rows."""
+    from reworld_b200 import paged_attention, paged_evict, paged_rotary_store, rotary_table
+    g = torch.Generator(device=cuda).manual_seed(11)
+    B, hq, hkv, page, width = 2, 4, 2, 16, 12
+    kp, vp = (torch.full((60, page, hkv, D), float("nan"), dtype=dtype, device=cuda) for _ in range(2))
+    table = torch.arange(B * width, dtype=torch.int32, device=cuda).view(B, width)
+    sums = torch.zeros(B, hkv, width * page, device=cuda)
+    tab = rotary_table(512, D, scaling=("linear", 2.0), device=cuda)
+    pos = [0, 0]                                         # tokens that a session has had
+    lens = [0, 0]
+    total = torch.zeros(B, hkv, width * page, dtype=torch.float64, device=cuda)
+
+    def step(lqs):
+        T = sum(lqs)
+        q, k, v = ((torch.randn(T, h, D, generator=g, device=cuda)).to(dtype) for h in (hq, hkv, hkv))
+        for b in range(B):
+            lens[b] += lqs[b]
+        kv = torch.tensor(lens, dtype=torch.int32, device=cuda)
+        s = _starts(cuda, lqs)
+        at = torch.tensor([pos[b] + i for b in range(B) for i in range(lqs[b])], dtype=torch.int32, device=cuda)
+        qr = paged_rotary_store(k, v, kp, vp, table, s, kv, table=tab, positions=at, q=q)
+        out, lse = paged_attention(qr, kp, vp, table, s, kv, max_q_len=max(lqs), weight_sums=sums, return_lse=True)
+        for b in range(B):
+            pos[b] += lqs[b]
+        want = op.attention(qr, kp, vp, table, s, kv, True, 1 / math.sqrt(D))
+        _check(out, lse, None, want, dtype, D, max(lens))
+        total.add_(want[2])
+        assert (sums.double() - total).abs().max() <= 1e-4 * max(1.0, float(total.max()))
+
+    step([70, 41])
+    for _ in range(3):
+        step([1, 1])
+    kv = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    dst = torch.arange(30, 30 + B * 3, dtype=torch.int32, device=cuda).view(B, 3)
+    kept, new_lens, new_sums = paged_evict(kp, vp, table, kv, sums, 48, dst, n_sink=2, n_recent=8)
+    assert new_lens.tolist() == [48, 44]
+    for b in range(B):
+        for h in range(hkv):
+            assert kept[b, h].tolist() == (lambda w: w + [-1] * (48 - len(w)))(op.evict(sums[b, h].cpu(), lens[b], 48, 2, 8))
+    ks = kept.clamp_min(0).long()
+    total = torch.where(torch.arange(width * page, device=cuda) < new_lens.view(B, 1, 1),
+                        torch.nn.functional.pad(total.gather(2, ks), (0, width * page - 48)), 0.0)
+    sums.copy_(new_sums)
+    table = torch.cat([dst, torch.arange(40, 40 + 4, dtype=torch.int32, device=cuda).view(B, 2)], dim=1)
+    table = torch.nn.functional.pad(table, (0, width - 5))
+    lens[:] = new_lens.tolist()
+    for lqs in ([1, 1], [20, 1], [1, 5]):
+        step(lqs)
+    _status_clean()
