@@ -1,0 +1,1123 @@
+// Attention of chunks of new tokens over a paged cache on the tensor cores: o =
+// softmax(q k^T * scale) v for a ragged batch, with shared key heads and causal order.
+//
+// A unit is the 256 rows (head dim 128) or 128 rows (head dim 64) of one sequence that
+// share a key head: the G query heads of the group by consecutive tokens, row = token *
+// G + head, so that a key tile is used by all heads that share it.  With G not a power of
+// two a tile of 128 holds floor(128 / G) * G rows.
+//
+// Head dim 128 runs on CTA pairs as attn_pair.cu does (2-SM tcgen05.mma, every CTA loads
+// half of each key and value tile): one CTA alone would need 64 KB of k and v for every
+// 128 x 128 scores, about twice what L2 delivers to all SMs at that rate.  With head dim
+// 64 the tiles are half as large and the time a tile takes is the same (the 128 x 128
+// exponentials), so one CTA reads what a pair's CTA does there; it runs alone.
+//   TMEM columns  O [0, D)  S0 [128, 256)  S1 [256, 384)  S2 [384, 512)
+// Key tile j lands in S buffer j mod 3 and its weights P (16-bit) overwrite the buffer's
+// first 64 columns; the tensor pipe runs QK up to three tiles ahead of the softmax.
+// Warps: two softmax warpgroups (tiles j even / odd, a row a thread), warp 8 loads,
+// warp 9 issues the MMAs, warp 10 writes the last value tile, warp 11 plans.
+//
+// Pages: a key tile is gathered by one TMA box a page (and 64 channels), issued by one
+// lane each; page indices are read one tile ahead.  Of the page that a sequence ends in,
+// the rows behind the end may hold anything: keys there are masked by selection, but a
+// weight of 0 times NaN is NaN, so the values of such a tile are not loaded by TMA; warp
+// 10 copies the rows that exist and writes zeros for the others.
+//
+// Work: lengths are device data, so every CTA sums the key tiles of all units itself
+// (a few microseconds' latency, no host, no extra launch).  Pairs first take whole units
+// in waves (pairs at work at the same time then share heads, and k and v come from L2),
+// if the units are about equal; what does not fill a wave, or all of it if they are not,
+// is one sequence of tiles of which every pair takes an equal share, and the parts of
+// units that more than one pair worked on are joined by join_kernel.
+#include "paged.cuh"
+#include "paged_chunk.h"
+
+namespace rw {
+namespace chunk {
+
+using paged::Num;
+using paged::Pool;
+using paged::Seq;
+
+constexpr int BM = 128;                      // rows of a CTA
+constexpr int BN = 128;                      // keys of a tile
+constexpr int NSBUF = 3;
+constexpr int NSTAGE = 4;
+constexpr int HALF_TILE = 16384;             // a CTA's part of a key or value tile
+constexpr int PRE_BYTES = NSBUF * HALF_TILE; // keys of tiles 0-2
+constexpr int STAGE_BYTES = 2 * HALF_TILE;   // stage j: values of tile j, then keys of tile j + 3
+constexpr int NWG = 2;
+constexpr int NUM_THREADS = 128 * (NWG + 1);
+constexpr int WARP_LOAD = 8, WARP_MMA = 9, WARP_TAIL = 10, WARP_PLAN = 11;
+constexpr int SOFTMAX_THREADS = 256;
+constexpr int REG_SOFTMAX = 208, REG_OTHER = 88;
+static_assert(NWG * 128 * REG_SOFTMAX + 128 * REG_OTHER <= NUM_THREADS * 168, "register split exceeds the launch's");
+constexpr float RESCALE_THRESHOLD = 8.0f;    // log2 units
+
+template <int D>
+struct Shape {
+  static constexpr int NCTA = D == 128 ? 2 : 1;
+  static constexpr int Q_BYTES = BM * D * 2;
+  static constexpr int KROWS = BN / NCTA;    // a CTA's keys of a tile
+  static constexpr int SMEM = Q_BYTES + PRE_BYTES + NSTAGE * STAGE_BYTES + 1024;
+  static constexpr long long SLOT_FLOATS = (long long)NCTA * BM * (D + 2);
+};
+
+// What a segment (the key tiles [kv0, kv0 + n) of one unit) needs.
+struct Seg {
+  int n;                 // 0: no more work
+  int kv0, last;         // last: the tile with which the unit ends (kv0 + n - 1 <= last)
+  int slot;              // -1: the whole unit
+  int b, hk, tok0;       // unit's first token within the sequence
+  int s0, lq, kv, keys;  // keys: rows that any token of the unit sees
+};
+
+struct Params {
+  Pool pool;
+  int T, Hq, G, causal;
+  int tpc;               // tokens of a CTA: floor(128 / G)
+  int C;                 // pairs (or CTAs) in the grid
+  float scale_log2;
+  uint8_t* out;
+  long long o_sl, o_sh;  // byte strides
+  float* lse;            // [T, Hq] or null
+  float2* row_ml;        // [T, Hq] (m, 1 / l) for the weight sums, or null
+  float* scratch;        // [2 C] slots
+  int4* header;          // [2 C]: (b + 1 or 0, hk, tok0, unused)
+  int kbox, vbox;        // rows of a TMA box: min(page, keys of a CTA), min(page, 128)
+  int* status;
+};
+
+struct __align__(8) Barriers {
+  uint64_t pre_full, q_full, o_done, drain, v_tail;
+  uint64_t stage_full[NSTAGE], stage_free[NSTAGE];
+  uint64_t s_full[NSBUF], p_ready[NSBUF], m_ready[NSBUF];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+struct Ctx {
+  Barriers* sb;
+  uint32_t peer_abort;
+  bool pair;
+  int* status;
+};
+
+__device__ __forceinline__ bool pwait(uint64_t* bar, uint32_t parity, const Ctx& c, int err) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  for (uint32_t it = 1;; ++it) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((it & 15u) == 0u) {
+      if (*(volatile int*)&c.sb->abort_flag) return false;
+      if (globaltimer_ns() - t0 > RW_WAIT_TIMEOUT_NS) {
+        c.sb->abort_flag = 1;
+        if (c.pair) st_shared_cluster_u32(c.peer_abort, 1u);
+        report_status(c.status, err);
+        return false;
+      }
+    }
+  }
+}
+__device__ __forceinline__ bool pwait_warp(uint64_t* bar, uint32_t parity, const Ctx& c, int err) {
+  return __all_sync(0xffffffffu, pwait(bar, parity, c, err));
+}
+
+// Tiled load into this CTA's shared memory, bytes counted on the barrier at the
+// shared::cluster address `bar` (the even CTA's for a pair).  No multicast.
+template <int NCTA>
+__device__ __forceinline__ void load_4d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2,
+                                        int c3) {
+  if constexpr (NCTA == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0),
+        "r"(c1), "r"(c2), "r"(c3) : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0),
+        "r"(c1), "r"(c2), "r"(c3) : "memory");
+}
+template <int NCTA>
+__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2) {
+  if constexpr (NCTA == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0),
+        "r"(c1), "r"(c2) : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0),
+        "r"(c1), "r"(c2) : "memory");
+}
+template <int NCTA>
+__device__ __forceinline__ void mma_ss_n(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  if constexpr (NCTA == 2) mma_ss_pair(d, a, b, id, acc); else mma_ss(d, a, b, id, acc);
+}
+template <int NCTA>
+__device__ __forceinline__ void mma_ts_n(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  if constexpr (NCTA == 2) mma_ts_pair(d, a, b, id, acc); else mma_ts(d, a, b, id, acc);
+}
+template <int NCTA>
+__device__ __forceinline__ void commit_n(uint64_t* bar) {  // arrives on every CTA's barrier
+  if constexpr (NCTA == 2) tc_commit_pair_mc(bar, 0x3); else tc_commit(bar);
+}
+
+template <bool HALF>
+constexpr uint32_t idesc(int M, int N, int b_mn) {
+  return HALF ? (idesc_bf16_f32(M, N, 0, b_mn) & ~((1u << 7) | (1u << 10))) : idesc_bf16_f32(M, N, 0, b_mn);
+}
+
+// ---------------------------------------------------------------- work
+__device__ __forceinline__ int units_of(const Params& p, const Seq& s, int upt) { return (s.lq + upt - 1) / upt; }
+
+// Key tiles of unit rt of a sequence (at least one: rows that see nothing are written too).
+__device__ __forceinline__ int tiles_of(const Params& p, const Seq& s, int rt, int upt, int* keys) {
+  const int end = min(s.lq, (rt + 1) * upt);
+  const int k = p.causal ? max(0, s.kv - s.lq + end) : s.kv;
+  *keys = k;
+  return max(1, (k + BN - 1) / BN);
+}
+
+struct Plan {
+  long long tiles[MAX_BATCH + 1];  // key tiles of the units of the sequences before each
+  int units[MAX_BATCH + 1];        // units before each
+  int longest;
+};
+
+// Filled by all threads; the caller synchronises.  tiles[b + 1], units[b + 1] first hold
+// the sequence's own numbers, then warp 0 sums them up.
+__device__ __forceinline__ void plan_own(const Params& p, Plan& pl, int upt, int warp, int lane, int nwarps,
+                                         bool report) {
+  for (int b = warp; b < p.pool.B; b += nwarps) {
+    const Seq s = paged::load_seq(p.pool, b, p.T, report && lane == 0 ? p.status : nullptr);
+    const int nu = units_of(p, s, upt);
+    long long sum = 0;
+    int top = 0, keys;
+    for (int rt = lane; rt < nu; rt += 32) {
+      const int n = tiles_of(p, s, rt, upt, &keys);
+      sum += n;
+      top = max(top, n);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+    if (lane == 0) {
+      pl.tiles[b + 1] = sum * p.pool.Hkv;
+      pl.units[b + 1] = nu * p.pool.Hkv;
+      atomicMax(&pl.longest, top);
+    }
+  }
+}
+__device__ __forceinline__ void plan_sum(const Params& p, Plan& pl, int lane) {
+  long long ct = 0;
+  int cu = 0;
+  for (int b0 = 0; b0 < p.pool.B; b0 += 32) {
+    const int b = b0 + lane;
+    long long t = b < p.pool.B ? pl.tiles[b + 1] : 0;
+    int u = b < p.pool.B ? pl.units[b + 1] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, t, o);
+      const int z = __shfl_up_sync(0xffffffffu, u, o);
+      if (lane >= o) { t += y; u += z; }
+    }
+    if (b < p.pool.B) {
+      pl.tiles[b + 1] = ct + t;
+      pl.units[b + 1] = cu + u;
+    }
+    ct += __shfl_sync(0xffffffffu, t, 31);
+    cu += __shfl_sync(0xffffffffu, u, 31);
+  }
+  if (lane == 0) { pl.tiles[0] = 0; pl.units[0] = 0; }
+  __syncwarp();
+}
+
+// Where a walker over the units in the order (sequence, head, row tile) stands.
+struct Walk {
+  int b, hk, rt, n, nu, keys;
+  Seq s;
+};
+
+__device__ __forceinline__ void enter(const Params& p, Walk& w, int upt) {
+  w.s = paged::load_seq(p.pool, w.b, p.T, nullptr);
+  w.nu = units_of(p, w.s, upt);
+}
+
+// Whole warp: the unit with index u.
+__device__ __forceinline__ Walk walk_to_unit(const Params& p, const Plan& pl, int u, int upt) {
+  Walk w;
+  int lo = 0, hi = p.pool.B - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (pl.units[mid] <= u) lo = mid; else hi = mid - 1;
+  }
+  w.b = lo;
+  enter(p, w, upt);
+  const int r = u - pl.units[lo];
+  w.hk = r / w.nu;
+  w.rt = r - w.hk * w.nu;
+  w.n = tiles_of(p, w.s, w.rt, upt, &w.keys);
+  return w;
+}
+// Whole warp: tiles of the units before that one.
+__device__ __forceinline__ long long tiles_before(const Params& p, const Plan& pl, const Walk& w, int upt, int lane) {
+  long long sum = 0, all = (pl.tiles[w.b + 1] - pl.tiles[w.b]) / p.pool.Hkv;
+  int keys;
+  for (int rt = lane; rt < w.rt; rt += 32) sum += tiles_of(p, w.s, rt, upt, &keys);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return pl.tiles[w.b] + all * w.hk + sum;
+}
+// Whole warp: the unit that holds tile t, and the tiles before it.
+__device__ __forceinline__ Walk walk_to_tile(const Params& p, const Plan& pl, long long t, int upt, int lane,
+                                             long long* before) {
+  Walk w;
+  int lo = 0, hi = p.pool.B - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (pl.tiles[mid] <= t) lo = mid; else hi = mid - 1;
+  }
+  w.b = lo;
+  enter(p, w, upt);
+  const long long each = (pl.tiles[lo + 1] - pl.tiles[lo]) / p.pool.Hkv;
+  w.hk = (int)((t - pl.tiles[lo]) / each);
+  long long at = pl.tiles[lo] + each * w.hk;
+  for (int r0 = 0; r0 < w.nu; r0 += 32) {
+    int keys;
+    const int n = r0 + lane < w.nu ? tiles_of(p, w.s, r0 + lane, upt, &keys) : 0;
+    int x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    const unsigned behind = __ballot_sync(0xffffffffu, at + x > t);  // lanes whose unit ends behind t
+    if (behind) {
+      const int f = __ffs(behind) - 1;
+      w.rt = r0 + f;
+      at += __shfl_sync(0xffffffffu, x - n, f);
+      break;
+    }
+    at += __shfl_sync(0xffffffffu, x, 31);
+  }
+  w.n = tiles_of(p, w.s, w.rt, upt, &w.keys);
+  *before = at;
+  return w;
+}
+__device__ __forceinline__ void next_unit(const Params& p, Walk& w, int upt) {
+  if (++w.rt == w.nu) {
+    w.rt = 0;
+    if (++w.hk == p.pool.Hkv) {
+      w.hk = 0;
+      do {
+        ++w.b;
+        enter(p, w, upt);
+      } while (w.nu == 0 && w.b + 1 < p.pool.B);   // there is another unit: the caller has tiles left
+    }
+  }
+  w.n = tiles_of(p, w.s, w.rt, upt, &w.keys);
+}
+
+template <bool HALF, int D>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+    chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Params p) {
+  constexpr int NCTA = Shape<D>::NCTA;
+  constexpr int Q_BYTES = Shape<D>::Q_BYTES;
+  constexpr int Q_BOX = BM * 128;              // 128 rows x 64 channels
+  constexpr int KROWS = Shape<D>::KROWS;
+  constexpr int K_BOX = KROWS * 128;
+  extern __shared__ uint8_t dsmem_raw[];
+  __shared__ Barriers sb;
+  __shared__ Plan pl;
+  __shared__ Seg seg_sh[2];
+  __shared__ float m_sh[NSBUF][BM];
+  __shared__ float fin[2 * NWG][BM];
+
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dsmem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* smem_q = smem;
+  uint8_t* pre = smem + Q_BYTES;
+  uint8_t* stages = pre + PRE_BYTES;
+  const uint32_t rank = NCTA == 2 ? cluster_ctarank() : 0;
+  const bool even = rank == 0;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);
+  const int lane = threadIdx.x & 31;
+  const int pid = blockIdx.x / NCTA;
+  const int upt = NCTA * p.tpc;                // tokens of a unit
+  const int used = p.tpc * p.G;                // rows of a CTA that hold tokens
+
+  if (threadIdx.x == WARP_LOAD * 32) {
+    mbar_init(&sb.pre_full, 1);
+    mbar_init(&sb.q_full, 1);
+    mbar_init(&sb.o_done, 1);
+    mbar_init(&sb.drain, 1);
+    mbar_init(&sb.v_tail, 32 * NCTA);
+    for (int t = 0; t < NSTAGE; ++t) {
+      mbar_init(&sb.stage_full[t], 1);
+      mbar_init(&sb.stage_free[t], 1);
+    }
+    for (int b = 0; b < NSBUF; ++b) {
+      mbar_init(&sb.s_full[b], 1);
+      mbar_init(&sb.p_ready[b], NCTA * BM);
+      mbar_init(&sb.m_ready[b], BM);
+    }
+    sb.abort_flag = 0;
+    pl.longest = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  if (warp == WARP_MMA) {
+    if constexpr (NCTA == 2) {
+      tmem_alloc_pair(&sb.tmem_base, 512);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(&sb.tmem_base, 512);
+      tmem_relinquish();
+    }
+  }
+  // rows of the Q tile that hold no token stay zero: no load or store reaches them
+  for (int i = threadIdx.x; i < (BM - used) * (D / 8); i += NUM_THREADS) {
+    const int r = used + i / (D / 8), c = i % (D / 8);
+    *reinterpret_cast<uint4*>(smem_q + (c >> 3) * Q_BOX + r * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async_smem();
+  griddep_wait();   // launched as a dependent: the cache and the lengths are written from here on
+  __syncthreads();  // pl.longest
+  plan_own(p, pl, upt, warp, lane, NUM_THREADS / 32, blockIdx.x == 0);
+  __syncthreads();
+
+  // ---- the planner's state (warp 11): its waves, then its share of the rest
+  long long t = 0, t1 = 0, t_first = 0, before = 0;
+  int waves = 0, wave = 0, C = p.C;
+  Walk wk{};
+  bool in_tail = false;
+  auto plan_next = [&](int i) {
+    Seg s{};
+    if (wave < waves) {
+      wk = walk_to_unit(p, pl, wave * C + pid, upt);
+      ++wave;
+      s.n = wk.n;
+      s.slot = -1;
+    } else if (t < t1) {
+      if (!in_tail) {
+        wk = walk_to_tile(p, pl, t, upt, lane, &before);
+        in_tail = true;
+      } else {
+        before += wk.n;
+        next_unit(p, wk, upt);
+      }
+      const long long e = min(t1, before + wk.n);
+      s.kv0 = (int)(t - before);
+      s.n = (int)(e - t);
+      s.slot = s.n == wk.n ? -1 : (t == t_first ? 2 * pid : 2 * pid + 1);
+      t = e;
+    }
+    if (s.n) {
+      s.last = wk.n - 1;
+      s.b = wk.b;
+      s.hk = wk.hk;
+      s.tok0 = wk.rt * upt;
+      s.s0 = wk.s.s0;
+      s.lq = wk.s.lq;
+      s.kv = wk.s.kv;
+      s.keys = wk.keys;
+      if (even && lane == 0 && s.slot >= 0) p.header[s.slot] = make_int4(s.b + 1, s.hk, s.tok0, 0);
+    }
+    if (lane == 0) seg_sh[i & 1] = s;
+    __syncwarp();
+  };
+  if (warp == WARP_PLAN) {
+    plan_sum(p, pl, lane);
+    const long long N = pl.tiles[p.pool.B];
+    const int U = pl.units[p.pool.B];
+    if (even && lane < 2) p.header[2 * pid + lane] = make_int4(0, 0, 0, 0);
+    __syncwarp();
+    // no share without a tile
+    if (N < C) C = (int)N;
+    if (pid < C) {
+      // about equal: no unit is over 1/8 longer than their mean
+      if ((long long)pl.longest * U * 8 <= N * 9) waves = U / C;
+      long long t0 = 0;
+      if (waves > 0 && waves * C < U) {
+        const Walk f = walk_to_unit(p, pl, waves * C, upt);
+        t0 = tiles_before(p, pl, f, upt, lane);
+      } else if (waves > 0) {
+        t0 = N;
+      }
+      const long long rest = N - t0;
+      t = t0 + rest * pid / C;
+      t1 = t0 + rest * (pid + 1) / C;
+      t_first = t;
+    }
+    plan_next(0);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (NCTA == 2) cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = sb.tmem_base;
+  const Ctx cx{&sb, NCTA == 2 ? mapa_shared(smem_u32(&sb.abort_flag), rank ^ 1u) : 0u, NCTA == 2, p.status};
+  auto aborted = [&]() { return *(volatile int*)&sb.abort_flag != 0; };
+  // all threads, between two segments
+  auto boundary = [&]() {
+    tc_fence_before();
+    if constexpr (NCTA == 2) cluster_sync(); else __syncthreads();
+    tc_fence_after();
+  };
+  auto even_addr = [&](uint64_t* bar) { return NCTA == 2 ? mapa_shared(smem_u32(bar), 0) : smem_u32(bar); };
+  // whether the values of tile j (of the unit) are written by warp 10
+  auto ragged = [&](const Seg& sg, int j) { return sg.kv - j * BN < BN; };
+
+  if (warp == WARP_LOAD) {
+    setmaxnreg_dec<REG_OTHER>();
+    int J0 = 0;
+    for (int si = 0;; ++si) {
+      const Seg sg = seg_sh[si & 1];
+      if (sg.n == 0) break;
+      const uint32_t sph = (uint32_t)si & 1u;
+      if (!aborted()) {
+        // boxes of a tile: keys first (KROWS / kbox pages x D / 64), values then (128 / vbox pages); a lane each
+        const int nkp = KROWS / p.kbox, nvp = BN / p.vbox;
+        const int kpg = lane % nkp, kch = lane / nkp;      // valid for lanes < nkp * D / 64
+        const bool klane = lane < nkp * (D / 64), vlane = lane < nvp;
+        auto page_at = [&](int row) {
+          return row < sg.kv ? paged::page_of(p.pool, sg.b, row, p.status) : 0;
+        };
+        const int mask = (1 << p.pool.page_shift) - 1;
+        const int koff = NCTA == 2 ? KROWS * (int)rank : 0;
+        auto krow = [&](int j) { return (sg.kv0 + j) * BN + koff + kpg * p.kbox; };
+        auto vrow = [&](int j) { return (sg.kv0 + j) * BN + lane * p.vbox; };
+        auto load_k = [&](uint32_t dst, uint32_t bar, int j, int pg) {
+          if (klane)
+            load_4d<NCTA>(dst + kch * K_BOX + kpg * p.kbox * 128, &tm_k, bar, 64 * kch, sg.hk, krow(j) & mask, pg);
+        };
+        if (even && lane == 0) mbar_expect_tx(&sb.q_full, NCTA * (D / 64) * used * 128);
+        __syncwarp();
+        const uint32_t qbar = even_addr(&sb.q_full);
+        if (lane < D / 64)
+          load_3d<NCTA>(smem_u32(smem_q) + lane * Q_BOX, &tm_q, qbar, 64 * lane, sg.hk * p.G,
+                        sg.s0 + sg.tok0 + (int)rank * p.tpc);
+        const int n_pre = min(sg.n, NSBUF);
+        if (even && lane == 0) mbar_expect_tx(&sb.pre_full, NCTA * HALF_TILE * n_pre);
+        __syncwarp();
+        int pk[NSBUF];
+#pragma unroll
+        for (int j = 0; j < NSBUF; ++j) pk[j] = j < n_pre && klane ? page_at(krow(j)) : 0;
+#pragma unroll
+        for (int j = 0; j < NSBUF; ++j)
+          if (j < n_pre) load_k(smem_u32(pre) + j * HALF_TILE, even_addr(&sb.pre_full), j, pk[j]);
+        // page indices one tile ahead
+        int kp = NSBUF < sg.n && klane ? page_at(krow(NSBUF)) : 0;
+        int vp = vlane ? page_at(vrow(0)) : 0;
+        bool ok = true;
+        for (int j = 0; j < sg.n; ++j) {
+          const int J = J0 + j, st = J % NSTAGE;
+          const bool has_k = j + NSBUF < sg.n, has_v = !ragged(sg, sg.kv0 + j);
+          const int kn = j + 1 + NSBUF < sg.n && klane ? page_at(krow(j + 1 + NSBUF)) : 0;
+          const int vn = j + 1 < sg.n && vlane ? page_at(vrow(j + 1)) : 0;
+          if (J >= NSTAGE &&
+              !(ok = pwait_warp(&sb.stage_free[st], (uint32_t)(J / NSTAGE - 1) & 1u, cx, RW_STATUS_TIMEOUT_LOAD)))
+            break;
+          if (even && lane == 0)
+            mbar_expect_tx(&sb.stage_full[st], NCTA * HALF_TILE * ((has_k ? 1 : 0) + (has_v ? 1 : 0)));
+          __syncwarp();
+          const uint32_t bar = even_addr(&sb.stage_full[st]);
+          const uint32_t dst = smem_u32(stages) + st * STAGE_BYTES;
+          if (has_v && vlane)
+            load_4d<NCTA>(dst + lane * p.vbox * 128, &tm_v, bar, 64 * (int)rank, sg.hk, vrow(j) & mask, vp);
+          if (has_k) load_k(dst + HALF_TILE, bar, j + NSBUF, kp);
+          kp = kn;
+          vp = vn;
+        }
+        // every copy has landed and every stage is released before the barriers are set up for the next segment
+        if (lane == 0) {
+          const int tail = sg.n > NSTAGE ? sg.n - NSTAGE : 0;
+          if (even) {
+            mbar_wait_drain(&sb.pre_full, sph);
+            for (int J = J0 + tail; J < J0 + sg.n; ++J)
+              mbar_wait_drain(&sb.stage_full[J % NSTAGE], (uint32_t)(J / NSTAGE) & 1u);
+            mbar_wait_drain(&sb.q_full, sph);
+          }
+          if (ok)
+            for (int J = J0 + tail; J < J0 + sg.n; ++J)
+              mbar_wait_drain(&sb.stage_free[J % NSTAGE], (uint32_t)(J / NSTAGE) & 1u);
+        }
+        __syncwarp();
+      }
+      J0 += sg.n;
+      boundary();
+    }
+  } else if (warp == WARP_MMA) {
+    setmaxnreg_dec<REG_OTHER>();
+    int J0 = 0, n_tail = 0;
+    for (int si = 0;; ++si) {
+      const Seg sg = seg_sh[si & 1];
+      if (sg.n == 0) break;
+      const uint32_t sph = (uint32_t)si & 1u;
+      if (even && !aborted()) {
+        constexpr uint32_t ID_QK = idesc<HALF>(NCTA * BM, BN, 0);
+        constexpr uint32_t ID_PV = idesc<HALF>(NCTA * BM, D, 1);
+        const uint64_t dq = umma_desc(smem_u32(smem_q), 16, 1024);
+        const uint64_t dk_pre = umma_desc(smem_u32(pre), 16, 1024);
+        const uint64_t dv_st = umma_desc(smem_u32(stages), 16384, 1024);
+        const uint64_t dk_st = umma_desc(smem_u32(stages + HALF_TILE), 16, 1024);
+        constexpr uint64_t PRE_DESC = HALF_TILE >> 4, STAGE_DESC = STAGE_BYTES >> 4;
+        auto issue_qk = [](uint32_t ts, uint64_t a, uint64_t b) {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            mma_ss_n<NCTA>(ts, a + (uint64_t)(((kk >> 2) * Q_BOX + (kk & 3) * 32) >> 4),
+                           b + (uint64_t)(((kk >> 2) * K_BOX + (kk & 3) * 32) >> 4), ID_QK, kk > 0 ? 1u : 0u);
+        };
+        auto issue_pv = [](uint32_t to, uint32_t ts, uint64_t b, bool acc) {
+#pragma unroll
+          for (int kk = 0; kk < BN / 16; ++kk)
+            mma_ts_n<NCTA>(to, ts + kk * 8, b + (uint64_t)((kk * 2048) >> 4), ID_PV, (acc || kk > 0) ? 1u : 0u);
+        };
+        bool ok = pwait_warp(&sb.q_full, sph, cx, RW_STATUS_TIMEOUT_MMA) &&
+                  pwait_warp(&sb.pre_full, sph, cx, RW_STATUS_TIMEOUT_MMA);
+        tc_fence_after();
+        if (ok) {
+          const int n_pre = min(sg.n, NSBUF);
+          if (elect_one()) {
+            for (int j = 0; j < n_pre; ++j) {
+              const int bk = (J0 + j) % NSBUF;
+              issue_qk(tmem + 128u + 128u * bk, dq, dk_pre + j * PRE_DESC);
+              commit_n<NCTA>(&sb.s_full[bk]);
+            }
+          }
+          __syncwarp();
+        }
+        int b = J0 % NSBUF, st = J0 % NSTAGE;
+        for (int j = 0; j < sg.n && ok; ++j) {
+          const int J = J0 + j;
+          if (!(ok = pwait_warp(&sb.p_ready[b], (uint32_t)(J / NSBUF) & 1u, cx, RW_STATUS_TIMEOUT_MMA))) break;
+          if (!(ok = pwait_warp(&sb.stage_full[st], (uint32_t)(J / NSTAGE) & 1u, cx, RW_STATUS_TIMEOUT_MMA))) break;
+          if (ragged(sg, sg.kv0 + j)) {
+            if (!(ok = pwait_warp(&sb.v_tail, (uint32_t)n_tail & 1u, cx, RW_STATUS_TIMEOUT_MMA))) break;
+            ++n_tail;
+          }
+          tc_fence_after();
+          if (elect_one()) {
+            issue_pv(tmem, tmem + 128u + 128u * b, dv_st + st * STAGE_DESC, j > 0);
+            if (j == sg.n - 1) commit_n<NCTA>(&sb.o_done);
+            if (j + NSBUF < sg.n) {
+              issue_qk(tmem + 128u + 128u * b, dq, dk_st + st * STAGE_DESC);
+              commit_n<NCTA>(&sb.s_full[b]);
+            }
+            commit_n<NCTA>(&sb.stage_free[st]);
+          }
+          __syncwarp();
+          if (++b == NSBUF) b = 0;
+          if (++st == NSTAGE) st = 0;
+        }
+        if (elect_one()) {
+          if constexpr (NCTA == 2) tc_commit_pair_mc(&sb.drain, 0x1); else tc_commit(&sb.drain);
+          mbar_wait_drain(&sb.drain, sph);
+        }
+        __syncwarp();
+      }
+      J0 += sg.n;
+      boundary();
+    }
+  } else if (warp == WARP_TAIL) {
+    setmaxnreg_dec<REG_OTHER>();
+    int J0 = 0;
+    for (int si = 0;; ++si) {
+      const Seg sg = seg_sh[si & 1];
+      if (sg.n == 0) break;
+      const int j = sg.n - 1;                  // only a unit's last tiles can be ragged, and only one of them is
+      if (ragged(sg, sg.kv0 + j) && !aborted()) {
+        const int J = J0 + j, st = J % NSTAGE;
+        const int row0 = (sg.kv0 + j) * BN, rows = max(0, sg.kv - row0);
+        const int c = lane & 7, r0 = lane >> 3;
+        const uint8_t* src = p.pool.v + (long long)sg.hk * p.pool.v_sh + 128 * rank + 16 * c;
+        const int mask = (1 << p.pool.page_shift) - 1;
+        const bool ok = J < NSTAGE ||
+                        pwait_warp(&sb.stage_free[st], (uint32_t)(J / NSTAGE - 1) & 1u, cx, RW_STATUS_TIMEOUT_LOAD);
+        if (ok) {
+          uint8_t* dst = stages + st * STAGE_BYTES;
+#pragma unroll 1
+          for (int r8 = 0; r8 < BN; r8 += 32) {
+            uint4 v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int r = r8 + 4 * i + r0;
+              v[i] = make_uint4(0, 0, 0, 0);
+              if (r < rows) {
+                const long long pg = paged::page_of(p.pool, sg.b, row0 + r, nullptr);
+                v[i] = *reinterpret_cast<const uint4*>(src + pg * p.pool.v_sp + ((row0 + r) & mask) * p.pool.v_sl);
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int r = r8 + 4 * i + r0;
+              *reinterpret_cast<uint4*>(dst + r * 128 + ((c ^ (r & 7)) << 4)) = v[i];
+            }
+          }
+          fence_proxy_async_smem();
+          mbar_arrive_cluster(even_addr(&sb.v_tail));
+        }
+      }
+      __syncwarp();
+      J0 += sg.n;
+      boundary();
+    }
+  } else if (warp == WARP_PLAN) {
+    setmaxnreg_dec<REG_OTHER>();
+    for (int si = 0;; ++si) {
+      const int n = seg_sh[si & 1].n;
+      if (n == 0) break;
+      plan_next(si + 1);
+      boundary();
+    }
+  } else {
+    // ------------------------------------------------------------ softmax, then the output
+    setmaxnreg_inc<REG_SOFTMAX>();
+    const int w = warp >> 2;
+    const int r = threadIdx.x & 127;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tO = tmem + lane_base;
+    const float sl2 = p.scale_log2;
+    const uint32_t p_ready0 = even_addr(&sb.p_ready[0]);
+    const int rtok = r / p.G, rg = r - rtok * p.G;   // the row's token (of the CTA's) and head (of the group's)
+    int J0 = 0;
+    for (int si = 0;; ++si) {
+      const Seg sg = seg_sh[si & 1];
+      if (sg.n == 0) break;
+      const uint32_t sph = (uint32_t)si & 1u;
+      const int tok = sg.tok0 + (int)rank * p.tpc + rtok;  // within the sequence
+      const bool there = r < used && tok < sg.lq;
+      // keys of the row; a row without a token takes them all (its values go nowhere)
+      const int lim = there ? (p.causal ? max(0, sg.kv - sg.lq + tok + 1) : sg.kv) : sg.kv;
+      // keys that every row of the CTA sees
+      const int all = p.causal ? max(0, min(sg.kv, sg.kv - sg.lq + sg.tok0 + (int)rank * p.tpc + 1)) : sg.kv;
+      bool ok = !aborted();
+      float m_base = -INFINITY;
+      uint64_t l2 = 0ull;
+      for (int j = w; j < sg.n && ok; j += NWG) {
+        const int J = J0 + j;
+        const int b = J % NSBUF;
+        const uint32_t tS = tmem + lane_base + 128u + 128u * b;
+        if (!(ok = pwait_warp(&sb.s_full[b], (uint32_t)(J / NSBUF) & 1u, cx, RW_STATUS_TIMEOUT_SOFTMAX))) break;
+        tc_fence_after();
+        const int key0 = (sg.kv0 + j) * BN;
+        const bool masked = key0 + BN > all;
+        const int cut = lim - key0;              // columns from here on are not seen
+        auto load_quarter = [&](int q, uint32_t (&v)[32]) {
+          tmem_ld32(tS + 32 * q, v);
+          tmem_wait_ld();
+          reg_fence32(v);
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (32 * q + e >= cut) v[e] = __float_as_uint(-INFINITY);
+          }
+        };
+        auto load_half = [&](int h, uint32_t (&v)[2][32]) {
+          tmem_ld32(tS + 64 * h, v[0]);
+          tmem_ld32(tS + 64 * h + 32, v[1]);
+          tmem_wait_ld();
+          reg_fence32(v[0]);
+          reg_fence32(v[1]);
+        };
+        auto quarter_max = [](const uint32_t (&v)[32], float row_max) -> float {
+          float a[4];
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const uint32_t* x = &v[g * 8];
+            float u = fmax3(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]));
+            u = fmax3(u, __uint_as_float(x[3]), __uint_as_float(x[4]));
+            u = fmax3(u, __uint_as_float(x[5]), __uint_as_float(x[6]));
+            a[g] = fmaxf(u, __uint_as_float(x[7]));
+          }
+          return fmax3(row_max, fmax3(a[0], a[1], a[2]), a[3]);
+        };
+        auto quarter_exp = [](const uint32_t (&v)[32], uint64_t s2, uint64_t nm2, uint32_t (&pk)[32], const int o,
+                              uint64_t (&lacc)[2]) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const uint64_t xv = ffma2(f2_pack(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), s2, nm2);
+            float x0, x1;
+            f2_unpack(xv, x0, x1);
+            const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+            lacc[e & 1] = fadd2(lacc[e & 1], f2_pack(p0, p1));
+            pk[o + e] = Num<HALF>::pack(p0, p1);
+          }
+        };
+        const uint64_t s2 = f2_pack(sl2, sl2);
+        // One pass over S where nothing is masked, against the exponent base of this
+        // warpgroup's previous tile; it stands when tile j - 1 kept that base and this
+        // tile does not ask for a new one.  Otherwise S is read a second time.
+        float row_max = -INFINITY, m_prev = -INFINITY;
+        bool fast = false;
+        const bool one_pass = j >= NWG && !masked;
+        if (one_pass) {
+          uint32_t pk[2][32];
+          uint64_t l2f = l2;
+          const float nm0 = -m_base * sl2;
+          const uint64_t nm02 = f2_pack(nm0, nm0);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t v[2][32];
+            load_half(h, v);
+            uint64_t lacc[2] = {0ull, 0ull};
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              row_max = quarter_max(v[c], row_max);
+              quarter_exp(v[c], s2, nm02, pk[h], 16 * c, lacc);
+            }
+            l2f = fadd2(l2f, fadd2(lacc[0], lacc[1]));
+          }
+          const int Jp = J - 1;
+          if (!(ok = pwait_warp(&sb.m_ready[Jp % NSBUF], (uint32_t)(Jp / NSBUF) & 1u, cx, RW_STATUS_TIMEOUT_SOFTMAX)))
+            break;
+          m_prev = m_sh[Jp % NSBUF][r];
+          const float m_new = fmaxf(m_prev, row_max);
+          // (a base of -inf has made P NaN: it never stands)
+          fast = __all_sync(0xffffffffu, m_prev == m_base && m_base != -INFINITY &&
+                                             !((m_new - m_prev) * sl2 > RESCALE_THRESHOLD));
+          if (fast) {
+            m_sh[b][r] = m_base;
+            mbar_arrive(&sb.m_ready[b]);
+            l2 = l2f;
+            tmem_st32(tS, pk[0]);
+            tmem_st32(tS + 32, pk[1]);
+          }
+        }
+        if (!fast) {
+          if (!one_pass) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint32_t v[32];
+              load_quarter(q, v);
+              row_max = quarter_max(v, row_max);
+            }
+            if (j > 0) {
+              const int Jp = J - 1;
+              if (!(ok = pwait_warp(&sb.m_ready[Jp % NSBUF], (uint32_t)(Jp / NSBUF) & 1u, cx,
+                                    RW_STATUS_TIMEOUT_SOFTMAX)))
+                break;
+              m_prev = m_sh[Jp % NSBUF][r];
+            }
+          }
+          const float m_new = fmaxf(m_prev, row_max);
+          const bool need = (m_new - m_prev) * sl2 > RESCALE_THRESHOLD;  // false where both are -inf
+          const float m_use = need ? m_new : m_prev;
+          m_sh[b][r] = m_use;
+          mbar_arrive(&sb.m_ready[b]);
+          if (j > 0 && __any_sync(0xffffffffu, need)) {
+            const float alpha = need ? fast_exp2((m_prev - m_use) * sl2) : 1.f;
+            if (!(ok = pwait_warp(&sb.stage_free[(J - 1) % NSTAGE], (uint32_t)((J - 1) / NSTAGE) & 1u, cx,
+                                  RW_STATUS_TIMEOUT_SOFTMAX)))
+              break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32(tO + 32 * c, o);
+              tmem_wait_ld();
+              reg_fence32(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st32(tO + 32 * c, o);
+            }
+          }
+          if (m_base != m_use) {
+            float lo, hi;
+            f2_unpack(l2, lo, hi);
+            const float f = fast_exp2((m_base - m_use) * sl2);
+            l2 = f2_pack(lo * f, hi * f);
+            m_base = m_use;
+          }
+          const float nm = m_use == -INFINITY ? 0.f : -m_use * sl2;  // nothing seen yet: weights of exp2(-inf) = 0
+          const uint64_t nm2 = f2_pack(nm, nm);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t pk[32];
+            uint64_t lacc[2] = {0ull, 0ull};
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              uint32_t v[32];
+              load_quarter(2 * h + c, v);
+              quarter_exp(v, s2, nm2, pk, 16 * c, lacc);
+            }
+            l2 = fadd2(l2, fadd2(lacc[0], lacc[1]));
+            tmem_st32(tS + 32 * h, pk);
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive_cluster(p_ready0 + 8u * (uint32_t)b);
+      }
+      {
+        float lo, hi;
+        f2_unpack(l2, lo, hi);
+        fin[2 * w][r] = m_base;
+        fin[2 * w + 1][r] = lo + hi;
+      }
+      named_bar_sync(1, SOFTMAX_THREADS);
+      const float m_fin = fmaxf(fin[0][r], fin[2][r]);
+      float l_row = 0.f;
+#pragma unroll
+      for (int g = 0; g < NWG; ++g) {
+        const float lg = fin[2 * g + 1][r];
+        // an empty sum adds nothing; anything else, NaN included, counts
+        if (lg != 0.f) l_row += lg * fast_exp2((fin[2 * g][r] - m_fin) * sl2);
+      }
+      ok = __all_sync(0xffffffffu, ok) && !aborted();
+      if (ok) ok = pwait_warp(&sb.o_done, sph, cx, RW_STATUS_TIMEOUT_SOFTMAX);
+      tc_fence_after();
+      constexpr int CW = D / NWG;                  // channels of a warpgroup
+      if (ok && sg.slot >= 0) {
+        float* base = p.scratch + (long long)sg.slot * Shape<D>::SLOT_FLOATS;
+        constexpr int R = NCTA * BM;
+        const int row = (int)rank * BM + r;
+#pragma unroll 1
+        for (int c = 0; c < CW / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(tO + CW * w + 32 * c, o);
+          tmem_wait_ld();
+          reg_fence32(o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) base[(long long)(CW * w + 32 * c + e) * R + row] = __uint_as_float(o[e]);
+        }
+        if (w == 0) {
+          base[(long long)D * R + row] = m_fin;
+          base[(long long)D * R + R + row] = l_row;
+        }
+      } else if (sg.slot < 0) {
+        // O / l in the type -> shared memory (over the Q tile, which no MMA reads any more) -> whole rows
+        const float inv = l_row != 0.f ? 1.f / l_row : 0.f;
+        if (ok && (warp & 3) * 32 < used) {         // a warp without a token has nothing to store
+#pragma unroll 1
+          for (int c = 0; c < CW / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(tO + CW * w + 32 * c, o);
+            tmem_wait_ld();
+            reg_fence32(o);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int ch = (CW * w + 32 * c) / 8 + q;
+              uint4 v;
+              v.x = Num<HALF>::pack(__uint_as_float(o[8 * q + 0]) * inv, __uint_as_float(o[8 * q + 1]) * inv);
+              v.y = Num<HALF>::pack(__uint_as_float(o[8 * q + 2]) * inv, __uint_as_float(o[8 * q + 3]) * inv);
+              v.z = Num<HALF>::pack(__uint_as_float(o[8 * q + 4]) * inv, __uint_as_float(o[8 * q + 5]) * inv);
+              v.w = Num<HALF>::pack(__uint_as_float(o[8 * q + 6]) * inv, __uint_as_float(o[8 * q + 7]) * inv);
+              if (r < used)
+                *reinterpret_cast<uint4*>(smem_q + (ch >> 3) * Q_BOX + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v;
+            }
+          }
+        }
+        if (ok && w == 0 && there) {
+          const long long at = (long long)(sg.s0 + tok) * p.Hq + sg.hk * p.G + rg;
+          if (p.lse) p.lse[at] = l_row != 0.f ? (m_fin * sl2 + log2f(l_row)) * 0.6931471805599453f : -INFINITY;
+          if (p.row_ml) p.row_ml[at] = make_float2(l_row != 0.f ? m_fin * sl2 : 0.f, inv);
+        }
+        named_bar_sync(1, SOFTMAX_THREADS);
+        constexpr int CH = D / 8;
+        for (int i = threadIdx.x; ok && i < used * CH; i += SOFTMAX_THREADS) {
+          const int rr = i / CH, ch = i % CH;
+          const int tk = rr / p.G, g = rr - tk * p.G;
+          const int tt = sg.tok0 + (int)rank * p.tpc + tk;
+          if (tt < sg.lq)
+            *reinterpret_cast<uint4*>(p.out + (long long)(sg.s0 + tt) * p.o_sl +
+                                      (long long)(sg.hk * p.G + g) * p.o_sh + 16 * ch) =
+                *reinterpret_cast<const uint4*>(smem_q + (ch >> 3) * Q_BOX + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4));
+        }
+        fence_proxy_async_smem();                  // read before the next segment's Q is loaded over it
+      }
+      J0 += sg.n;
+      boundary();
+    }
+  }
+
+  if (warp == WARP_LOAD && lane == 0 && aborted()) {
+    // after a timeout some copies may be in flight without a wait for them: time to land
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) {
+    }
+  }
+  if (threadIdx.x == 0) griddep_launch_dependents();
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (NCTA == 2) cluster_sync();
+  if (warp == WARP_MMA) {
+    tc_fence_after();
+    if constexpr (NCTA == 2) tmem_dealloc_pair(tmem, 512); else tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the parts of the units that more than one pair worked on.  The parts of a unit
+// lie in consecutive used slots; the block of the first of them joins them, in the order
+// of the keys.  A thread has one row and 32 channels.
+template <bool HALF, int D>
+__global__ void __launch_bounds__(BM) join_kernel(const __grid_constant__ Params p) {
+  griddep_launch_dependents();
+  griddep_wait();
+  constexpr int R = Shape<D>::NCTA * BM;
+  const int s = blockIdx.x;
+  const int4 h = __ldcg(p.header + s);
+  if (h.x == 0) return;
+  auto same = [&](const int4& o) { return o.x == h.x && o.y == h.y && o.z == h.z; };
+  for (int o = s - 1; o >= 0; --o) {
+    const int4 x = __ldcg(p.header + o);
+    if (x.x == 0) continue;
+    if (same(x)) return;
+    break;
+  }
+  const int rank = blockIdx.y, r = threadIdx.x, row = rank * BM + r, c0 = 32 * blockIdx.z;
+  const Seq sq = paged::load_seq(p.pool, h.x - 1, p.T, nullptr);
+  const int rtok = r / p.G, g = r - rtok * p.G;
+  const int tok = h.z + rank * p.tpc + rtok;
+  if (r >= p.tpc * p.G || tok >= sq.lq) return;
+  float m = -INFINITY;
+  int end = s;
+  for (int o = s; o < 2 * p.C; ++o) {
+    const int4 x = __ldcg(p.header + o);
+    if (x.x == 0) continue;
+    if (!same(x)) break;
+    end = o;
+    m = fmaxf(m, __ldcg(p.scratch + (long long)o * Shape<D>::SLOT_FLOATS + (long long)D * R + row));
+  }
+  float acc[32], l = 0.f;
+#pragma unroll
+  for (int e = 0; e < 32; ++e) acc[e] = 0.f;
+  const float base = m == -INFINITY ? 0.f : m;
+  for (int o = s; o <= end; ++o) {
+    if (__ldcg(&p.header[o].x) == 0) continue;
+    const float* sl = p.scratch + (long long)o * Shape<D>::SLOT_FLOATS;
+    const float f = fast_exp2((__ldcg(sl + (long long)D * R + row) - base) * p.scale_log2);
+    l += f * __ldcg(sl + (long long)D * R + R + row);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) acc[e] += f * __ldcg(sl + (long long)(c0 + e) * R + row);
+  }
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  const int head = h.y * p.G + g;
+  uint4* dst = reinterpret_cast<uint4*>(p.out + (long long)(sq.s0 + tok) * p.o_sl + (long long)head * p.o_sh + 2 * c0);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint4 v;
+    v.x = Num<HALF>::pack(acc[8 * q + 0] * inv, acc[8 * q + 1] * inv);
+    v.y = Num<HALF>::pack(acc[8 * q + 2] * inv, acc[8 * q + 3] * inv);
+    v.z = Num<HALF>::pack(acc[8 * q + 4] * inv, acc[8 * q + 5] * inv);
+    v.w = Num<HALF>::pack(acc[8 * q + 6] * inv, acc[8 * q + 7] * inv);
+    dst[q] = v;
+  }
+  if (c0 == 0) {
+    const long long at = (long long)(sq.s0 + tok) * p.Hq + head;
+    if (p.lse) p.lse[at] = l != 0.f ? (m * p.scale_log2 + log2f(l)) * 0.6931471805599453f : -INFINITY;
+    if (p.row_ml) p.row_ml[at] = make_float2(l != 0.f ? m * p.scale_log2 : 0.f, inv);
+  }
+}
+
+// ---------------------------------------------------------------- host
+inline CUtensorMapDataType dt(int dtype) {
+  return dtype == RW_DTYPE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
+
+// A pool as (D, Hkv, page_size, num_pages), boxes of 64 channels x 1 head x `rows` rows of a page.
+int pool_map(CUtensorMap* m, const rw_paged_t* c, bool values, int rows) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (!enc) return RW_ERR_DRIVER;
+  const void* ptr = values ? c->v : c->k;
+  long long sp = values ? c->v_sp : c->k_sp, sl = values ? c->v_sl : c->k_sl, sh = values ? c->v_sh : c->k_sh;
+  // strides of dimensions of one are never used, but have to be valid
+  if (c->num_pages == 1) sp = 8;
+  if (c->Hkv == 1) sh = 8;
+  cuuint64_t dims[4] = {(cuuint64_t)c->D, (cuuint64_t)c->Hkv, (cuuint64_t)c->page_size, (cuuint64_t)c->num_pages};
+  cuuint64_t strides[3] = {(cuuint64_t)sh * 2, (cuuint64_t)sl * 2, (cuuint64_t)sp * 2};
+  cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1};
+  cuuint32_t es[4] = {1, 1, 1, 1};
+  return enc(m, dt(c->dtype), 4, const_cast<void*>(ptr), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? RW_OK : RW_ERR_DRIVER;
+}
+
+// q as (D, Hq, T), boxes of 64 channels x `heads` heads x `tokens` tokens.
+int q_map(CUtensorMap* m, const void* q, int dtype, int T, int Hq, int D, long long sl, long long sh, int heads,
+          int tokens) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (!enc) return RW_ERR_DRIVER;
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)Hq, (cuuint64_t)T};
+  cuuint64_t strides[2] = {(cuuint64_t)sh * 2, (cuuint64_t)sl * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)heads, (cuuint32_t)tokens};
+  cuuint32_t es[3] = {1, 1, 1};
+  return enc(m, dt(dtype), 3, const_cast<void*>(q), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? RW_OK : RW_ERR_DRIVER;
+}
+
+int grid_size(int D) {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 0;
+  return D == 128 ? sms / 2 : sms;
+}
+
+long long workspace_bytes(int D) {
+  const long long C = grid_size(D);
+  return 2 * C * ((D == 128 ? Shape<128>::SLOT_FLOATS : Shape<64>::SLOT_FLOATS) * 4 + 16);
+}
+
+template <bool HALF, int D>
+int launch_one(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, cudaStream_t st) {
+  static std::atomic<unsigned long long> done{0};
+  constexpr int NCTA = Shape<D>::NCTA;
+  if (!ensure_smem_attr(reinterpret_cast<const void*>(chunk_kernel<HALF, D>), Shape<D>::SMEM, &done))
+    return RW_ERR_CUDA;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(NCTA * p.C);
+  cfg.blockDim = dim3(NUM_THREADS);
+  cfg.dynamicSmemBytes = Shape<D>::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = NCTA;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = NCTA == 2 ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, chunk_kernel<HALF, D>, mq, mk, mv, p) != cudaSuccess) return RW_ERR_CUDA;
+  return launch_dependent(join_kernel<HALF, D>, dim3(2 * p.C, NCTA, D / 32), dim3(BM), 0, st, p) == cudaSuccess
+             ? RW_OK : RW_ERR_CUDA;
+}
+
+int launch(const rw_paged_t* cache, const Pool& pool, const Call& c, void* workspace, cudaStream_t st) {
+  Params p{};
+  p.pool = pool;
+  p.T = c.T; p.Hq = c.Hq; p.G = c.Hq / pool.Hkv; p.causal = c.causal;
+  p.tpc = BM / p.G;
+  p.C = grid_size(cache->D);
+  if (p.C < 1) return RW_ERR_CUDA;
+  p.scale_log2 = c.scale_log2;
+  p.out = static_cast<uint8_t*>(c.out);
+  p.o_sl = 2 * c.o_sl; p.o_sh = 2 * c.o_sh;
+  p.lse = c.lse;
+  p.row_ml = c.row_ml;
+  p.header = static_cast<int4*>(workspace);
+  p.scratch = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 2LL * p.C * 16);
+  const int krows = cache->D == 128 ? Shape<128>::KROWS : Shape<64>::KROWS;
+  p.kbox = cache->page_size < krows ? cache->page_size : krows;
+  p.vbox = cache->page_size < BN ? cache->page_size : BN;
+  p.status = c.status;
+  CUtensorMap mq, mk, mv;
+  if (q_map(&mq, c.q, cache->dtype, c.T, c.Hq, cache->D, c.q_sl, c.q_sh, p.G, p.tpc) ||
+      pool_map(&mk, cache, false, p.kbox) || pool_map(&mv, cache, true, p.vbox))
+    return RW_ERR_DRIVER;
+  if (cache->dtype == RW_DTYPE_FP16)
+    return cache->D == 128 ? launch_one<true, 128>(mq, mk, mv, p, st) : launch_one<true, 64>(mq, mk, mv, p, st);
+  return cache->D == 128 ? launch_one<false, 128>(mq, mk, mv, p, st) : launch_one<false, 64>(mq, mk, mv, p, st);
+}
+
+}  // namespace chunk
+}  // namespace rw

@@ -20,6 +20,7 @@
 // of 16-byte cp.async; rows behind the last visible one are filled with zeros, never
 // read, so what a page holds there (NaN included) does not matter.
 #include "paged.cuh"
+#include "paged_chunk.h"
 
 namespace rw {
 namespace rows {
@@ -489,6 +490,10 @@ inline int grid_size(int D) {
   return sms * (D == 128 ? 2 : 4);
 }
 
+// Which kernel: 16 rows of a sequence and key head are all that rows_kernel can use of a
+// key tile it has read; with more, the tiles of chunk_kernel.
+inline bool on_tensor_tiles(int B, long long nrt) { return nrt > 1 && B <= chunk::MAX_BATCH; }
+
 struct Layout {
   long long part, ml, scores, total;  // byte offsets
 };
@@ -535,6 +540,14 @@ extern "C" int rw_paged_attn(const rw_paged_t* cache, const void* q, void* out, 
   const long long nrt = ((long long)(max_q_len < T ? max_q_len : T) * G + rows::RT - 1) / rows::RT;
   if (nrt * cache->B * p.pool.Hkv > (1ll << 30)) return RW_ERR_CAPACITY;
   const long long cap = (long long)cache->table_width * cache->page_size;
+  const float scale_log2 = softmax_scale * 1.4426950408889634f;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (rows::on_tensor_tiles(cache->B, nrt) && !sums) {
+    if (!workspace || !aligned16(workspace) || workspace_bytes < chunk::workspace_bytes(cache->D))
+      return RW_ERR_INVALID_ARG;
+    const chunk::Call c{q, out, lse, nullptr, T, Hq, causal != 0, q_sl, q_sh, o_sl, o_sh, scale_log2, status};
+    return chunk::launch(cache, p.pool, c, workspace, st);
+  }
   const int C = rows::grid_size(cache->D);
   if (C == 0) return RW_ERR_CUDA;
   const rows::Layout lay = rows::layout(cache->D, C, cache->B, p.pool.Hkv, (int)nrt, cap, sums != nullptr);
@@ -548,14 +561,13 @@ extern "C" int rw_paged_attn(const rw_paged_t* cache, const void* q, void* out, 
   p.q_sl = 2 * q_sl; p.q_sh = 2 * q_sh; p.o_sl = 2 * o_sl; p.o_sh = 2 * o_sh;
   p.T = T; p.Hq = Hq; p.G = G; p.nrt = (int)nrt; p.causal = causal != 0;
   p.min_tiles = 1;
-  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.scale_log2 = scale_log2;
   p.part = reinterpret_cast<float*>(ws + lay.part);
   p.counters = counters;
   p.scores = sums ? reinterpret_cast<float*>(ws + lay.scores) : nullptr;
   p.row_ml = sums ? reinterpret_cast<float2*>(ws + lay.ml) : nullptr;
   p.cap = cap;
   p.status = status;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
   int rc;
   if (cache->dtype == RW_DTYPE_FP16)
     rc = cache->D == 128 ? rows::launch_rows<true, 128>(p, C, st) : rows::launch_rows<true, 64>(p, C, st);
@@ -582,6 +594,7 @@ extern "C" long long rw_paged_attn_workspace_bytes(int T, int Hq, int Hkv, int D
     return 0;
   const long long nrt = ((long long)(max_q_len < T ? max_q_len : T) * (Hq / Hkv) + rows::RT - 1) / rows::RT;
   if (nrt * B * Hkv > (1ll << 30)) return 0;
+  if (rows::on_tensor_tiles(B, nrt) && !with_sums) return chunk::workspace_bytes(D);
   if (n_counters) *n_counters = rows::counters_needed(B, Hkv, (int)nrt);
   return rows::layout(D, rows::grid_size(D), B, Hkv, (int)nrt, cache_rows, with_sums != 0).total;
 }

@@ -364,11 +364,11 @@ def paged_attention(q, k_pages, v_pages, block_table, q_starts, kv_lens, max_q_l
                                                      n)
             stream = torch.cuda.current_stream(dev).cuda_stream
             ws = torch.empty(need, dtype=torch.uint8, device=dev)
-            counters = _zeroed(dev, n.value, stream)
+            counters = _zeroed(dev, n.value, stream) if n.value else None
             code = lib.rw_paged_attn(
                 pg, q.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else None, T, Hq, longest,
-                *_sl_sh(q), *_sl_sh(out), int(bool(causal)), scale, *sums, counters.data_ptr(), counters.numel(),
-                ws.data_ptr(), need, _native.status_tensor(dev).data_ptr(), stream)
+                *_sl_sh(q), *_sl_sh(out), int(bool(causal)), scale, *sums, counters.data_ptr() if n.value else None,
+                n.value, ws.data_ptr(), need, _native.status_tensor(dev).data_ptr(), stream)
         _native.check(code, "rw_paged_attn")
     return (out, lse) if return_lse else out
 

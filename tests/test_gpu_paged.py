@@ -98,6 +98,15 @@ def _run(cuda, lqs, lens, hq, hkv, D, dtype, page=16, causal=True, layout="rows"
     _check(out[:n], lse[:n], w[..., :-5] if sums else None, want, dtype, D, max(lens + [1]), 0.5)
     if sums:
         assert (w[..., -5:] == 0.5).all()
+    if sums:
+        # and without the sums
+        plain = torch.full_like(q, 7.0)
+        _, lse3 = paged_attention(q, k, v, table, starts, kv, max_q_len=max(lqs) if max_q is None else max_q,
+                                  causal=causal, return_lse=True, out=plain)
+        torch.cuda.synchronize()
+        _status_clean()
+        assert (plain[n:] == 7.0).all()
+        _check(plain[:n], lse3[:n], None, want, dtype, D, max(lens + [1]))
     # the same call again gives the same bits
     if sums:
         w2 = torch.full_like(w, 0.5)
