@@ -48,13 +48,19 @@ __device__ __forceinline__ Seq load_seq(const Pool& p, int b, int T, int* status
 
 // Page of a sequence's row; a page outside the pool becomes page 0 (its rows are
 // then wrong, and said to be) so that no address leaves the pool.
-__device__ __forceinline__ int page_of(const Pool& p, int b, int row, int* status) {
-  const int pg = __ldg(p.table + b * p.table_stride + (row >> p.page_shift));
+__device__ __forceinline__ int raw_page_of(const Pool& p, int b, int row) {
+  return __ldg(p.table + b * p.table_stride + (row >> p.page_shift));
+}
+// (apart from the load, so that a page index fetched ahead is waited for only where it is used)
+__device__ __forceinline__ int checked_page(const Pool& p, int pg, int* status) {
   if ((unsigned)pg >= (unsigned)p.num_pages) {
     report_status(status, RW_STATUS_BAD_SLOT);
     return 0;
   }
   return pg;
+}
+__device__ __forceinline__ int page_of(const Pool& p, int b, int row, int* status) {
+  return checked_page(p, raw_page_of(p, b, row), status);
 }
 
 // The two 16-bit types.  Values are widened to fp32 exactly and rounded once, to

@@ -14,11 +14,11 @@
 //   TMEM columns  O [0, D)  S0 [128, 256)  S1 [256, 384)  S2 [384, 512)
 // Key tile j lands in S buffer j mod 3 and its weights P (16-bit) overwrite the buffer's
 // first 64 columns; the tensor pipe runs QK up to three tiles ahead of the softmax.
-// Warps: two softmax warpgroups (tiles j even / odd, a row a thread), warp 8 loads,
-// warp 9 issues the MMAs, warp 10 writes the last value tile, warp 11 plans.
+// Warps: two softmax warpgroups (tiles j even / odd, a row a thread), warp 8 loads q and keys,
+// warp 9 issues the MMAs, warp 10 loads the values, warp 11 plans.
 //
-// Pages: a key tile is gathered by one TMA box a page (and 64 channels), issued by one
-// lane each; page indices are read one tile ahead.  Of the page that a sequence ends in,
+// Pages: a tile is gathered by one TMA box a page (and 64 channels); page indices are read
+// one tile ahead.  Of the page that a sequence ends in,
 // the rows behind the end may hold anything: keys there are masked by selection, but a
 // weight of 0 times NaN is NaN, so the values of such a tile are not loaded by TMA; warp
 // 10 copies the rows that exist and writes zeros for the others.
@@ -48,11 +48,16 @@ constexpr int PRE_BYTES = NSBUF * HALF_TILE; // keys of tiles 0-2
 constexpr int STAGE_BYTES = 2 * HALF_TILE;   // stage j: values of tile j, then keys of tile j + 3
 constexpr int NWG = 2;
 constexpr int NUM_THREADS = 128 * (NWG + 1);
-constexpr int WARP_LOAD = 8, WARP_MMA = 9, WARP_TAIL = 10, WARP_PLAN = 11;
+constexpr int WARP_LOAD = 8, WARP_MMA = 9, WARP_V = 10, WARP_PLAN = 11;
 constexpr int SOFTMAX_THREADS = 256;
 constexpr int REG_SOFTMAX = 208, REG_OTHER = 88;
 static_assert(NWG * 128 * REG_SOFTMAX + 128 * REG_OTHER <= NUM_THREADS * 168, "register split exceeds the launch's");
 constexpr float RESCALE_THRESHOLD = 8.0f;    // log2 units
+constexpr int MAX_PARTS = 1024;              // slots of a launch (two a CTA or pair): checked by the host
+constexpr int MIN_SHARE = 12;                // cost of a share, where there is little work
+// What a unit costs beside its key tiles, in tiles: filling and draining the pipeline (q and
+// the first keys, the last softmax, the output) takes 5 to 8 us, a tile 0.75 to 0.9.
+constexpr int UNIT_COST = 7;
 
 template <int D>
 struct Shape {
@@ -66,7 +71,7 @@ struct Shape {
 // What a segment (the key tiles [kv0, kv0 + n) of one unit) needs.
 struct Seg {
   int n;                 // 0: no more work
-  int kv0, last;         // last: the tile with which the unit ends (kv0 + n - 1 <= last)
+  int kv0;
   int slot;              // -1: the whole unit
   int b, hk, tok0;       // unit's first token within the sequence
   int s0, lq, kv, keys;  // keys: rows that any token of the unit sees
@@ -85,11 +90,12 @@ struct Params {
   float* scratch;        // [2 C] slots
   int4* header;          // [2 C]: (b + 1 or 0, hk, tok0, unused)
   int kbox, vbox;        // rows of a TMA box: min(page, keys of a CTA), min(page, 128)
+  int k_head, k_page;    // strides of head and page in the key map's last dimension
   int* status;
 };
 
 struct __align__(8) Barriers {
-  uint64_t pre_full, q_full, o_done, drain, v_tail;
+  uint64_t pre_full, q_full, o_done, drain, v_tail, planned;
   uint64_t stage_full[NSTAGE], stage_free[NSTAGE];
   uint64_t s_full[NSBUF], p_ready[NSBUF], m_ready[NSBUF];
   uint32_t tmem_base;
@@ -140,6 +146,20 @@ __device__ __forceinline__ void load_4d(uint32_t dst, const CUtensorMap* m, uint
         "r"(c1), "r"(c2), "r"(c3) : "memory");
 }
 template <int NCTA>
+__device__ __forceinline__ void load_5d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2,
+                                        int c3, int c4) {
+  if constexpr (NCTA == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0),
+        "r"(c1), "r"(c2), "r"(c3), "r"(c4) : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0),
+        "r"(c1), "r"(c2), "r"(c3), "r"(c4) : "memory");
+}
+template <int NCTA>
 __device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2) {
   if constexpr (NCTA == 2)
     asm volatile(
@@ -165,6 +185,23 @@ __device__ __forceinline__ void commit_n(uint64_t* bar) {  // arrives on every C
   if constexpr (NCTA == 2) tc_commit_pair_mc(bar, 0x3); else tc_commit(bar);
 }
 
+// f(i, x of lane i) for i < n, by one lane, 8 at a time: an election for every box made
+// the loading warps, which have 12 boxes a tile with pages of 16, the slowest part.
+template <typename F>
+__device__ __forceinline__ void for_pages(int x, int n, F f) {
+  for (int i0 = 0; i0 < n; i0 += 8) {
+    int y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x, i0 + i);
+    if (elect_one()) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i0 + i < n) f(i0 + i, y[i]);
+    }
+    __syncwarp();
+  }
+}
+
 template <bool HALF>
 constexpr uint32_t idesc(int M, int N, int b_mn) {
   return HALF ? (idesc_bf16_f32(M, N, 0, b_mn) & ~((1u << 7) | (1u << 10))) : idesc_bf16_f32(M, N, 0, b_mn);
@@ -181,13 +218,14 @@ __device__ __forceinline__ int tiles_of(const Params& p, const Seq& s, int rt, i
   return max(1, (k + BN - 1) / BN);
 }
 
+// The work is dealt out by cost: a unit of n tiles is UNIT_COST + n long.
 struct Plan {
-  long long tiles[MAX_BATCH + 1];  // key tiles of the units of the sequences before each
+  long long cost[MAX_BATCH + 1];   // cost of the units of the sequences before each
   int units[MAX_BATCH + 1];        // units before each
   int longest;
 };
 
-// Filled by all threads; the caller synchronises.  tiles[b + 1], units[b + 1] first hold
+// Filled by all threads; the caller synchronises.  cost[b + 1], units[b + 1] first hold
 // the sequence's own numbers, then warp 0 sums them up.
 __device__ __forceinline__ void plan_own(const Params& p, Plan& pl, int upt, int warp, int lane, int nwarps,
                                          bool report) {
@@ -197,7 +235,7 @@ __device__ __forceinline__ void plan_own(const Params& p, Plan& pl, int upt, int
     long long sum = 0;
     int top = 0, keys;
     for (int rt = lane; rt < nu; rt += 32) {
-      const int n = tiles_of(p, s, rt, upt, &keys);
+      const int n = UNIT_COST + tiles_of(p, s, rt, upt, &keys);
       sum += n;
       top = max(top, n);
     }
@@ -207,7 +245,7 @@ __device__ __forceinline__ void plan_own(const Params& p, Plan& pl, int upt, int
       top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
     }
     if (lane == 0) {
-      pl.tiles[b + 1] = sum * p.pool.Hkv;
+      pl.cost[b + 1] = sum * p.pool.Hkv;
       pl.units[b + 1] = nu * p.pool.Hkv;
       atomicMax(&pl.longest, top);
     }
@@ -218,7 +256,7 @@ __device__ __forceinline__ void plan_sum(const Params& p, Plan& pl, int lane) {
   int cu = 0;
   for (int b0 = 0; b0 < p.pool.B; b0 += 32) {
     const int b = b0 + lane;
-    long long t = b < p.pool.B ? pl.tiles[b + 1] : 0;
+    long long t = b < p.pool.B ? pl.cost[b + 1] : 0;
     int u = b < p.pool.B ? pl.units[b + 1] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -227,13 +265,13 @@ __device__ __forceinline__ void plan_sum(const Params& p, Plan& pl, int lane) {
       if (lane >= o) { t += y; u += z; }
     }
     if (b < p.pool.B) {
-      pl.tiles[b + 1] = ct + t;
+      pl.cost[b + 1] = ct + t;
       pl.units[b + 1] = cu + u;
     }
     ct += __shfl_sync(0xffffffffu, t, 31);
     cu += __shfl_sync(0xffffffffu, u, 31);
   }
-  if (lane == 0) { pl.tiles[0] = 0; pl.units[0] = 0; }
+  if (lane == 0) { pl.cost[0] = 0; pl.units[0] = 0; }
   __syncwarp();
 }
 
@@ -264,32 +302,32 @@ __device__ __forceinline__ Walk walk_to_unit(const Params& p, const Plan& pl, in
   w.n = tiles_of(p, w.s, w.rt, upt, &w.keys);
   return w;
 }
-// Whole warp: tiles of the units before that one.
-__device__ __forceinline__ long long tiles_before(const Params& p, const Plan& pl, const Walk& w, int upt, int lane) {
-  long long sum = 0, all = (pl.tiles[w.b + 1] - pl.tiles[w.b]) / p.pool.Hkv;
+// Whole warp: cost of the units before that one.
+__device__ __forceinline__ long long cost_before(const Params& p, const Plan& pl, const Walk& w, int upt, int lane) {
+  long long sum = 0, all = (pl.cost[w.b + 1] - pl.cost[w.b]) / p.pool.Hkv;
   int keys;
-  for (int rt = lane; rt < w.rt; rt += 32) sum += tiles_of(p, w.s, rt, upt, &keys);
+  for (int rt = lane; rt < w.rt; rt += 32) sum += UNIT_COST + tiles_of(p, w.s, rt, upt, &keys);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  return pl.tiles[w.b] + all * w.hk + sum;
+  return pl.cost[w.b] + all * w.hk + sum;
 }
-// Whole warp: the unit that holds tile t, and the tiles before it.
-__device__ __forceinline__ Walk walk_to_tile(const Params& p, const Plan& pl, long long t, int upt, int lane,
+// Whole warp: the unit in which the work before reaches cost t, and the cost before that unit.
+__device__ __forceinline__ Walk walk_to_cost(const Params& p, const Plan& pl, long long t, int upt, int lane,
                                              long long* before) {
   Walk w;
   int lo = 0, hi = p.pool.B - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (pl.tiles[mid] <= t) lo = mid; else hi = mid - 1;
+    if (pl.cost[mid] <= t) lo = mid; else hi = mid - 1;
   }
   w.b = lo;
   enter(p, w, upt);
-  const long long each = (pl.tiles[lo + 1] - pl.tiles[lo]) / p.pool.Hkv;
-  w.hk = (int)((t - pl.tiles[lo]) / each);
-  long long at = pl.tiles[lo] + each * w.hk;
+  const long long each = (pl.cost[lo + 1] - pl.cost[lo]) / p.pool.Hkv;
+  w.hk = (int)((t - pl.cost[lo]) / each);
+  long long at = pl.cost[lo] + each * w.hk;
   for (int r0 = 0; r0 < w.nu; r0 += 32) {
     int keys;
-    const int n = r0 + lane < w.nu ? tiles_of(p, w.s, r0 + lane, upt, &keys) : 0;
+    const int n = r0 + lane < w.nu ? UNIT_COST + tiles_of(p, w.s, r0 + lane, upt, &keys) : 0;
     int x = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -331,13 +369,16 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   constexpr int Q_BYTES = Shape<D>::Q_BYTES;
   constexpr int Q_BOX = BM * 128;              // 128 rows x 64 channels
   constexpr int KROWS = Shape<D>::KROWS;
-  constexpr int K_BOX = KROWS * 128;
+  // A key tile in shared memory: groups of 8 rows, in each the D / 64 blocks of 64 channels (8 x 128 bytes,
+  // swizzled), so that one TMA box brings all channels of a page's rows.
+  constexpr int K_GROUP = 1024 * (D / 64);
   extern __shared__ uint8_t dsmem_raw[];
   __shared__ Barriers sb;
   __shared__ Plan pl;
   __shared__ Seg seg_sh[2];
   __shared__ float m_sh[NSBUF][BM];
   __shared__ float fin[2 * NWG][BM];
+  __shared__ uint8_t* row_out[BM];
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dsmem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* smem_q = smem;
@@ -357,6 +398,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     mbar_init(&sb.o_done, 1);
     mbar_init(&sb.drain, 1);
     mbar_init(&sb.v_tail, 32 * NCTA);
+    mbar_init(&sb.planned, 1);
     for (int t = 0; t < NSTAGE; ++t) {
       mbar_init(&sb.stage_full[t], 1);
       mbar_init(&sb.stage_free[t], 1);
@@ -382,7 +424,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       tmem_relinquish();
     }
   }
-  // rows of the Q tile that hold no token stay zero: no load or store reaches them
+  // rows of the Q tile that hold no token stay zero: no load reaches them
   for (int i = threadIdx.x; i < (BM - used) * (D / 8); i += NUM_THREADS) {
     const int r = used + i / (D / 8), c = i % (D / 8);
     *reinterpret_cast<uint4*>(smem_q + (c >> 3) * Q_BOX + r * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
@@ -394,7 +436,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   __syncthreads();
 
   // ---- the planner's state (warp 11): its waves, then its share of the rest
-  long long t = 0, t1 = 0, t_first = 0, before = 0;
+  long long t = 0, t1 = 0, before = 0;
   int waves = 0, wave = 0, C = p.C;
   Walk wk{};
   bool in_tail = false;
@@ -405,22 +447,24 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       ++wave;
       s.n = wk.n;
       s.slot = -1;
-    } else if (t < t1) {
-      if (!in_tail) {
-        wk = walk_to_tile(p, pl, t, upt, lane, &before);
-        in_tail = true;
-      } else {
-        before += wk.n;
-        next_unit(p, wk, upt);
+    } else {
+      while (t < t1 && s.n == 0) {
+        if (!in_tail) {
+          wk = walk_to_cost(p, pl, t, upt, lane, &before);
+          in_tail = true;
+        } else {
+          before += UNIT_COST + wk.n;
+          next_unit(p, wk, upt);
+        }
+        // a unit's own cost comes before its first tile: a share that begins or ends in it has none of its tiles
+        const long long e = min(t1, before + UNIT_COST + wk.n);
+        s.kv0 = (int)max(0ll, t - before - UNIT_COST);
+        s.n = (int)max(0ll, e - before - UNIT_COST) - s.kv0;
+        s.slot = s.n == wk.n ? -1 : (s.kv0 > 0 ? 2 * pid : 2 * pid + 1);
+        t = e;
       }
-      const long long e = min(t1, before + wk.n);
-      s.kv0 = (int)(t - before);
-      s.n = (int)(e - t);
-      s.slot = s.n == wk.n ? -1 : (t == t_first ? 2 * pid : 2 * pid + 1);
-      t = e;
     }
     if (s.n) {
-      s.last = wk.n - 1;
       s.b = wk.b;
       s.hk = wk.hk;
       s.tok0 = wk.rt * upt;
@@ -430,31 +474,32 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       s.keys = wk.keys;
       if (even && lane == 0 && s.slot >= 0) p.header[s.slot] = make_int4(s.b + 1, s.hk, s.tok0, 0);
     }
-    if (lane == 0) seg_sh[i & 1] = s;
+    if (lane == 0) {
+      seg_sh[i & 1] = s;
+      mbar_arrive(&sb.planned);                // segment i is known (the loading warp reads it before the boundary)
+    }
     __syncwarp();
   };
   if (warp == WARP_PLAN) {
     plan_sum(p, pl, lane);
-    const long long N = pl.tiles[p.pool.B];
+    const long long N = pl.cost[p.pool.B];       // of all work
     const int U = pl.units[p.pool.B];
     if (even && lane < 2) p.header[2 * pid + lane] = make_int4(0, 0, 0, 0);
     __syncwarp();
-    // no share without a tile
-    if (N < C) C = (int)N;
+    if (N < (long long)C * MIN_SHARE) C = (int)min((long long)C, max((long long)U, (N + MIN_SHARE - 1) / MIN_SHARE));
     if (pid < C) {
       // about equal: no unit is over 1/8 longer than their mean
       if ((long long)pl.longest * U * 8 <= N * 9) waves = U / C;
       long long t0 = 0;
       if (waves > 0 && waves * C < U) {
         const Walk f = walk_to_unit(p, pl, waves * C, upt);
-        t0 = tiles_before(p, pl, f, upt, lane);
+        t0 = cost_before(p, pl, f, upt, lane);
       } else if (waves > 0) {
         t0 = N;
       }
       const long long rest = N - t0;
       t = t0 + rest * pid / C;
       t1 = t0 + rest * (pid + 1) / C;
-      t_first = t;
     }
     plan_next(0);
   }
@@ -477,64 +522,67 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 
   if (warp == WARP_LOAD) {
     setmaxnreg_dec<REG_OTHER>();
+    // a key tile: KROWS / kbox boxes; lane i holds page i's index, one lane issues
+    const int nkp = KROWS / p.kbox;
+    const int mask = (1 << p.pool.page_shift) - 1;
+    const int koff = NCTA == 2 ? KROWS * (int)rank : 0;
+    auto page_at = [&](const Seg& sg, int j) {
+      const int row = (sg.kv0 + j) * BN + koff + lane * p.kbox;
+      return lane < nkp && j < sg.n && row < sg.kv ? paged::raw_page_of(p.pool, sg.b, row) : 0;
+    };
+    auto load_k = [&](const Seg& sg, uint32_t dst, uint32_t bar, int j, int pages) {
+      const int row0 = nkp == 1 ? ((sg.kv0 + j) * BN + koff) & mask : 0;  // within a page that holds several boxes
+      pages = paged::checked_page(p.pool, pages, p.status);
+      const int head = sg.hk * p.k_head;
+      for_pages(head + pages * p.k_page, nkp, [&](int i, int line) {
+        load_5d<NCTA>(dst + i * p.kbox * 2 * D, &tm_k, bar, 0, 0, 0, row0 >> 3, line);
+      });
+    };
+    // q and the keys of the first tiles: for the next segment already while this one's output is written
+    auto begin = [&](const Seg& sg) {
+      int pk[NSBUF];
+#pragma unroll
+      for (int j = 0; j < NSBUF; ++j) pk[j] = page_at(sg, j);
+      const int n_pre = min(sg.n, NSBUF);
+      if (even && lane == 0) {
+        mbar_expect_tx(&sb.q_full, NCTA * (D / 64) * used * 128);
+        mbar_expect_tx(&sb.pre_full, NCTA * HALF_TILE * n_pre);
+      }
+      __syncwarp();
+      if (lane < D / 64)
+        load_3d<NCTA>(smem_u32(smem_q) + lane * Q_BOX, &tm_q, even_addr(&sb.q_full), 64 * lane, sg.hk * p.G,
+                      sg.s0 + sg.tok0 + (int)rank * p.tpc);
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < NSBUF; ++j)
+        if (j < n_pre) load_k(sg, smem_u32(pre) + j * HALF_TILE, even_addr(&sb.pre_full), j, pk[j]);
+    };
     int J0 = 0;
+    bool begun = false;
     for (int si = 0;; ++si) {
       const Seg sg = seg_sh[si & 1];
       if (sg.n == 0) break;
       const uint32_t sph = (uint32_t)si & 1u;
-      if (!aborted()) {
-        // boxes of a tile: keys first (KROWS / kbox pages x D / 64), values then (128 / vbox pages); a lane each
-        const int nkp = KROWS / p.kbox, nvp = BN / p.vbox;
-        const int kpg = lane % nkp, kch = lane / nkp;      // valid for lanes < nkp * D / 64
-        const bool klane = lane < nkp * (D / 64), vlane = lane < nvp;
-        auto page_at = [&](int row) {
-          return row < sg.kv ? paged::page_of(p.pool, sg.b, row, p.status) : 0;
-        };
-        const int mask = (1 << p.pool.page_shift) - 1;
-        const int koff = NCTA == 2 ? KROWS * (int)rank : 0;
-        auto krow = [&](int j) { return (sg.kv0 + j) * BN + koff + kpg * p.kbox; };
-        auto vrow = [&](int j) { return (sg.kv0 + j) * BN + lane * p.vbox; };
-        auto load_k = [&](uint32_t dst, uint32_t bar, int j, int pg) {
-          if (klane)
-            load_4d<NCTA>(dst + kch * K_BOX + kpg * p.kbox * 128, &tm_k, bar, 64 * kch, sg.hk, krow(j) & mask, pg);
-        };
-        if (even && lane == 0) mbar_expect_tx(&sb.q_full, NCTA * (D / 64) * used * 128);
-        __syncwarp();
-        const uint32_t qbar = even_addr(&sb.q_full);
-        if (lane < D / 64)
-          load_3d<NCTA>(smem_u32(smem_q) + lane * Q_BOX, &tm_q, qbar, 64 * lane, sg.hk * p.G,
-                        sg.s0 + sg.tok0 + (int)rank * p.tpc);
-        const int n_pre = min(sg.n, NSBUF);
-        if (even && lane == 0) mbar_expect_tx(&sb.pre_full, NCTA * HALF_TILE * n_pre);
-        __syncwarp();
-        int pk[NSBUF];
-#pragma unroll
-        for (int j = 0; j < NSBUF; ++j) pk[j] = j < n_pre && klane ? page_at(krow(j)) : 0;
-#pragma unroll
-        for (int j = 0; j < NSBUF; ++j)
-          if (j < n_pre) load_k(smem_u32(pre) + j * HALF_TILE, even_addr(&sb.pre_full), j, pk[j]);
-        // page indices one tile ahead
-        int kp = NSBUF < sg.n && klane ? page_at(krow(NSBUF)) : 0;
-        int vp = vlane ? page_at(vrow(0)) : 0;
+      if (!begun && !aborted()) {
+        begin(sg);
+        begun = true;
+      }
+      if (begun) {
+        int kp = page_at(sg, NSBUF);                 // page indices one tile ahead
         bool ok = true;
         for (int j = 0; j < sg.n; ++j) {
           const int J = J0 + j, st = J % NSTAGE;
           const bool has_k = j + NSBUF < sg.n, has_v = !ragged(sg, sg.kv0 + j);
-          const int kn = j + 1 + NSBUF < sg.n && klane ? page_at(krow(j + 1 + NSBUF)) : 0;
-          const int vn = j + 1 < sg.n && vlane ? page_at(vrow(j + 1)) : 0;
+          const int kn = page_at(sg, j + 1 + NSBUF);
           if (J >= NSTAGE &&
               !(ok = pwait_warp(&sb.stage_free[st], (uint32_t)(J / NSTAGE - 1) & 1u, cx, RW_STATUS_TIMEOUT_LOAD)))
             break;
           if (even && lane == 0)
             mbar_expect_tx(&sb.stage_full[st], NCTA * HALF_TILE * ((has_k ? 1 : 0) + (has_v ? 1 : 0)));
           __syncwarp();
-          const uint32_t bar = even_addr(&sb.stage_full[st]);
-          const uint32_t dst = smem_u32(stages) + st * STAGE_BYTES;
-          if (has_v && vlane)
-            load_4d<NCTA>(dst + lane * p.vbox * 128, &tm_v, bar, 64 * (int)rank, sg.hk, vrow(j) & mask, vp);
-          if (has_k) load_k(dst + HALF_TILE, bar, j + NSBUF, kp);
+          if (has_k)
+            load_k(sg, smem_u32(stages) + st * STAGE_BYTES + HALF_TILE, even_addr(&sb.stage_full[st]), j + NSBUF, kp);
           kp = kn;
-          vp = vn;
         }
         // every copy has landed and every stage is released before the barriers are set up for the next segment
         if (lane == 0) {
@@ -550,6 +598,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               mbar_wait_drain(&sb.stage_free[J % NSTAGE], (uint32_t)(J / NSTAGE) & 1u);
         }
         __syncwarp();
+        // (the last release follows every MMA of the segment: q and the first key tiles are read no more)
+        begun = false;
+        if (ok && pwait_warp(&sb.planned, (uint32_t)(si + 1) & 1u, cx, RW_STATUS_TIMEOUT_LOAD)) {
+          const Seg nx = seg_sh[(si + 1) & 1];
+          if (nx.n > 0 && !__any_sync(0xffffffffu, aborted())) {
+            begin(nx);
+            begun = true;
+          }
+        }
       }
       J0 += sg.n;
       boundary();
@@ -565,15 +622,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         constexpr uint32_t ID_QK = idesc<HALF>(NCTA * BM, BN, 0);
         constexpr uint32_t ID_PV = idesc<HALF>(NCTA * BM, D, 1);
         const uint64_t dq = umma_desc(smem_u32(smem_q), 16, 1024);
-        const uint64_t dk_pre = umma_desc(smem_u32(pre), 16, 1024);
+        const uint64_t dk_pre = umma_desc(smem_u32(pre), 16, K_GROUP);
         const uint64_t dv_st = umma_desc(smem_u32(stages), 16384, 1024);
-        const uint64_t dk_st = umma_desc(smem_u32(stages + HALF_TILE), 16, 1024);
+        const uint64_t dk_st = umma_desc(smem_u32(stages + HALF_TILE), 16, K_GROUP);
         constexpr uint64_t PRE_DESC = HALF_TILE >> 4, STAGE_DESC = STAGE_BYTES >> 4;
         auto issue_qk = [](uint32_t ts, uint64_t a, uint64_t b) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
             mma_ss_n<NCTA>(ts, a + (uint64_t)(((kk >> 2) * Q_BOX + (kk & 3) * 32) >> 4),
-                           b + (uint64_t)(((kk >> 2) * K_BOX + (kk & 3) * 32) >> 4), ID_QK, kk > 0 ? 1u : 0u);
+                           b + (uint64_t)(((kk >> 2) * 1024 + (kk & 3) * 32) >> 4), ID_QK, kk > 0 ? 1u : 0u);
         };
         auto issue_pv = [](uint32_t to, uint32_t ts, uint64_t b, bool acc) {
 #pragma unroll
@@ -626,14 +683,39 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       J0 += sg.n;
       boundary();
     }
-  } else if (warp == WARP_TAIL) {
+  } else if (warp == WARP_V) {
     setmaxnreg_dec<REG_OTHER>();
     int J0 = 0;
     for (int si = 0;; ++si) {
       const Seg sg = seg_sh[si & 1];
       if (sg.n == 0) break;
-      const int j = sg.n - 1;                  // only a unit's last tiles can be ragged, and only one of them is
-      if (ragged(sg, sg.kv0 + j) && !aborted()) {
+      // values: 128 / vbox boxes a tile, up to the last tile where the sequence ends inside it
+      const bool tail = ragged(sg, sg.kv0 + sg.n - 1);
+      if (!aborted()) {
+        const int nvp = BN / p.vbox, n = tail ? sg.n - 1 : sg.n;
+        const int mask = (1 << p.pool.page_shift) - 1;
+        auto page_at = [&](int j) {
+          const int row = (sg.kv0 + j) * BN + lane * p.vbox;
+          return lane < nvp && j < n ? paged::raw_page_of(p.pool, sg.b, row) : 0;
+        };
+        int vp = page_at(0);
+        for (int j = 0; j < n; ++j) {
+          const int J = J0 + j, st = J % NSTAGE;
+          const int vn = page_at(j + 1);
+          if (J >= NSTAGE &&
+              !pwait_warp(&sb.stage_free[st], (uint32_t)(J / NSTAGE - 1) & 1u, cx, RW_STATUS_TIMEOUT_LOAD))
+            break;
+          const uint32_t bar = even_addr(&sb.stage_full[st]), dst = smem_u32(stages) + st * STAGE_BYTES;
+          const int row0 = ((sg.kv0 + j) * BN) & mask;
+          vp = paged::checked_page(p.pool, vp, p.status);
+          for_pages(vp, nvp, [&](int i, int pg) {
+            load_4d<NCTA>(dst + i * p.vbox * 128, &tm_v, bar, 64 * (int)rank, sg.hk, nvp == 1 ? row0 : 0, pg);
+          });
+          vp = vn;
+        }
+      }
+      if (tail && !aborted()) {
+        const int j = sg.n - 1;                  // only a unit's last tile can be one
         const int J = J0 + j, st = J % NSTAGE;
         const int row0 = (sg.kv0 + j) * BN, rows = max(0, sg.kv - row0);
         const int c = lane & 7, r0 = lane >> 3;
@@ -710,22 +792,19 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         const int key0 = (sg.kv0 + j) * BN;
         const bool masked = key0 + BN > all;
         const int cut = lim - key0;              // columns from here on are not seen
-        auto load_quarter = [&](int q, uint32_t (&v)[32]) {
-          tmem_ld32(tS + 32 * q, v);
-          tmem_wait_ld();
-          reg_fence32(v);
-          if (masked) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (32 * q + e >= cut) v[e] = __float_as_uint(-INFINITY);
-          }
-        };
-        auto load_half = [&](int h, uint32_t (&v)[2][32]) {
+        auto load_half = [&](int h, uint32_t (&v)[2][32], const bool mask) {
           tmem_ld32(tS + 64 * h, v[0]);
           tmem_ld32(tS + 64 * h + 32, v[1]);
           tmem_wait_ld();
           reg_fence32(v[0]);
           reg_fence32(v[1]);
+          if (mask) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (64 * h + 32 * c + e >= cut) v[c][e] = __float_as_uint(-INFINITY);
+          }
         };
         auto quarter_max = [](const uint32_t (&v)[32], float row_max) -> float {
           float a[4];
@@ -766,7 +845,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t v[2][32];
-            load_half(h, v);
+            load_half(h, v, false);
             uint64_t lacc[2] = {0ull, 0ull};
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -794,10 +873,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         if (!fast) {
           if (!one_pass) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint32_t v[32];
-              load_quarter(q, v);
-              row_max = quarter_max(v, row_max);
+            for (int h = 0; h < 2; ++h) {
+              uint32_t v[2][32];
+              load_half(h, v, masked);
+              row_max = quarter_max(v[1], quarter_max(v[0], row_max));
             }
             if (j > 0) {
               const int Jp = J - 1;
@@ -842,12 +921,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           for (int h = 0; h < 2; ++h) {
             uint32_t pk[32];
             uint64_t lacc[2] = {0ull, 0ull};
+            uint32_t v[2][32];
+            load_half(h, v, masked);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              uint32_t v[32];
-              load_quarter(2 * h + c, v);
-              quarter_exp(v, s2, nm2, pk, 16 * c, lacc);
-            }
+            for (int c = 0; c < 2; ++c) quarter_exp(v[c], s2, nm2, pk, 16 * c, lacc);
             l2 = fadd2(l2, fadd2(lacc[0], lacc[1]));
             tmem_st32(tS + 32 * h, pk);
           }
@@ -893,7 +970,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           base[(long long)D * R + R + row] = l_row;
         }
       } else if (sg.slot < 0) {
-        // O / l in the type -> shared memory (over the Q tile, which no MMA reads any more) -> whole rows
+        // O / l in the type -> shared memory (the first stage, which no MMA reads any more and no load
+        // reaches before the boundary) -> whole rows
+        uint8_t* staged = stages;
         const float inv = l_row != 0.f ? 1.f / l_row : 0.f;
         if (ok && (warp & 3) * 32 < used) {         // a warp without a token has nothing to store
 #pragma unroll 1
@@ -911,10 +990,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               v.z = Num<HALF>::pack(__uint_as_float(o[8 * q + 4]) * inv, __uint_as_float(o[8 * q + 5]) * inv);
               v.w = Num<HALF>::pack(__uint_as_float(o[8 * q + 6]) * inv, __uint_as_float(o[8 * q + 7]) * inv);
               if (r < used)
-                *reinterpret_cast<uint4*>(smem_q + (ch >> 3) * Q_BOX + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v;
+                *reinterpret_cast<uint4*>(staged + (ch >> 3) * Q_BOX + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v;
             }
           }
         }
+        if (w == 0)
+          row_out[r] = there ? p.out + (long long)(sg.s0 + tok) * p.o_sl + (long long)(sg.hk * p.G + rg) * p.o_sh
+                             : nullptr;
         if (ok && w == 0 && there) {
           const long long at = (long long)(sg.s0 + tok) * p.Hq + sg.hk * p.G + rg;
           if (p.lse) p.lse[at] = l_row != 0.f ? (m_fin * sl2 + log2f(l_row)) * 0.6931471805599453f : -INFINITY;
@@ -924,14 +1006,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         constexpr int CH = D / 8;
         for (int i = threadIdx.x; ok && i < used * CH; i += SOFTMAX_THREADS) {
           const int rr = i / CH, ch = i % CH;
-          const int tk = rr / p.G, g = rr - tk * p.G;
-          const int tt = sg.tok0 + (int)rank * p.tpc + tk;
-          if (tt < sg.lq)
-            *reinterpret_cast<uint4*>(p.out + (long long)(sg.s0 + tt) * p.o_sl +
-                                      (long long)(sg.hk * p.G + g) * p.o_sh + 16 * ch) =
-                *reinterpret_cast<const uint4*>(smem_q + (ch >> 3) * Q_BOX + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4));
+          uint8_t* dst = row_out[rr];
+          if (dst != nullptr)
+            *reinterpret_cast<uint4*>(dst + 16 * ch) = *reinterpret_cast<const uint4*>(
+                staged + (ch >> 3) * Q_BOX + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4));
         }
-        fence_proxy_async_smem();                  // read before the next segment's Q is loaded over it
+        fence_proxy_async_smem();                  // read before the next segment's loads go there
       }
       J0 += sg.n;
       boundary();
@@ -962,41 +1042,53 @@ __global__ void __launch_bounds__(BM) join_kernel(const __grid_constant__ Params
   griddep_launch_dependents();
   griddep_wait();
   constexpr int R = Shape<D>::NCTA * BM;
-  const int s = blockIdx.x;
+  __shared__ int part[MAX_PARTS];
+  __shared__ int n_parts, n_before;
+  const int s = blockIdx.x, r = threadIdx.x;
   const int4 h = __ldcg(p.header + s);
   if (h.x == 0) return;
   auto same = [&](const int4& o) { return o.x == h.x && o.y == h.y && o.z == h.z; };
-  for (int o = s - 1; o >= 0; --o) {
-    const int4 x = __ldcg(p.header + o);
-    if (x.x == 0) continue;
-    if (same(x)) return;
-    break;
+  // the unit's slots from s on, in order (a unit's used slots follow one another); none may come before s
+  if (r == 0) { n_parts = 0; n_before = 0; }
+  __syncthreads();
+  for (int o = r; o < 2 * p.C; o += BM) {
+    if (!same(__ldcg(p.header + o))) continue;
+    if (o < s) n_before = 1; else atomicAdd(&n_parts, 1);
   }
-  const int rank = blockIdx.y, r = threadIdx.x, row = rank * BM + r, c0 = 32 * blockIdx.z;
+  __syncthreads();
+  if (n_before) return;
+  const int n = n_parts;
+  if (r < 32) {
+    // compaction by the first warp, in order
+    int at = 0;
+    for (int o0 = s; o0 < 2 * p.C && at < n; o0 += 32) {
+      const bool mine = o0 + r < 2 * p.C && same(__ldcg(p.header + o0 + r));
+      const unsigned m = __ballot_sync(0xffffffffu, mine);
+      if (mine) part[at + __popc(m & ((1u << r) - 1u))] = o0 + r;
+      at += __popc(m);
+    }
+  }
+  __syncthreads();
+  const int rank = blockIdx.y, row = rank * BM + r, c0 = 32 * blockIdx.z;
   const Seq sq = paged::load_seq(p.pool, h.x - 1, p.T, nullptr);
   const int rtok = r / p.G, g = r - rtok * p.G;
   const int tok = h.z + rank * p.tpc + rtok;
   if (r >= p.tpc * p.G || tok >= sq.lq) return;
+  const float* ml = p.scratch + (long long)D * R + row;
   float m = -INFINITY;
-  int end = s;
-  for (int o = s; o < 2 * p.C; ++o) {
-    const int4 x = __ldcg(p.header + o);
-    if (x.x == 0) continue;
-    if (!same(x)) break;
-    end = o;
-    m = fmaxf(m, __ldcg(p.scratch + (long long)o * Shape<D>::SLOT_FLOATS + (long long)D * R + row));
-  }
+#pragma unroll 8
+  for (int i = 0; i < n; ++i) m = fmaxf(m, __ldcg(ml + part[i] * Shape<D>::SLOT_FLOATS));
   float acc[32], l = 0.f;
 #pragma unroll
   for (int e = 0; e < 32; ++e) acc[e] = 0.f;
   const float base = m == -INFINITY ? 0.f : m;
-  for (int o = s; o <= end; ++o) {
-    if (__ldcg(&p.header[o].x) == 0) continue;
-    const float* sl = p.scratch + (long long)o * Shape<D>::SLOT_FLOATS;
-    const float f = fast_exp2((__ldcg(sl + (long long)D * R + row) - base) * p.scale_log2);
-    l += f * __ldcg(sl + (long long)D * R + R + row);
+#pragma unroll 2
+  for (int i = 0; i < n; ++i) {
+    const float* sl = p.scratch + part[i] * Shape<D>::SLOT_FLOATS + row;
+    const float f = fast_exp2((__ldcg(sl + (long long)D * R) - base) * p.scale_log2);
+    l += f * __ldcg(sl + (long long)D * R + R);
 #pragma unroll
-    for (int e = 0; e < 32; ++e) acc[e] += f * __ldcg(sl + (long long)(c0 + e) * R + row);
+    for (int e = 0; e < 32; ++e) acc[e] += f * __ldcg(sl + (long long)(c0 + e) * R);
   }
   const float inv = l != 0.f ? 1.f / l : 0.f;
   const int head = h.y * p.G + g;
@@ -1022,22 +1114,56 @@ inline CUtensorMapDataType dt(int dtype) {
   return dtype == RW_DTYPE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
 }
 
-// A pool as (D, Hkv, page_size, num_pages), boxes of 64 channels x 1 head x `rows` rows of a page.
-int pool_map(CUtensorMap* m, const rw_paged_t* c, bool values, int rows) {
+// The value pool as (D, Hkv, page_size, num_pages), boxes of 64 channels x 1 head x `rows` rows of a page.
+int value_map(CUtensorMap* m, const rw_paged_t* c, int rows) {
   EncodeTiledFn enc = encode_tiled_fn();
   if (!enc) return RW_ERR_DRIVER;
-  const void* ptr = values ? c->v : c->k;
-  long long sp = values ? c->v_sp : c->k_sp, sl = values ? c->v_sl : c->k_sl, sh = values ? c->v_sh : c->k_sh;
   // strides of dimensions of one are never used, but have to be valid
-  if (c->num_pages == 1) sp = 8;
-  if (c->Hkv == 1) sh = 8;
+  const long long sp = c->num_pages == 1 ? 8 : c->v_sp, sh = c->Hkv == 1 ? 8 : c->v_sh;
   cuuint64_t dims[4] = {(cuuint64_t)c->D, (cuuint64_t)c->Hkv, (cuuint64_t)c->page_size, (cuuint64_t)c->num_pages};
-  cuuint64_t strides[3] = {(cuuint64_t)sh * 2, (cuuint64_t)sl * 2, (cuuint64_t)sp * 2};
+  cuuint64_t strides[3] = {(cuuint64_t)sh * 2, (cuuint64_t)c->v_sl * 2, (cuuint64_t)sp * 2};
   cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1};
   cuuint32_t es[4] = {1, 1, 1, 1};
-  return enc(m, dt(c->dtype), 4, const_cast<void*>(ptr), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  return enc(m, dt(c->dtype), 4, c->v, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? RW_OK : RW_ERR_DRIVER;
+}
+
+// The key pool's head and page are one dimension of the map, in steps of the strides'
+// greatest common divisor (a map has five dimensions).
+struct KeyLines {
+  long long step, lines;  // elements; lines of the dimension
+};
+inline KeyLines key_lines(const rw_paged_t* c) {
+  long long a = c->num_pages == 1 ? 0 : c->k_sp, b = c->Hkv == 1 ? 0 : c->k_sh;
+  const long long last = (c->num_pages - 1) * a + (c->Hkv - 1) * b;
+  while (b) {
+    const long long r = a % b;
+    a = b;
+    b = r;
+  }
+  if (a == 0) a = 8;  // one page, one head
+  return {a, last / a + 1};
+}
+
+// The key pool as (64 channels, 8 rows, D / 64, page_size / 8, head and page), boxes of all
+// channels of `rows` rows of a page.
+int key_map(CUtensorMap* m, const rw_paged_t* c, int rows) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (!enc) return RW_ERR_DRIVER;
+  const KeyLines kl = key_lines(c);
+  cuuint64_t dims[5] = {64, 8, (cuuint64_t)(c->D / 64), (cuuint64_t)(c->page_size / 8), (cuuint64_t)kl.lines};
+  cuuint64_t strides[4] = {(cuuint64_t)c->k_sl * 2, 128, (cuuint64_t)c->k_sl * 16, (cuuint64_t)kl.step * 2};
+  cuuint32_t box[5] = {64, 8, (cuuint32_t)(c->D / 64), (cuuint32_t)(rows / 8), 1};
+  cuuint32_t es[5] = {1, 1, 1, 1, 1};
+  return enc(m, dt(c->dtype), 5, c->k, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? RW_OK : RW_ERR_DRIVER;
+}
+
+bool supported(const rw_paged_t* c) {
+  // coordinates are 32-bit, and a row's stride of 16 has to fit a map's
+  return c->B <= MAX_BATCH && key_lines(c).lines < (1ll << 31) && c->k_sl < (1ll << 35);
 }
 
 // q as (D, Hq, T), boxes of 64 channels x `heads` heads x `tokens` tokens.
@@ -1098,7 +1224,7 @@ int launch(const rw_paged_t* cache, const Pool& pool, const Call& c, void* works
   p.T = c.T; p.Hq = c.Hq; p.G = c.Hq / pool.Hkv; p.causal = c.causal;
   p.tpc = BM / p.G;
   p.C = grid_size(cache->D);
-  if (p.C < 1) return RW_ERR_CUDA;
+  if (p.C < 1 || 2 * p.C > MAX_PARTS) return RW_ERR_CUDA;
   p.scale_log2 = c.scale_log2;
   p.out = static_cast<uint8_t*>(c.out);
   p.o_sl = 2 * c.o_sl; p.o_sh = 2 * c.o_sh;
@@ -1109,10 +1235,13 @@ int launch(const rw_paged_t* cache, const Pool& pool, const Call& c, void* works
   const int krows = cache->D == 128 ? Shape<128>::KROWS : Shape<64>::KROWS;
   p.kbox = cache->page_size < krows ? cache->page_size : krows;
   p.vbox = cache->page_size < BN ? cache->page_size : BN;
+  const KeyLines kl = key_lines(cache);
+  p.k_head = cache->Hkv == 1 ? 0 : (int)(cache->k_sh / kl.step);
+  p.k_page = cache->num_pages == 1 ? 0 : (int)(cache->k_sp / kl.step);
   p.status = c.status;
   CUtensorMap mq, mk, mv;
   if (q_map(&mq, c.q, cache->dtype, c.T, c.Hq, cache->D, c.q_sl, c.q_sh, p.G, p.tpc) ||
-      pool_map(&mk, cache, false, p.kbox) || pool_map(&mv, cache, true, p.vbox))
+      key_map(&mk, cache, p.kbox) || value_map(&mv, cache, p.vbox))
     return RW_ERR_DRIVER;
   if (cache->dtype == RW_DTYPE_FP16)
     return cache->D == 128 ? launch_one<true, 128>(mq, mk, mv, p, st) : launch_one<true, 64>(mq, mk, mv, p, st);

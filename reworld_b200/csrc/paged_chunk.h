@@ -22,6 +22,7 @@ struct Call {
 
 int launch(const rw_paged_t* cache, const paged::Pool& pool, const Call& c, void* workspace, cudaStream_t st);
 long long workspace_bytes(int D);
+bool supported(const rw_paged_t* cache);
 
 }  // namespace chunk
 }  // namespace rw

@@ -11,7 +11,7 @@
 // tiles of one sequence, row tile and head), whole units, and the beginning of another.
 // Units that lie in one share are written out directly; the others leave their
 // unnormalised O, m and l in scratch, and the CTA that comes last to a unit (a counter)
-// joins its parts, in the order of the keys, so results do not depend on who is last.
+// joins its parts, always in the same order, so results do not depend on who is last.
 //
 // In a CTA each of the 4 warps takes 16 keys of a 64-key tile with a running maximum and
 // sum of its own (mma.sync m16n8k16 feeds far more than memory delivers here: a tile of
@@ -19,6 +19,8 @@
 // joined when the unit's tiles are done.  Keys and values come through a ring of 3 stages
 // of 16-byte cp.async; rows behind the last visible one are filled with zeros, never
 // read, so what a page holds there (NaN included) does not matter.
+#include <algorithm>
+
 #include "paged.cuh"
 #include "paged_chunk.h"
 
@@ -46,6 +48,7 @@ struct Params {
   float scale_log2;
   float* part;                  // [2 C][16 * D + 32]: O, then m, then l
   int* counters;                // [B * nrt * Hkv], zero before and after
+  int* header;                  // [2 C]: 1 + the unit of every part, 0: none (join_kernel joins); null: the last CTA joins
   // raw scores (log2 units) and (m, 1 / l) of every row, for the weight sums; null otherwise
   float* scores;                // [B * Hkv * nrt * 16][cap]
   float2* row_ml;               // [B * Hkv * nrt * 16]
@@ -110,6 +113,25 @@ __device__ __forceinline__ int tiles_of(const Entry& n) {
   return n.rows > 0 ? max(1, (n.keys + TILE - 1) / TILE) : 0;
 }
 
+// Channels c, c + 1 of row r of a unit: O / l, and with channel 0 the row's lse and (m, 1 / l).
+template <bool HALF>
+__device__ __forceinline__ void put_row(const Params& p, const Entry& en, int b, int hk, int r, int c, float2 v,
+                                        float mm, float ll) {
+  const int rr = en.row0 + r, tok = rr / p.G, g = rr - tok * p.G;
+  const float inv = ll != 0.f ? 1.f / ll : 0.f;
+  uint8_t* dst = p.out + (long long)(en.s.s0 + tok) * p.o_sl + (long long)(hk * p.G + g) * p.o_sh;
+  *reinterpret_cast<uint32_t*>(dst + 2 * c) = Num<HALF>::pack(v.x * inv, v.y * inv);
+  if (c == 0) {
+    if (p.lse)
+      p.lse[(long long)(en.s.s0 + tok) * p.Hq + hk * p.G + g] =
+          ll != 0.f ? (mm + log2f(ll)) * 0.6931471805599453f : -INFINITY;
+    if (p.row_ml) {
+      const long long line = (((long long)b * p.pool.Hkv + hk) * p.nrt + en.row0 / RT) * RT + r;
+      p.row_ml[line] = make_float2(mm == -INFINITY ? 0.f : mm, inv);
+    }
+  }
+}
+
 template <bool HALF, int D>
 __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant__ Params p) {
   constexpr int PITCH = 2 * D;               // bytes of a row in shared memory
@@ -150,6 +172,7 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
   }
   const long long N = base[THREADS];
   const int C = (int)max(1ll, min((long long)gridDim.x, N / p.min_tiles)), cta = blockIdx.x;
+  if (p.header && tid < 2) p.header[2 * cta + tid] = 0;
   if (cta >= C) return;
   const long long t0 = N * cta / C, t1 = N * (cta + 1) / C;
   if (t0 >= t1) return;
@@ -211,11 +234,12 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
     const int slot_mask = (1 << p.pool.page_shift) - 1;
     auto pages = [&](int j) {
       const int row = j * TILE + 8 * (lane & 7);
-      return (j < k1 && row < en.keys) ? paged::page_of(p.pool, b, row, p.status) : 0;
+      return (j < k1 && row < en.keys) ? paged::raw_page_of(p.pool, b, row) : 0;
     };
     auto load = [&](int j, int pg) {
       const uint32_t st = sbase + (uint32_t)((j - k0) % STAGES) * STAGE;
       const int c = tid % CH, r0 = tid / CH;
+      pg = paged::checked_page(p.pool, pg, p.status);
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         const int r = r0 + i * RSTEP;
@@ -357,23 +381,10 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
     __syncthreads();
 
     const bool whole = k0 == 0 && k1 == n_tiles;
+    if (p.header && !whole && tid == 0) p.header[2 * cta + (t == t0 ? 0 : 1)] = 1 + e * p.pool.Hkv + hk;
     float* slot = p.part + (long long)(2 * cta + (t == t0 ? 0 : 1)) * SLOT;
+    auto put = [&](int r, int c, float2 v, float mm, float ll) { put_row<HALF>(p, en, b, hk, r, c, v, mm, ll); };
     // 2 channels of a row a thread and step
-    auto put = [&](int r, int c, float2 v, float mm, float ll) {
-      const int rr = en.row0 + r, tok = rr / p.G, g = rr - tok * p.G;
-      const float inv = ll > 0.f ? 1.f / ll : 0.f;
-      uint8_t* dst = p.out + (long long)(s.s0 + tok) * p.o_sl + (long long)(hk * p.G + g) * p.o_sh;
-      *reinterpret_cast<uint32_t*>(dst + 2 * c) = Num<HALF>::pack(v.x * inv, v.y * inv);
-      if (c == 0) {
-        if (p.lse)
-          p.lse[(long long)(s.s0 + tok) * p.Hq + hk * p.G + g] =
-              ll > 0.f ? (mm + log2f(ll)) * 0.6931471805599453f : -INFINITY;
-        if (p.row_ml) {
-          const long long line = (((long long)b * p.pool.Hkv + hk) * p.nrt + en.row0 / RT) * RT + r;
-          p.row_ml[line] = make_float2(mm == -INFINITY ? 0.f : mm, inv);
-        }
-      }
-    };
     for (int i = tid; i < en.rows * (D / 2); i += THREADS) {
       const int r = i / (D / 2), c = 2 * (i % (D / 2));
       float mm = sm_m[0][r];
@@ -400,7 +411,7 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
         }
       }
     }
-    if (!whole) {
+    if (!whole && !p.header) {
       // the CTAs whose shares meet the unit: the one that holds tile u0 to the one that holds u1 - 1
       auto owner = [&](long long x) {        // largest c with N c / C <= x
         long long c = (x * C) / N;
@@ -414,36 +425,145 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
       __syncthreads();
       if (tid == 0) come = atomicAdd(counter, 1);
       __syncthreads();
-      // shares that hold no tile (N < C) leave no part
-      int parts = 0;
-      for (int c = ca; c <= cb; ++c) parts += N * c / C < N * (c + 1) / C;
+      const int parts = cb - ca + 1;         // (C <= N: every share has a tile)
       if (come == parts - 1) {
         __threadfence();
         if (tid == 0) *counter = 0;          // ready for the next call
-        for (int i = tid; i < en.rows * (D / 2); i += THREADS) {
-          const int r = i / (D / 2), c = 2 * (i % (D / 2));
-          float mm = -INFINITY, ll = 0.f;
-          float2 v = make_float2(0.f, 0.f);
-          for (int cc = ca; cc <= cb; ++cc) {
-            const long long c0 = N * cc / C;
-            if (c0 >= N * (cc + 1) / C) continue;
-            const float* sl = p.part + (long long)(2 * cc + (c0 >= u0 ? 0 : 1)) * SLOT;
-            const float m2 = __ldcg(sl + RT * D + r), l2 = __ldcg(sl + RT * D + RT + r);
-            const float2 x = __ldcg(reinterpret_cast<const float2*>(sl + r * D + c));
-            const float mn = fmaxf(mm, m2), bs = mn == -INFINITY ? 0.f : mn;
-            const float fa = fast_exp2(mm - bs), fb = fast_exp2(m2 - bs);
-            v.x = v.x * fa + x.x * fb;
-            v.y = v.y * fa + x.y * fb;
-            ll = ll * fa + l2 * fb;
-            mm = mn;
+        // part i of the unit, from CTA ca + i: in that CTA's first slot unless its share began before the unit
+        auto slot_of = [&](int i) {
+          return p.part + (2LL * (ca + i) + (i == 0 && N * ca / C < u0 ? 1 : 0)) * SLOT;
+        };
+        // factor of every part and row, [parts][16], and the rows' m and l; a warp has 4 rows
+        float* fac = reinterpret_cast<float*>(smem);
+        for (int i = tid; i < parts * RT; i += THREADS) fac[i] = __ldcg(slot_of(i / RT) + RT * D + i % RT);
+        __syncthreads();
+        for (int r = warp * 4; r < warp * 4 + 4; ++r) {
+          float mm = -INFINITY;
+          for (int i = lane; i < parts; i += 32) mm = fmaxf(mm, fac[i * RT + r]);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+          const float bs = mm == -INFINITY ? 0.f : mm;
+          float ll = 0.f;
+          for (int i = lane; i < parts; i += 32) {
+            const float f = fast_exp2(fac[i * RT + r] - bs);
+            fac[i * RT + r] = f;
+            ll += f * __ldcg(slot_of(i) + RT * D + RT + r);
           }
-          put(r, c, v, mm, ll);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
+          if (lane == 0) {
+            sm_m[0][r] = mm;
+            sm_l[0][r] = ll;
+          }
+        }
+        __syncthreads();
+        // 4 channels of a row a thread and step; 16 parts' loads under way at once
+        for (int i = tid; i < en.rows * (D / 4); i += THREADS) {
+          const int r = i / (D / 4), c = 4 * (i % (D / 4));
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          auto add = [&](const float4& x, float f) {
+            v.x += f * x.x;
+            v.y += f * x.y;
+            v.z += f * x.z;
+            v.w += f * x.w;
+          };
+          // the first part may be in its CTA's second slot; the others lie 2 SLOT apart
+          add(__ldcg(reinterpret_cast<const float4*>(slot_of(0) + r * D + c)), fac[r]);
+          const float* at = p.part + 2LL * ca * SLOT + r * D + c;
+#pragma unroll 16
+          for (int k = 1; k < parts; ++k)
+            add(__ldcg(reinterpret_cast<const float4*>(at + 2LL * k * SLOT)), fac[k * RT + r]);
+          put(r, c, make_float2(v.x, v.y), sm_m[0][r], sm_l[0][r]);
+          put(r, c + 2, make_float2(v.z, v.w), sm_m[0][r], sm_l[0][r]);
         }
       }
     }
     __syncthreads();                         // shared memory is free for the next segment
     t = u0 + k1;
   }
+}
+
+// Joins the parts of the units that more than one CTA worked on, where units are few and
+// have many parts: a block takes one row of one unit, its 8 groups of D / 4 threads every
+// eighth part each.  (One CTA joining 148 parts of 8 rows, 600 KB, took 35 us.)
+constexpr int JOIN_GROUPS = 8;
+constexpr int WIDE_JOIN = 8;     // CTAs a unit, from which on this kernel joins
+constexpr int MAX_PARTS = 2048;
+
+template <bool HALF, int D>
+__global__ void __launch_bounds__(JOIN_GROUPS * D / 4) join_kernel(const __grid_constant__ Params p, int C) {
+  constexpr int SLOT = RT * D + 2 * RT;
+  constexpr int NT = JOIN_GROUPS * D / 4;
+  __shared__ int part[MAX_PARTS];
+  __shared__ float fac[MAX_PARTS];
+  __shared__ int n_sh;
+  __shared__ float red[2];
+  __shared__ float4 acc[JOIN_GROUPS][D / 4];
+  griddep_launch_dependents();
+  griddep_wait();
+  const int u = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+  const int e = u / p.pool.Hkv, hk = u - e * p.pool.Hkv;
+  const Entry en = load_entry(p, e, nullptr);
+  if (r >= en.rows) return;
+  if (tid < 32) {
+    int n = 0;
+#pragma unroll 4
+    for (int o0 = 0; o0 < 2 * C; o0 += 32) {
+      const bool mine = o0 + lane < 2 * C && __ldcg(p.header + o0 + lane) == u + 1;
+      const unsigned m = __ballot_sync(0xffffffffu, mine);
+      if (mine) part[n + __popc(m & ((1u << lane) - 1u))] = o0 + lane;
+      n += __popc(m);
+    }
+    __syncwarp();
+    float mm = -INFINITY;
+    for (int i = lane; i < n; i += 32) {
+      fac[i] = __ldcg(p.part + (long long)part[i] * SLOT + RT * D + r);
+      mm = fmaxf(mm, fac[i]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+    const float bs = mm == -INFINITY ? 0.f : mm;
+    float ll = 0.f;
+    for (int i = lane; i < n; i += 32) {
+      fac[i] = fast_exp2(fac[i] - bs);
+      ll += fac[i] * __ldcg(p.part + (long long)part[i] * SLOT + RT * D + RT + r);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
+    if (lane == 0) {
+      n_sh = n;
+      red[0] = mm;
+      red[1] = ll;
+    }
+  }
+  __syncthreads();
+  const int n = n_sh;
+  if (n == 0) return;                          // one CTA did it all, and wrote it
+  const int g = tid / (D / 4), c = 4 * (tid % (D / 4));
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int i = g; i < n; i += JOIN_GROUPS) {
+    const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part + (long long)part[i] * SLOT + r * D + c));
+    const float f = fac[i];
+    v.x += f * x.x;
+    v.y += f * x.y;
+    v.z += f * x.z;
+    v.w += f * x.w;
+  }
+  acc[g][c / 4] = v;
+  __syncthreads();
+  if (g != 0) return;
+#pragma unroll
+  for (int i = 1; i < JOIN_GROUPS; ++i) {
+    const float4 x = acc[i][c / 4];
+    v.x += x.x;
+    v.y += x.y;
+    v.z += x.z;
+    v.w += x.w;
+  }
+  const int b = e / p.nrt;
+  put_row<HALF>(p, en, b, hk, r, c, make_float2(v.x, v.y), red[0], red[1]);
+  put_row<HALF>(p, en, b, hk, r, c + 2, make_float2(v.z, v.w), red[0], red[1]);
 }
 
 // sums[b, hk, j] += sum over the rows of exp2(score - m) / l, rows in their order.
@@ -495,13 +615,14 @@ inline int grid_size(int D) {
 inline bool on_tensor_tiles(int B, long long nrt) { return nrt > 1 && B <= chunk::MAX_BATCH; }
 
 struct Layout {
-  long long part, ml, scores, total;  // byte offsets
+  long long part, header, ml, scores, total;  // byte offsets
 };
 
 inline Layout layout(int D, int C, int B, int Hkv, int nrt, long long cap, bool sums) {
   Layout l;
   l.part = 0;
-  l.ml = (2LL * C * (RT * D + 2 * RT) * 4 + 255) & ~255LL;
+  l.header = (2LL * C * (RT * D + 2 * RT) * 4 + 255) & ~255LL;
+  l.ml = (l.header + 8LL * C + 255) & ~255LL;
   const long long lines = (long long)B * Hkv * nrt * RT;
   l.scores = l.ml + (sums ? (lines * 8 + 255) & ~255LL : 0);
   l.total = l.scores + (sums ? lines * cap * 4 : 0);
@@ -513,8 +634,12 @@ int launch_rows(const Params& p, int C, cudaStream_t stream) {
   static std::atomic<unsigned long long> done{0};
   const int bytes = STAGES * 2 * TILE * 2 * D;
   if (!ensure_smem_attr(reinterpret_cast<const void*>(rows_kernel<HALF, D>), bytes, &done)) return RW_ERR_CUDA;
-  return launch_dependent(rows_kernel<HALF, D>, dim3(C), dim3(THREADS), bytes, stream, p) == cudaSuccess ? RW_OK
-                                                                                                       : RW_ERR_CUDA;
+  if (launch_dependent(rows_kernel<HALF, D>, dim3(C), dim3(THREADS), bytes, stream, p) != cudaSuccess)
+    return RW_ERR_CUDA;
+  if (!p.header) return RW_OK;
+  const dim3 grid(p.pool.B * p.nrt * p.pool.Hkv, std::min(RT, p.T * p.G));
+  return launch_dependent(join_kernel<HALF, D>, grid, dim3(JOIN_GROUPS * D / 4), 0, stream, p, C) == cudaSuccess
+             ? RW_OK : RW_ERR_CUDA;
 }
 
 }  // namespace rows
@@ -542,14 +667,14 @@ extern "C" int rw_paged_attn(const rw_paged_t* cache, const void* q, void* out, 
   const long long cap = (long long)cache->table_width * cache->page_size;
   const float scale_log2 = softmax_scale * 1.4426950408889634f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (rows::on_tensor_tiles(cache->B, nrt) && !sums) {
+  if (rows::on_tensor_tiles(cache->B, nrt) && !sums && chunk::supported(cache)) {
     if (!workspace || !aligned16(workspace) || workspace_bytes < chunk::workspace_bytes(cache->D))
       return RW_ERR_INVALID_ARG;
     const chunk::Call c{q, out, lse, nullptr, T, Hq, causal != 0, q_sl, q_sh, o_sl, o_sh, scale_log2, status};
     return chunk::launch(cache, p.pool, c, workspace, st);
   }
   const int C = rows::grid_size(cache->D);
-  if (C == 0) return RW_ERR_CUDA;
+  if (C == 0 || 2 * C > rows::MAX_PARTS) return RW_ERR_CUDA;
   const rows::Layout lay = rows::layout(cache->D, C, cache->B, p.pool.Hkv, (int)nrt, cap, sums != nullptr);
   if (!workspace || !aligned16(workspace) || workspace_bytes < lay.total || !counters ||
       n_counters < rows::counters_needed(cache->B, p.pool.Hkv, (int)nrt))
@@ -564,6 +689,9 @@ extern "C" int rw_paged_attn(const rw_paged_t* cache, const void* q, void* out, 
   p.scale_log2 = scale_log2;
   p.part = reinterpret_cast<float*>(ws + lay.part);
   p.counters = counters;
+  // Where a unit can have many parts, they are joined by a kernel of their own: with 1 sequence of 131072 rows and
+  // 2 key heads @@; where it has few, by the last CTA that comes to it, without another launch.
+  if ((long long)C > rows::WIDE_JOIN * cache->B * p.pool.Hkv * nrt) p.header = reinterpret_cast<int*>(ws + lay.header);
   p.scores = sums ? reinterpret_cast<float*>(ws + lay.scores) : nullptr;
   p.row_ml = sums ? reinterpret_cast<float2*>(ws + lay.ml) : nullptr;
   p.cap = cap;
@@ -594,7 +722,7 @@ extern "C" long long rw_paged_attn_workspace_bytes(int T, int Hq, int Hkv, int D
     return 0;
   const long long nrt = ((long long)(max_q_len < T ? max_q_len : T) * (Hq / Hkv) + rows::RT - 1) / rows::RT;
   if (nrt * B * Hkv > (1ll << 30)) return 0;
-  if (rows::on_tensor_tiles(B, nrt) && !with_sums) return chunk::workspace_bytes(D);
   if (n_counters) *n_counters = rows::counters_needed(B, Hkv, (int)nrt);
-  return rows::layout(D, rows::grid_size(D), B, Hkv, (int)nrt, cache_rows, with_sums != 0).total;
+  const long long own = rows::layout(D, rows::grid_size(D), B, Hkv, (int)nrt, cache_rows, with_sums != 0).total;
+  return rows::on_tensor_tiles(B, nrt) && !with_sums ? std::max(own, chunk::workspace_bytes(D)) : own;
 }
