@@ -487,7 +487,9 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
 // have many parts: a block takes one row of one unit, its 8 groups of D / 4 threads every
 // eighth part each.  (One CTA joining 148 parts of 8 rows, 600 KB, took 35 us.)
 constexpr int JOIN_GROUPS = 8;
-constexpr int WIDE_JOIN = 8;     // CTAs a unit, from which on this kernel joins
+// Parts a unit, above which this kernel joins: 2 units of 8 parts 18.4 us without and 20.5 with it, 24 units of 12
+// parts 38.9 and 34.8 (4000 rows), 4 units of 74 parts 86 and 74, 1 unit of 296 parts 86 and 51.
+constexpr int WIDE_JOIN = 10;
 constexpr int MAX_PARTS = 2048;
 
 template <bool HALF, int D>
@@ -689,9 +691,10 @@ extern "C" int rw_paged_attn(const rw_paged_t* cache, const void* q, void* out, 
   p.scale_log2 = scale_log2;
   p.part = reinterpret_cast<float*>(ws + lay.part);
   p.counters = counters;
-  // Where a unit can have many parts, they are joined by a kernel of their own: with 1 sequence of 131072 rows and
-  // 2 key heads @@; where it has few, by the last CTA that comes to it, without another launch.
-  if ((long long)C > rows::WIDE_JOIN * cache->B * p.pool.Hkv * nrt) p.header = reinterpret_cast<int*>(ws + lay.header);
+  // Where a unit can have many parts (CTAs a unit, tiles of a unit), they are joined by a kernel of their own; where
+  // it has few, by the last CTA that comes to it, without another launch.
+  if (std::min((long long)C / (cache->B * p.pool.Hkv * nrt), cap / rows::TILE) > rows::WIDE_JOIN)
+    p.header = reinterpret_cast<int*>(ws + lay.header);
   p.scores = sums ? reinterpret_cast<float*>(ws + lay.scores) : nullptr;
   p.row_ml = sums ? reinterpret_cast<float2*>(ws + lay.ml) : nullptr;
   p.cap = cap;

@@ -26,6 +26,7 @@ the landmark bank's eviction (longctx/inference/landmark_cache_v2.py:465-479) by
 attention weight instead of pose.
 """
 import ctypes
+import functools
 import math
 
 import torch
@@ -36,92 +37,101 @@ from ._native import RwPaged
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 
 
+def _stream(device):
+    """Handle of the device's current stream (what torch.cuda.current_stream(device).cuda_stream is)."""
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
 # ------------------------------------------------------------------ arguments
+# (A decoding step is a few microseconds of GPU time: the checks look at each property once.)
 
-def _check_heads(t, name, dtype, device):
-    """A packed [T, heads, D] tensor that the kernels can read as it is."""
-    if t.dim() != 3 or t.dtype != dtype or t.device != device:
-        raise ValueError(f"{name} must be a {dtype} [T, heads, D] tensor on {device}")
-    if not _heads_ok(t):
-        raise ValueError(f"{name}: channels must be contiguous, 16-byte aligned, other strides multiples of 8")
-    return t
-
-
-def _heads_ok(t):
-    st = t.stride()
-    return st[2] == 1 and st[0] % 8 == 0 and st[1] % 8 == 0 and t.data_ptr() % 16 == 0 and \
-        (st[0] > 0 or t.shape[0] == 1) and (st[1] > 0 or t.shape[1] == 1)
-
-
-def _in(t, name, dtype, device):
-    """Same for an input: one that the kernels cannot read as it is gets copied."""
-    if t.dim() != 3 or t.dtype != dtype or t.device != device:
-        raise ValueError(f"{name} must be a {dtype} [T, heads, D] tensor on {device}")
-    return t if _heads_ok(t) else t.contiguous().clone() if t.is_contiguous() else t.contiguous()
+def _heads(t, name, dtype, dev):
+    """(strides, data pointer) of a packed [T, heads, D] tensor, which the kernels read or write as it is."""
+    if t.dtype != dtype or t.device != dev or t.dim() != 3:
+        raise ValueError(f"{name} must be a {dtype} [T, heads, D] tensor on {dev}")
+    st, ptr = t.stride(), t.data_ptr()
+    if st[2] != 1 or st[0] % 8 or st[1] % 8 or ptr % 16 or st[0] <= 0 or st[1] <= 0:
+        T, H, _ = t.shape
+        if st[2] != 1 or (T > 1 and (st[0] % 8 or st[0] <= 0)) or (H > 1 and (st[1] % 8 or st[1] <= 0)) or ptr % 16:
+            raise ValueError(f"{name}: channels must be contiguous, 16-byte aligned, other strides multiples of 8")
+        # strides of a dimension of one are never used, but have to be valid
+        st = (st[0] if T > 1 else 8, st[1] if H > 1 else 8, 1)
+    return st, ptr
 
 
-def _ints(t, name, shape, device):
-    if t.dtype != torch.int32 or t.device != device or tuple(t.shape) != shape:
-        raise ValueError(f"{name} must be an int32 {list(shape)} tensor on {device}")
-    if t.dim() == 1 and t.shape[0] > 1 and t.stride(0) != 1:
-        raise ValueError(f"{name} must be contiguous")
-    return t
+def _in(t, name, dtype, dev):
+    """(tensor, strides, data pointer) of an input: one that the kernels cannot read as it is gets copied."""
+    try:
+        return (t, *_heads(t, name, dtype, dev))
+    except ValueError:
+        if t.dtype != dtype or t.device != dev or t.dim() != 3:
+            raise
+        t = t.clone(memory_format=torch.contiguous_format)
+        return (t, *_heads(t, name, dtype, dev))
+
+
+def _ints(t, name, n, dev):
+    """Data pointer of a contiguous int32 vector."""
+    if t.dtype != torch.int32 or t.device != dev or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name} must be a contiguous int32 [{n}] tensor on {dev}")
+    return t.data_ptr()
+
+
+def _table(t, name, dev):
+    """(sequences, pages of each, stride, data pointer) of a block table."""
+    if t.dtype != torch.int32 or t.device != dev or t.dim() != 2:
+        raise ValueError(f"{name} must be an int32 [B, pages] tensor on {dev}")
+    B, width = t.shape
+    s0, s1 = t.stride()
+    if (width > 1 and s1 != 1) or (B > 1 and s0 < width):
+        raise ValueError(f"{name}: a sequence's pages must be contiguous, and rows apart")
+    return B, width, s0 if B > 1 and s0 > width else width, t.data_ptr()
 
 
 def _cache(k_pages, v_pages, block_table, kv_lens, q_starts=None):
     dev, dt = k_pages.device, k_pages.dtype
     if dev.type != "cuda":
         raise ValueError("a paged cache lives on a CUDA device")
-    if dt not in _DTYPES:
+    code = _DTYPES.get(dt)
+    if code is None:
         raise ValueError("a paged cache is bf16 or fp16")
-    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype != dt or v_pages.device != dev:
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype != dt or v_pages.device != dev:
         raise ValueError("k_pages and v_pages must be alike, [num_pages, page_size, Hkv, D]")
-    n, page, hkv, D = k_pages.shape
-    if D not in (64, 128):
+    n, page, hkv, D = shape
+    if D != 128 and D != 64:
         raise NotImplementedError(f"head_dim {D}: the paged kernels have 64 and 128")
     if page < 8 or page & (page - 1):
         raise NotImplementedError(f"page_size {page}: must be a power of two >= 8")
     if n < 1 or hkv < 1:
         raise ValueError("the pools have no pages or heads")
-    ks, vs = k_pages.stride(), v_pages.stride()
-    for t, st, name in ((k_pages, ks, "k_pages"), (v_pages, vs, "v_pages")):
-        if st[3] != 1 or t.data_ptr() % 16 or any(s <= 0 or s % 8 for s in st[:3]):
-            raise ValueError(f"{name}: channels must be contiguous, 16-byte aligned, other strides multiples of 8")
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.device != dev:
-        raise ValueError(f"block_table must be an int32 [B, pages] tensor on {dev}")
-    B, width = block_table.shape
-    ts = _table_stride(block_table, "block_table")
-    _ints(kv_lens, "kv_lens", (B,), dev)
-    if q_starts is not None:
-        _ints(q_starts, "q_starts", (B + 1,), dev)
-    return RwPaged(k_pages.data_ptr(), v_pages.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], n, page, hkv, D,
-                   _DTYPES[dt], B, width, 0, block_table.data_ptr() or k_pages.data_ptr(), ts,
-                   q_starts.data_ptr() if q_starts is not None else None,
-                   kv_lens.data_ptr() or k_pages.data_ptr())
+    a, b, c, d = k_pages.stride()
+    e, f, g, h = v_pages.stride()
+    kp, vp = k_pages.data_ptr(), v_pages.data_ptr()
+    if d != 1 or h != 1 or (a | b | c | e | f | g) % 8 or (kp | vp) % 16 or min(a, b, c, e, f, g) <= 0:
+        raise ValueError("k_pages, v_pages: channels must be contiguous, 16-byte aligned, other strides multiples of 8")
+    B, width, ts, tp = _table(block_table, "block_table", dev)
+    lp = _ints(kv_lens, "kv_lens", B, dev)
+    sp = _ints(q_starts, "q_starts", B + 1, dev) if q_starts is not None else None
+    return RwPaged(kp, vp, a, b, c, e, f, g, n, page, hkv, D, code, B, width, 0, tp or kp, ts, sp, lp or kp)
 
 
-def _table_stride(t, name):
-    B, width = t.shape
-    if width > 1 and t.stride(1) != 1:
-        raise ValueError(f"{name}: a sequence's pages must be contiguous")
-    if B > 1 and t.stride(0) < width:
-        raise ValueError(f"{name}: rows overlap")
-    return max(t.stride(0), width) if B > 1 else width
+_scratch = {}
 
 
-_counters = {}
-
-
-def _zeroed(device, n, stream):
-    """Counters that every call leaves zero: one buffer for each stream, since calls on
-    different streams may overlap; a captured call gets one of its own graph's memory."""
+def _workspace(dev, stream, nbytes, ncounters):
+    """(workspace, counters) of a call: kept for each stream, since calls on different streams may
+    overlap (every call leaves the counters zero); a captured call has its own, of its graph's memory."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(n, dtype=torch.int32, device=device)
-    key = (device.index, stream)
-    t = _counters.get(key)
-    if t is None or t.numel() < n:
-        t = _counters[key] = torch.zeros(max(n, 1 << 14), dtype=torch.int32, device=device)
-    return t
+        return (torch.empty(nbytes, dtype=torch.uint8, device=dev),
+                torch.zeros(ncounters, dtype=torch.int32, device=dev))
+    key = (dev.index, stream)
+    kept = _scratch.get(key)
+    if kept is None or kept[0].numel() < nbytes or kept[1].numel() < ncounters:
+        old = (0, 0) if kept is None else (kept[0].numel(), kept[1].numel())
+        kept = _scratch[key] = (torch.empty(max(nbytes, old[0]), dtype=torch.uint8, device=dev),
+                                torch.zeros(max(ncounters, old[1], 1 << 14), dtype=torch.int32, device=dev))
+    return kept
 
 
 class _on:
@@ -200,66 +210,59 @@ def rotary(x, table, positions, interleaved=False, out=None):
     table: rotary_table(...); its rotary_dim first channels turn, the others pass.
     positions: int32 [T].  interleaved: pairs (2i, 2i + 1), else (i, i + rotary_dim / 2).
     out may be x.  One launch of rw_rotary."""
-    if not x.is_cuda or x.dtype not in _DTYPES or x.dim() != 3:
+    dev, dt = x.device, x.dtype
+    if dev.type != "cuda" or dt not in _DTYPES or x.dim() != 3:
         raise ValueError("rotary runs on bf16 or fp16 CUDA tensors [T, heads, D]")
     T, H, D = x.shape
     if D not in (64, 128):
         raise NotImplementedError(f"head_dim {D}: the rotary kernel has 64 and 128")
-    dev = x.device
     tab = _table_args(table, D, dev)
-    _ints(positions, "positions", (T,), dev)
-    src = _in(x, "x", x.dtype, dev)
+    pp = _ints(positions, "positions", T, dev)
+    src, xs, xp = _in(x, "x", dt, dev)
     if out is None:
-        out = torch.empty((T, H, D), dtype=x.dtype, device=dev)
-    else:
-        _check_out(out, "out", src, (T, H, D), x)
+        out = torch.empty((T, H, D), dtype=dt, device=dev)
+    os, op = _out(out, "out", x, (T, H, D), dt, dev)
     if T == 0 or H == 0:
         return out
     with _on(dev):
-        code = _native.lib().rw_rotary(src.data_ptr(), out.data_ptr(), T, H, D, _DTYPES[x.dtype], *_sl_sh(src),
-                                       *_sl_sh(out), *tab, int(interleaved), positions.data_ptr(),
-                                       _native.status_tensor(dev).data_ptr(), _native.stream_ptr(dev))
+        code = _native.lib().rw_rotary(xp, op, T, H, D, _DTYPES[dt], xs[0], xs[1], os[0], os[1], *tab,
+                                       int(interleaved), pp, _native.status_tensor(dev).data_ptr(), _stream(dev.index))
     _native.check(code, "rw_rotary")
     return out
 
 
-def _sl_sh(t):
-    """Strides of token and head; those of a dimension of one are never used, but must be valid."""
-    T, H, D = t.shape
-    return (t.stride(0) if T > 1 else H * D), (t.stride(1) if H > 1 else D)
-
-
 def _span(t):
-    """First and last byte of a tensor's elements."""
+    """First byte of a tensor's elements, and the one behind them."""
     lo = t.data_ptr()
     return lo, lo + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
 
 
-def _check_out(out, name, src, shape, given):
-    """An output tensor of the caller's: its form, and that it is the input itself or apart from it."""
+def _meet(a, b):
+    """Whether two tensors may share bytes (two slices of the rows of one packed tensor do not)."""
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    if a1 <= b0 or b1 <= a0:
+        return False
+    if a.stride() == b.stride() and a.shape[0] == b.shape[0] and a.shape[0] > 1:
+        # heads [i, j) and [k, l) of the same rows
+        row = a.stride(0) * a.element_size()
+        wa, wb = (t.element_size() * (1 + (t.shape[1] - 1) * t.stride(1) + t.shape[2] - 1) for t in (a, b))
+        lo, hi, wlo = (a0, b0, wa) if a0 < b0 else (b0, a0, wb)
+        whi = wb if a0 < b0 else wa
+        d = hi - lo
+        return not (wlo <= d and d + whi <= row)
+    return True
+
+
+def _out(out, name, given, shape, dt, dev):
+    """(strides, data pointer) of an output, which must be the input itself or apart from it."""
     if tuple(out.shape) != shape:
         raise ValueError(f"{name} must have the shape {list(shape)}")
-    _check_heads(out, name, src.dtype, src.device)
-    for n, s in zip(out.shape, out.stride()):
-        if n > 1 and s == 0:
-            raise ValueError(f"{name} must not be an expanded tensor")
-    if out.numel() and src is given and not (out.data_ptr() == src.data_ptr() and out.stride() == src.stride()):
-        a, b = _span(out), _span(src)
-        if a[0] < b[1] and b[0] < a[1] and out.untyped_storage().data_ptr() == src.untyped_storage().data_ptr() and \
-                not _interleave(out, src):
-            raise ValueError(f"{name} overlaps its input without being it")
-
-
-def _interleave(a, b):
-    """Whether two views with the same strides (slices of one packed q|k|v row, say) cannot meet."""
-    if a.stride() != b.stride() or a.stride(0) <= 0 or a.shape[0] < 2:
-        return False
-    row = a.stride(0) * a.element_size()
-    width = [t.element_size() * (1 + (t.shape[1] - 1) * t.stride(1) + t.shape[2] - 1) for t in (a, b)]
-    if max(width) > row:
-        return False
-    d = (a.data_ptr() - b.data_ptr()) % row
-    return d >= width[1] and d + width[0] <= row
+    st, ptr = _heads(out, name, dt, dev)
+    if given is not None and out is not given and out.numel() and \
+            not (ptr == given.data_ptr() and out.stride() == given.stride() and given.shape == out.shape) and \
+            _meet(out, given):
+        raise ValueError(f"{name} overlaps its input without being it")
+    return st, ptr
 
 
 def paged_rotary_store(k, v, k_pages, v_pages, block_table, q_starts, kv_lens, table=None, positions=None, q=None,
@@ -274,34 +277,37 @@ def paged_rotary_store(k, v, k_pages, v_pages, block_table, q_starts, kv_lens, t
     Replaces the cache write of wan_5b/modules/action_model.py:265-292."""
     pg = _cache(k_pages, v_pages, block_table, kv_lens, q_starts)
     dev, dt = k_pages.device, k_pages.dtype
-    k, v = _in(k, "k", dt, dev), _in(v, "v", dt, dev)
+    k, ks, kp = _in(k, "k", dt, dev)
+    v, vs, vp = _in(v, "v", dt, dev)
     T = k.shape[0]
     if k.shape != (T, pg.Hkv, pg.D) or v.shape != k.shape:
         raise ValueError(f"k and v must be [T, {pg.Hkv}, {pg.D}], as the pools")
-    Hq, qa = 0, (0, 0, 0, 0)
+    Hq, qs, qp, os, op = 0, (0, 0), None, (0, 0), None
     if q is not None:
         given = q
-        q = _in(q, "q", dt, dev)
+        q, qs, qp = _in(q, "q", dt, dev)
         Hq = q.shape[1]
         if q.shape != (T, Hq, pg.D):
             raise ValueError(f"q must be [{T}, heads, {pg.D}]")
         if q_out is None:
             q_out = torch.empty((T, Hq, pg.D), dtype=dt, device=dev)
+            os, op = _heads(q_out, "q_out", dt, dev)
         else:
-            _check_out(q_out, "q_out", q, (T, Hq, pg.D), given)
-        qa = (*_sl_sh(q), *_sl_sh(q_out))
+            os, op = _out(q_out, "q_out", given, (T, Hq, pg.D), dt, dev)
+            if q_out.numel() and (_meet(q_out, k) or _meet(q_out, v)):
+                raise ValueError("q_out overlaps k or v")
+        if Hq == 0:
+            qp = op = None
     elif q_out is not None:
         raise ValueError("q_out needs q")
     tab = _table_args(table, pg.D, dev) if table is not None else (None, 0, 0)
-    if positions is not None:
-        _ints(positions, "positions", (T,), dev)
+    pp = _ints(positions, "positions", T, dev) if positions is not None else None
     if T == 0 or pg.B == 0:
         return q_out
     with _on(dev):
         code = _native.lib().rw_paged_rotary_store(
-            pg, k.data_ptr(), v.data_ptr(), q.data_ptr() if Hq else None, q_out.data_ptr() if Hq else None, T, Hq,
-            *_sl_sh(k), *_sl_sh(v), *qa, *tab, int(interleaved), positions.data_ptr() if positions is not None else None,
-            _native.status_tensor(dev).data_ptr(), _native.stream_ptr(dev))
+            pg, kp, vp, qp, op, T, Hq, ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], os[0], os[1], *tab, int(interleaved),
+            pp, _native.status_tensor(dev).data_ptr(), _stream(dev.index))
     _native.check(code, "rw_paged_rotary_store")
     return q_out
 
@@ -323,54 +329,62 @@ def paged_attention(q, k_pages, v_pages, block_table, q_starts, kv_lens, max_q_l
     The paged form of wan_5b/modules/attention.py:133-179."""
     pg = _cache(k_pages, v_pages, block_table, kv_lens, q_starts)
     dev, dt = k_pages.device, k_pages.dtype
-    q = _in(q, "q", dt, dev)
+    q, qs, qp = _in(q, "q", dt, dev)
     T, Hq, D = q.shape
-    if D != pg.D or Hq < 1 or Hq % pg.Hkv:
-        raise ValueError(f"q must be [T, heads, {pg.D}] with a multiple of {pg.Hkv} heads")
-    if Hq // pg.Hkv > 128:
+    hkv, B, rows = pg.Hkv, pg.B, pg.table_width * pg.page_size
+    if D != pg.D or Hq < 1 or Hq % hkv:
+        raise ValueError(f"q must be [T, heads, {pg.D}] with a multiple of {hkv} heads")
+    if Hq // hkv > 128:
         raise NotImplementedError("more than 128 query heads share a key head")
     if out is None:
         out = torch.empty((T, Hq, D), dtype=dt, device=dev)
+        os, op = (Hq * D, D), out.data_ptr()
     else:
         if tuple(out.shape) != (T, Hq, D):
             raise ValueError(f"out must be [{T}, {Hq}, {D}]")
-        _check_heads(out, "out", dt, dev)
-        if out.numel() and out.untyped_storage().data_ptr() == q.untyped_storage().data_ptr():
-            a, b = _span(out), _span(q)
-            if a[0] < b[1] and b[0] < a[1]:
-                raise ValueError("out overlaps q")
+        os, op = _heads(out, "out", dt, dev)
+        if out.numel() and _meet(out, q):
+            raise ValueError("out overlaps q")
     scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
     if not 0.0 < scale < 1e30:
         raise ValueError("softmax_scale must be positive and finite")
-    longest = T if max_q_len is None else int(max_q_len)
+    longest = T if max_q_len is None else min(int(max_q_len), T)
     if longest < 0:
         raise ValueError("max_q_len must not be negative")
-    rows = pg.table_width * pg.page_size
-    sums = (None, 0, 0)
-    if weight_sums is not None:
-        w = weight_sums
-        if w.dtype != torch.float32 or w.device != dev or w.dim() != 3 or w.shape[0] != pg.B or \
-                w.shape[1] != pg.Hkv or w.shape[2] < rows or (w.shape[2] > 1 and w.stride(2) != 1):
-            raise ValueError(f"weight_sums must be fp32 [{pg.B}, {pg.Hkv}, >= {rows}] on {dev}")
-        if (pg.Hkv > 1 and w.stride(1) < rows) or (pg.B > 1 and w.stride(0) < rows):
-            raise ValueError("weight_sums: rows overlap")
-        sums = (w.data_ptr() or None, w.stride(0), w.stride(1))
+    wp, w0, w1 = _sums_args(weight_sums, B, hkv, rows, dev) if weight_sums is not None else (None, 0, 0)
     lse = torch.empty((T, Hq), dtype=torch.float32, device=dev) if return_lse else None
-    if T > 0 and pg.B > 0 and longest > 0:
+    if T > 0 and B > 0 and longest > 0:
         with _on(dev):
-            lib = _native.lib()
-            n = ctypes.c_longlong()
-            need = lib.rw_paged_attn_workspace_bytes(T, Hq, pg.Hkv, D, pg.B, longest, rows, int(sums[0] is not None),
-                                                     n)
-            stream = torch.cuda.current_stream(dev).cuda_stream
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
-            counters = _zeroed(dev, n.value, stream) if n.value else None
-            code = lib.rw_paged_attn(
-                pg, q.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else None, T, Hq, longest,
-                *_sl_sh(q), *_sl_sh(out), int(bool(causal)), scale, *sums, counters.data_ptr() if n.value else None,
-                n.value, ws.data_ptr(), need, _native.status_tensor(dev).data_ptr(), stream)
+            need, counters = _attn_needs(dev.index, T, Hq, hkv, D, B, longest, rows, wp is not None)
+            stream = _stream(dev.index)
+            ws, cn = _workspace(dev, stream, need, counters)
+            code = _native.lib().rw_paged_attn(
+                pg, qp, op, lse.data_ptr() if return_lse else None, T, Hq, longest, qs[0], qs[1], os[0], os[1],
+                int(bool(causal)), scale, wp, w0, w1, cn.data_ptr(), counters, ws.data_ptr(), need,
+                _native.status_tensor(dev).data_ptr(), stream)
         _native.check(code, "rw_paged_attn")
     return (out, lse) if return_lse else out
+
+
+def _sums_args(w, B, hkv, rows, dev):
+    """(data pointer, strides of sequence and head) of an accumulator of weights."""
+    if w.dtype != torch.float32 or w.device != dev or w.dim() != 3:
+        raise ValueError(f"weight_sums must be fp32 [{B}, {hkv}, >= {rows}] on {dev}")
+    n, h, cap = w.shape
+    s0, s1, s2 = w.stride()
+    if n != B or h != hkv or cap < rows or (cap > 1 and s2 != 1):
+        raise ValueError(f"weight_sums must be fp32 [{B}, {hkv}, >= {rows}] on {dev}")
+    if (h > 1 and s1 < cap) or (n > 1 and s0 < cap) or (n > 1 and h > 1 and s0 < (h - 1) * s1 + cap and
+                                                      s1 < (n - 1) * s0 + cap):
+        raise ValueError("weight_sums: rows overlap")
+    return w.data_ptr() or None, s0, s1
+
+
+@functools.lru_cache(maxsize=4096)
+def _attn_needs(device, T, Hq, Hkv, D, B, longest, rows, sums):
+    """Workspace bytes and counters of a call of these sizes on the current device."""
+    n = ctypes.c_longlong()
+    return _native.lib().rw_paged_attn_workspace_bytes(T, Hq, Hkv, D, B, longest, rows, int(sums), n), n.value
 
 
 # ------------------------------------------------------------------ eviction
@@ -391,24 +405,21 @@ def paged_evict(k_pages, v_pages, block_table, kv_lens, weight_sums, keep, dst_t
     keep, n_sink, n_recent = int(keep), int(n_sink), int(n_recent)
     if keep < 1 or n_sink < 0 or n_recent < 0 or n_sink + n_recent > keep:
         raise ValueError("keep must be positive and hold n_sink + n_recent rows")
-    w, rows = weight_sums, pg.table_width * pg.page_size
-    if w.dtype != torch.float32 or w.device != dev or w.dim() != 3 or w.shape[0] != pg.B or w.shape[1] != pg.Hkv or \
-            w.shape[2] < max(rows, keep) or (w.shape[2] > 1 and w.stride(2) != 1):
-        raise ValueError(f"weight_sums must be fp32 [{pg.B}, {pg.Hkv}, >= {max(rows, keep)}] on {dev}")
-    if dst_table.dim() != 2 or dst_table.dtype != torch.int32 or dst_table.device != dev or \
-            dst_table.shape[0] != pg.B:
+    rows = max(pg.table_width * pg.page_size, keep)
+    wp, w0, w1 = _sums_args(weight_sums, pg.B, pg.Hkv, rows, dev)
+    cap = weight_sums.shape[2]
+    B, width, ds, dp = _table(dst_table, "dst_table", dev)
+    if B != pg.B:
         raise ValueError(f"dst_table must be an int32 [{pg.B}, pages] tensor on {dev}")
-    if dst_table.shape[1] * pg.page_size < keep:
-        raise ValueError(f"dst_table holds {dst_table.shape[1] * pg.page_size} rows, {keep} are kept")
-    ds = _table_stride(dst_table, "dst_table")
-    kept = torch.empty((pg.B, pg.Hkv, keep), dtype=torch.int32, device=dev)
-    lens = torch.empty((pg.B,), dtype=torch.int32, device=dev)
-    new = torch.empty((pg.B, pg.Hkv, w.shape[2]), dtype=torch.float32, device=dev)
-    if pg.B > 0:
+    if width * pg.page_size < keep:
+        raise ValueError(f"dst_table holds {width * pg.page_size} rows, {keep} are kept")
+    kept = torch.empty((B, pg.Hkv, keep), dtype=torch.int32, device=dev)
+    lens = torch.empty((B,), dtype=torch.int32, device=dev)
+    new = torch.empty((B, pg.Hkv, cap), dtype=torch.float32, device=dev)
+    if B > 0:
         with _on(dev):
             code = _native.lib().rw_paged_evict(
-                pg, w.data_ptr(), w.stride(0), w.stride(1), new.data_ptr(), w.shape[2], kept.data_ptr(),
-                lens.data_ptr(), keep, n_sink, n_recent, dst_table.data_ptr(), ds, dst_table.shape[1],
-                _native.status_tensor(dev).data_ptr(), _native.stream_ptr(dev))
+                pg, wp, w0, w1, new.data_ptr(), cap, kept.data_ptr(), lens.data_ptr(), keep, n_sink, n_recent, dp, ds,
+                width, _native.status_tensor(dev).data_ptr(), _stream(dev.index))
         _native.check(code, "rw_paged_evict")
     return kept, lens, new
