@@ -25,4 +25,12 @@ long long workspace_bytes(int D);
 bool supported(const rw_paged_t* cache);
 
 }  // namespace chunk
+
+namespace weigh {
+
+// Adds the weights of a chunk::launch that filled c.row_ml.
+int launch(const rw_paged_t* cache, const paged::Pool& pool, const chunk::Call& c, float* sums, long long sums_sb,
+           long long sums_sh, cudaStream_t st);
+
+}  // namespace weigh
 }  // namespace rw

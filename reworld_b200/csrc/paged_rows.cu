@@ -669,12 +669,18 @@ extern "C" int rw_paged_attn(const rw_paged_t* cache, const void* q, void* out, 
   const long long cap = (long long)cache->table_width * cache->page_size;
   const float scale_log2 = softmax_scale * 1.4426950408889634f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (rows::on_tensor_tiles(cache->B, nrt) && !sums && chunk::supported(cache)) {
-    if (!workspace || !aligned16(workspace) || workspace_bytes < chunk::workspace_bytes(cache->D))
+  if (rows::on_tensor_tiles(cache->B, nrt) && chunk::supported(cache)) {
+    const long long parts = chunk::workspace_bytes(cache->D);
+    if (!workspace || !aligned16(workspace) || workspace_bytes < parts + (sums ? 8LL * T * Hq : 0))
       return RW_ERR_INVALID_ARG;
-    const chunk::Call c{q, out, lse, nullptr, T, Hq, causal != 0, q_sl, q_sh, o_sl, o_sh, scale_log2, status};
-    return chunk::launch(cache, p.pool, c, workspace, st);
+    float2* ml = sums ? reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + parts) : nullptr;
+    const chunk::Call c{q, out, lse, ml, T, Hq, causal != 0, q_sl, q_sh, o_sl, o_sh, scale_log2, status};
+    const int rc = chunk::launch(cache, p.pool, c, workspace, st);
+    return rc != RW_OK || !sums ? rc : weigh::launch(cache, p.pool, c, sums, sums_sb, sums_sh, st);
   }
+  // (a pool of over 2^31 lines of its strides' common divisor takes no tensor map; the rows kernel reads it, but
+  // would need a workspace for a chunk's scores)
+  if (rows::on_tensor_tiles(cache->B, nrt) && sums) return RW_ERR_UNSUPPORTED;
   const int C = rows::grid_size(cache->D);
   if (C == 0 || 2 * C > rows::MAX_PARTS) return RW_ERR_CUDA;
   const rows::Layout lay = rows::layout(cache->D, C, cache->B, p.pool.Hkv, (int)nrt, cap, sums != nullptr);
@@ -726,6 +732,10 @@ extern "C" long long rw_paged_attn_workspace_bytes(int T, int Hq, int Hkv, int D
   const long long nrt = ((long long)(max_q_len < T ? max_q_len : T) * (Hq / Hkv) + rows::RT - 1) / rows::RT;
   if (nrt * B * Hkv > (1ll << 30)) return 0;
   if (n_counters) *n_counters = rows::counters_needed(B, Hkv, (int)nrt);
-  const long long own = rows::layout(D, rows::grid_size(D), B, Hkv, (int)nrt, cache_rows, with_sums != 0).total;
-  return rows::on_tensor_tiles(B, nrt) && !with_sums ? std::max(own, chunk::workspace_bytes(D)) : own;
+  if (rows::on_tensor_tiles(B, nrt)) {
+    const long long tiles = chunk::workspace_bytes(D) + (with_sums ? 8LL * T * Hq : 0);
+    // (a pool whose strides no tensor map takes falls back to the rows kernel, which needs no more without sums)
+    return with_sums ? tiles : std::max(tiles, rows::layout(D, rows::grid_size(D), B, Hkv, (int)nrt, 0, false).total);
+  }
+  return rows::layout(D, rows::grid_size(D), B, Hkv, (int)nrt, cache_rows, with_sums != 0).total;
 }

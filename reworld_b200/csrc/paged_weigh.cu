@@ -1,0 +1,357 @@
+// What weight every cached row received from a chunk of new tokens: sums[b, g, j] += sum
+// over the rows of key head g's group of exp(s - m) / l, with the scores s computed again
+// and (m, 1 / l) of every row from the attention (paged_chunk.cu).
+//
+// Why again: a weight is known only when its row's total is, which is after the last key,
+// and a chunk's scores are too many to keep (rows x keys x 4 bytes; the rows of a single
+// token are few, and paged_rows.cu keeps theirs).  The second product is half of the
+// attention's operations and needs no values.
+//
+// Transposed tiles: S^T[128 keys][128 rows] = K Q^T, so that a thread owns one key, adds
+// up its columns in registers, and no reduction across threads, no atomics and no order
+// that could change are needed; a unit (128 keys of a sequence and key head) stays in
+// shared memory while the rows' tiles pass by.  Rows are packed as in paged_chunk.cu
+// (token * G + head).  Two warpgroups take 64 columns each.  Bound by the exponentials
+// (128 x 128 of them against 128 x 128 x D products): the S buffers, four, keep the
+// tensor pipe ahead.
+#include "paged_chunk.h"
+#include "paged_tiles.cuh"
+
+namespace rw {
+namespace weigh {
+
+using paged::Pool;
+using paged::Seq;
+using namespace tiles;
+
+constexpr int NS = 4;                        // S buffers (and row parameters)
+constexpr int NQ = 4;                        // row tiles in shared memory
+constexpr int NK = 2;                        // key tiles
+constexpr int NUM_THREADS = 384;
+constexpr int WARP_LOAD = 8, WARP_MMA = 9, WARP_ROWS = 10;
+
+struct Params {
+  Pool pool;
+  int T, Hq, G, causal, tpc;
+  int kbox, k_head, k_page;
+  float scale_log2;
+  const float2* row_ml;                      // [T, Hq]
+  float* sums;
+  long long sums_sb, sums_sh;
+  int* status;
+};
+
+struct __align__(8) Barriers {
+  uint64_t k_full[NK], k_free[NK], q_full[NQ], q_free[NQ], s_full[NS], s_free[NS], r_full[NS];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+struct Unit {
+  int b, hk, key0, first, n;                 // row tiles [first, first + n) see any of the keys
+  Seq s;
+};
+
+template <bool HALF, int D>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+    weigh_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                 const __grid_constant__ Params p) {
+  constexpr int TILE_BYTES = BM * D * 2;
+  constexpr int Q_BOX = BM * 128;
+  constexpr int K_GROUP = 1024 * (D / 64);
+  extern __shared__ uint8_t dsmem_raw[];
+  __shared__ Barriers sb;
+  __shared__ int before[chunk::MAX_BATCH + 1];   // units before each sequence
+  __shared__ int3 seq[chunk::MAX_BATCH];         // s0, lq, kv
+  __shared__ float4 par[NS][BM / 2];             // (-m, -m', 1 / l, 1 / l') of column pairs
+  __shared__ float half_sum[2][BM];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dsmem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ks = smem;
+  uint8_t* qs = smem + NK * TILE_BYTES;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);
+  const int lane = threadIdx.x & 31;
+  const int used = p.tpc * p.G;
+
+  if (threadIdx.x == WARP_LOAD * 32) {
+    for (int i = 0; i < NK; ++i) { mbar_init(&sb.k_full[i], 1); mbar_init(&sb.k_free[i], 1); }
+    for (int i = 0; i < NQ; ++i) { mbar_init(&sb.q_full[i], 1); mbar_init(&sb.q_free[i], 1); }
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&sb.s_full[i], 1);
+      mbar_init(&sb.s_free[i], 256);
+      mbar_init(&sb.r_full[i], 32);
+    }
+    sb.abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+  }
+  if (warp == WARP_MMA) {
+    tmem_alloc(&sb.tmem_base, 512);
+    tmem_relinquish();
+  }
+  // rows of the row tiles that hold no token stay zero: no load reaches them
+  for (int i = threadIdx.x; i < NQ * (BM - used) * (D / 8); i += NUM_THREADS) {
+    const int c = i % (D / 8), r = used + (i / (D / 8)) % (BM - used), st = i / (D / 8) / (BM - used);
+    *reinterpret_cast<uint4*>(qs + st * TILE_BYTES + (c >> 3) * Q_BOX + r * 128 + ((c & 7) << 4)) =
+        make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async_smem();
+  griddep_wait();
+  for (int b = threadIdx.x; b < p.pool.B; b += NUM_THREADS) {
+    const Seq s = paged::load_seq(p.pool, b, p.T, nullptr);
+    seq[b] = make_int3(s.s0, s.lq, s.kv);
+    before[b + 1] = s.lq > 0 ? (s.kv + BM - 1) / BM * p.pool.Hkv : 0;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) {
+    int c = 0;
+    for (int b0 = 0; b0 < p.pool.B; b0 += 32) {
+      int u = b0 + lane < p.pool.B ? before[b0 + lane + 1] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int z = __shfl_up_sync(0xffffffffu, u, o);
+        if (lane >= o) u += z;
+      }
+      if (b0 + lane < p.pool.B) before[b0 + lane + 1] = c + u;
+      c += __shfl_sync(0xffffffffu, u, 31);
+    }
+    if (lane == 0) before[0] = 0;
+  }
+  __syncthreads();
+  const uint32_t tmem = sb.tmem_base;
+  const int U = before[p.pool.B];
+  volatile int* abort_flag = &sb.abort_flag;
+  auto wait = [&](uint64_t* bar, uint32_t parity, int err) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status, err));
+  };
+  // neighbouring units cost about the same, and CTAs at work at the same time share a head's rows
+  auto unit = [&](int u) {
+    Unit x;
+    int lo = 0, hi = p.pool.B - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (before[mid] <= u) lo = mid; else hi = mid - 1;
+    }
+    x.b = lo;
+    const int3 s = seq[lo];
+    x.s = Seq{s.x, s.y, s.z};
+    const int nk = (x.s.kv + BM - 1) / BM, r = u - before[lo];
+    x.hk = r / nk;
+    x.key0 = (r - x.hk * nk) * BM;
+    // the first token that sees key0
+    const int tok = p.causal ? max(0, x.key0 - (x.s.kv - x.s.lq)) : 0;
+    x.first = tok / p.tpc;
+    x.n = (x.s.lq + p.tpc - 1) / p.tpc - x.first;
+    return x;
+  };
+
+  if (warp == WARP_LOAD) {
+    int i = 0, k = 0;                          // row tiles and units so far
+    bool ok = true;
+    const int nkp = BM / p.kbox, mask = (1 << p.pool.page_shift) - 1;
+    for (int u = blockIdx.x; u < U && ok; u += gridDim.x, ++k) {
+      const Unit x = unit(u);
+      const int row = x.key0 + lane * p.kbox;
+      int pg = lane < nkp && row < x.s.kv ? paged::raw_page_of(p.pool, x.b, row) : 0;
+      const int sk = k % NK;
+      if (k >= NK && !(ok = wait(&sb.k_free[sk], (uint32_t)(k / NK - 1) & 1u, RW_STATUS_TIMEOUT_LOAD))) break;
+      if (lane == 0) mbar_expect_tx(&sb.k_full[sk], TILE_BYTES);
+      pg = paged::checked_page(p.pool, pg, p.status);
+      __syncwarp();
+      const int row0 = nkp == 1 ? x.key0 & mask : 0;
+      for_pages(x.hk * p.k_head + pg * p.k_page, nkp, [&](int j, int line) {
+        load_5d<1>(smem_u32(ks) + sk * TILE_BYTES + j * p.kbox * 2 * D, &tm_k, smem_u32(&sb.k_full[sk]), 0, 0, 0,
+                   row0 >> 3, line);
+      });
+      for (int j = 0; j < x.n; ++j, ++i) {
+        const int sq = i % NQ;
+        if (i >= NQ && !(ok = wait(&sb.q_free[sq], (uint32_t)(i / NQ - 1) & 1u, RW_STATUS_TIMEOUT_LOAD))) break;
+        if (elect_one()) {
+          mbar_expect_tx(&sb.q_full[sq], (D / 64) * used * 128);
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c)
+            load_3d<1>(smem_u32(qs) + sq * TILE_BYTES + c * Q_BOX, &tm_q, smem_u32(&sb.q_full[sq]), 64 * c, x.hk * p.G,
+                       x.s.s0 + (x.first + j) * p.tpc);
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp == WARP_MMA) {
+    constexpr uint32_t ID = idesc<HALF>(BM, BM, 0);
+    const uint64_t dk = umma_desc(smem_u32(ks), 16, K_GROUP), dq = umma_desc(smem_u32(qs), 16, 1024);
+    int i = 0, k = 0;
+    bool ok = true;
+    for (int u = blockIdx.x; u < U && ok; u += gridDim.x, ++k) {
+      const int n = unit(u).n, sk = k % NK;
+      if (!(ok = wait(&sb.k_full[sk], (uint32_t)(k / NK) & 1u, RW_STATUS_TIMEOUT_MMA))) break;
+      for (int j = 0; j < n; ++j, ++i) {
+        const int sq = i % NQ, s = i % NS;
+        if (!(ok = wait(&sb.q_full[sq], (uint32_t)(i / NQ) & 1u, RW_STATUS_TIMEOUT_MMA))) break;
+        if (i >= NS && !(ok = wait(&sb.s_free[s], (uint32_t)(i / NS - 1) & 1u, RW_STATUS_TIMEOUT_MMA))) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t a = dk + (uint64_t)((sk * TILE_BYTES) >> 4), b = dq + (uint64_t)((sq * TILE_BYTES) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            mma_ss(tmem + 128u * s, a + (uint64_t)(((kk >> 2) * 1024 + (kk & 3) * 32) >> 4),
+                   b + (uint64_t)(((kk >> 2) * Q_BOX + (kk & 3) * 32) >> 4), ID, kk > 0 ? 1u : 0u);
+          tc_commit(&sb.s_full[s]);
+          tc_commit(&sb.q_free[sq]);
+          if (j == n - 1) tc_commit(&sb.k_free[sk]);
+        }
+        __syncwarp();
+      }
+    }
+    // the last row tiles' MMAs are seen to end by the warpgroups; their releases land before the CTA leaves
+    if (ok)
+      for (int t = max(0, i - NQ); t < i; ++t) mbar_wait_drain(&sb.q_free[t % NQ], (uint32_t)(t / NQ) & 1u);
+    if (ok)
+      for (int t = max(0, k - NK); t < k; ++t) mbar_wait_drain(&sb.k_free[t % NK], (uint32_t)(t / NK) & 1u);
+  } else if (warp == WARP_ROWS) {
+    // (-m, 1 / l) of a row tile's rows, in column pairs; fetched one tile ahead
+    int i = 0;
+    bool ok = true;
+    float2 next[4];
+    for (int u = blockIdx.x; u < U && ok; u += gridDim.x) {
+      const Unit x = unit(u);
+      auto fetch = [&](int j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * lane + e, t = r / p.G, tok = (x.first + j) * p.tpc + t;
+          // a row that is none: no weight
+          next[e] = r < used && tok < x.s.lq && j < x.n
+                        ? __ldg(p.row_ml + (long long)(x.s.s0 + tok) * p.Hq + x.hk * p.G + (r - t * p.G))
+                        : make_float2(INFINITY, 0.f);
+        }
+      };
+      fetch(0);
+      for (int j = 0; j < x.n; ++j, ++i) {
+        const int s = i % NS;
+        float2 now[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) now[e] = next[e];
+        fetch(j + 1);
+        if (i >= NS && !(ok = wait(&sb.s_free[s], (uint32_t)(i / NS - 1) & 1u, RW_STATUS_TIMEOUT_LOAD))) break;
+        par[s][2 * lane] = make_float4(-now[0].x, -now[1].x, now[0].y, now[1].y);
+        par[s][2 * lane + 1] = make_float4(-now[2].x, -now[3].x, now[2].y, now[3].y);
+        mbar_arrive(&sb.r_full[s]);
+      }
+    }
+  } else if (warp < 8) {
+    const int w = warp >> 2;                   // columns [64 w, 64 w + 64)
+    const int r = threadIdx.x & 127;           // the thread's key
+    const uint32_t t0 = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 64u * w;
+    const uint64_t s2 = f2_pack(p.scale_log2, p.scale_log2);
+    int i = 0, k = 0;
+    bool ok = true;
+    for (int u = blockIdx.x; u < U; u += gridDim.x, ++k) {
+      const Unit x = unit(u);
+      uint64_t acc[2] = {0ull, 0ull};
+      // rows (token * G + head) of the sequence that see the thread's key begin here
+      const long long from = p.causal ? (long long)max(0, x.key0 + r - (x.s.kv - x.s.lq)) * p.G : 0;
+      const int all = p.causal ? max(0, x.key0 + BM - 1 - (x.s.kv - x.s.lq)) : 0;  // first token that sees all keys
+      for (int j = 0; j < x.n; ++j, ++i) {
+        const int s = i % NS;
+        ok = ok && wait(&sb.s_full[s], (uint32_t)(i / NS) & 1u, RW_STATUS_TIMEOUT_SOFTMAX) &&
+             wait(&sb.r_full[s], (uint32_t)(i / NS) & 1u, RW_STATUS_TIMEOUT_SOFTMAX);
+        if (!ok) continue;
+        tc_fence_after();
+        uint32_t v[2][32];
+        tmem_ld32(t0 + 128u * s, v[0]);
+        tmem_ld32(t0 + 128u * s + 32, v[1]);
+        tmem_wait_ld();
+        reg_fence32(v[0]);
+        reg_fence32(v[1]);
+        const int tok0 = (x.first + j) * p.tpc;
+        const bool masked = tok0 < all || tok0 + p.tpc > x.s.lq || used < BM;
+        if (masked) {
+          // columns [lo, hi) count; the scores of the others are whatever lies there
+          const int lo = (int)max(0ll, min((long long)BM, from - (long long)tok0 * p.G)) - 64 * w;
+          const int hi = min(used, (x.s.lq - tok0) * p.G) - 64 * w;
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (32 * c + e < lo || 32 * c + e >= hi) v[c][e] = __float_as_uint(-INFINITY);
+        }
+        const float4* pr = par[s] + 32 * w;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float4 q = pr[16 * c + e];
+            const uint64_t xv = ffma2(f2_pack(__uint_as_float(v[c][2 * e]), __uint_as_float(v[c][2 * e + 1])), s2,
+                                      f2_pack(q.x, q.y));
+            float a, b;
+            f2_unpack(xv, a, b);
+            acc[e & 1] = ffma2(f2_pack(fast_exp2(a), fast_exp2(b)), f2_pack(q.z, q.w), acc[e & 1]);
+          }
+        tc_fence_before();
+        mbar_arrive(&sb.s_free[s]);
+      }
+      float a, b;
+      f2_unpack(fadd2(acc[0], acc[1]), a, b);
+      if (w == 1) half_sum[k & 1][r] = a + b;
+      named_bar_sync(1, 256);
+      if (w == 0 && ok && x.key0 + r < x.s.kv) {
+        float* dst = p.sums + x.b * p.sums_sb + x.hk * p.sums_sh + x.key0 + r;
+        *dst += (a + b) + half_sum[k & 1][r];
+      }
+    }
+  }
+
+  if (warp == WARP_LOAD && lane == 0 && *abort_flag) {
+    const uint64_t t0 = globaltimer_ns();      // after a timeout: copies in flight get time to land
+    while (globaltimer_ns() - t0 < 200000ull) {
+    }
+  }
+  if (threadIdx.x == 0) griddep_launch_dependents();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == WARP_MMA) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <bool HALF, int D>
+int launch_one(const CUtensorMap& mq, const CUtensorMap& mk, const Params& p, int sms, cudaStream_t st) {
+  static std::atomic<unsigned long long> done{0};
+  constexpr int SMEM = (NK + NQ) * BM * D * 2 + 1024;
+  if (!ensure_smem_attr(reinterpret_cast<const void*>(weigh_kernel<HALF, D>), SMEM, &done)) return RW_ERR_CUDA;
+  return launch_dependent(weigh_kernel<HALF, D>, dim3(sms), dim3(NUM_THREADS), SMEM, st, mq, mk, p) == cudaSuccess
+             ? RW_OK : RW_ERR_CUDA;
+}
+
+int launch(const rw_paged_t* cache, const Pool& pool, const chunk::Call& c, float* sums, long long sums_sb,
+           long long sums_sh, cudaStream_t st) {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return RW_ERR_CUDA;
+  Params p{};
+  p.pool = pool;
+  p.T = c.T; p.Hq = c.Hq; p.G = c.Hq / pool.Hkv; p.causal = c.causal;
+  p.tpc = BM / p.G;
+  p.kbox = cache->page_size < BM ? cache->page_size : BM;
+  const KeyLines kl = key_lines(cache);
+  p.k_head = cache->Hkv == 1 ? 0 : (int)(cache->k_sh / kl.step);
+  p.k_page = cache->num_pages == 1 ? 0 : (int)(cache->k_sp / kl.step);
+  p.scale_log2 = c.scale_log2;
+  p.row_ml = c.row_ml;
+  p.sums = sums;
+  p.sums_sb = sums_sb;
+  p.sums_sh = sums_sh;
+  p.status = c.status;
+  CUtensorMap mq, mk;
+  if (q_map(&mq, c.q, cache->dtype, c.T, c.Hq, cache->D, c.q_sl, c.q_sh, p.G, p.tpc) || key_map(&mk, cache, p.kbox))
+    return RW_ERR_DRIVER;
+  if (cache->dtype == RW_DTYPE_FP16)
+    return cache->D == 128 ? launch_one<true, 128>(mq, mk, p, sms, st) : launch_one<true, 64>(mq, mk, p, sms, st);
+  return cache->D == 128 ? launch_one<false, 128>(mq, mk, p, sms, st) : launch_one<false, 64>(mq, mk, p, sms, st);
+}
+
+}  // namespace weigh
+}  // namespace rw
