@@ -87,7 +87,7 @@ struct Params {
   uint8_t* out;
   long long o_sl, o_sh;  // byte strides
   float* lse;            // [T, Hq] or null
-  float2* row_ml;        // [T, Hq] (m, 1 / l) for the weight sums, or null
+  float* row_b;          // [T, Hq]: -(m + log2 l) for the weight sums, or null
   float* scratch;        // [2 C] slots
   int4* header;          // [2 C]: (b + 1 or 0, hk, tok0, unused)
   int kbox, vbox;        // rows of a TMA box: min(page, keys of a CTA), min(page, 128)
@@ -936,7 +936,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         if (ok && w == 0 && there) {
           const long long at = (long long)(sg.s0 + tok) * p.Hq + sg.hk * p.G + rg;
           if (p.lse) p.lse[at] = l_row != 0.f ? (m_fin * sl2 + log2f(l_row)) * 0.6931471805599453f : -INFINITY;
-          if (p.row_ml) p.row_ml[at] = make_float2(l_row != 0.f ? m_fin * sl2 : 0.f, inv);
+          if (p.row_b) p.row_b[at] = l_row != 0.f ? -(m_fin * sl2 + log2f(l_row)) : -INFINITY;
         }
         named_bar_sync(1, SOFTMAX_THREADS);
         constexpr int CH = D / 8;
@@ -1041,7 +1041,7 @@ __global__ void __launch_bounds__(BM) join_kernel(const __grid_constant__ Params
   if (c0 == 0) {
     const long long at = (long long)(sq.s0 + tok) * p.Hq + head;
     if (p.lse) p.lse[at] = l != 0.f ? (m * p.scale_log2 + log2f(l)) * 0.6931471805599453f : -INFINITY;
-    if (p.row_ml) p.row_ml[at] = make_float2(l != 0.f ? m * p.scale_log2 : 0.f, inv);
+    if (p.row_b) p.row_b[at] = l != 0.f ? -(m * p.scale_log2 + log2f(l)) : -INFINITY;
   }
 }
 
@@ -1115,7 +1115,7 @@ int launch(const rw_paged_t* cache, const Pool& pool, const Call& c, void* works
   p.out = static_cast<uint8_t*>(c.out);
   p.o_sl = 2 * c.o_sl; p.o_sh = 2 * c.o_sh;
   p.lse = c.lse;
-  p.row_ml = c.row_ml;
+  p.row_b = c.row_b;
   p.header = static_cast<int4*>(workspace);
   p.scratch = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 2LL * p.C * 16);
   const int krows = cache->D == 128 ? Shape<128>::KROWS : Shape<64>::KROWS;

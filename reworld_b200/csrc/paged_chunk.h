@@ -13,7 +13,7 @@ struct Call {
   const void* q;
   void* out;
   float* lse;
-  float2* row_ml;
+  float* row_b;
   int T, Hq, causal;
   long long q_sl, q_sh, o_sl, o_sh;  // element strides
   float scale_log2;
@@ -28,7 +28,7 @@ bool supported(const rw_paged_t* cache);
 
 namespace weigh {
 
-// Adds the weights of a chunk::launch that filled c.row_ml.
+// Adds the weights of a chunk::launch that filled c.row_b.
 int launch(const rw_paged_t* cache, const paged::Pool& pool, const chunk::Call& c, float* sums, long long sums_sb,
            long long sums_sh, cudaStream_t st);
 

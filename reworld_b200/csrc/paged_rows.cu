@@ -671,10 +671,10 @@ extern "C" int rw_paged_attn(const rw_paged_t* cache, const void* q, void* out, 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (rows::on_tensor_tiles(cache->B, nrt) && chunk::supported(cache)) {
     const long long parts = chunk::workspace_bytes(cache->D);
-    if (!workspace || !aligned16(workspace) || workspace_bytes < parts + (sums ? 8LL * T * Hq : 0))
+    if (!workspace || !aligned16(workspace) || workspace_bytes < parts + (sums ? 4LL * T * Hq : 0))
       return RW_ERR_INVALID_ARG;
-    float2* ml = sums ? reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + parts) : nullptr;
-    const chunk::Call c{q, out, lse, ml, T, Hq, causal != 0, q_sl, q_sh, o_sl, o_sh, scale_log2, status};
+    float* rb = sums ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + parts) : nullptr;
+    const chunk::Call c{q, out, lse, rb, T, Hq, causal != 0, q_sl, q_sh, o_sl, o_sh, scale_log2, status};
     const int rc = chunk::launch(cache, p.pool, c, workspace, st);
     return rc != RW_OK || !sums ? rc : weigh::launch(cache, p.pool, c, sums, sums_sb, sums_sh, st);
   }
@@ -733,7 +733,7 @@ extern "C" long long rw_paged_attn_workspace_bytes(int T, int Hq, int Hkv, int D
   if (nrt * B * Hkv > (1ll << 30)) return 0;
   if (n_counters) *n_counters = rows::counters_needed(B, Hkv, (int)nrt);
   if (rows::on_tensor_tiles(B, nrt)) {
-    const long long tiles = chunk::workspace_bytes(D) + (with_sums ? 8LL * T * Hq : 0);
+    const long long tiles = chunk::workspace_bytes(D) + (with_sums ? 4LL * T * Hq : 0);
     // (a pool whose strides no tensor map takes falls back to the rows kernel, which needs no more without sums)
     return with_sums ? tiles : std::max(tiles, rows::layout(D, rows::grid_size(D), B, Hkv, (int)nrt, 0, false).total);
   }

@@ -1,6 +1,6 @@
 // What weight every cached row received from a chunk of new tokens: sums[b, g, j] += sum
-// over the rows of key head g's group of exp(s - m) / l, with the scores s computed again
-// and (m, 1 / l) of every row from the attention (paged_chunk.cu).
+// over the rows of key head g's group of exp(s - lse), with the scores s computed again and
+// the rows' lse from the attention (paged_chunk.cu).
 //
 // Why again: a weight is known only when its row's total is, which is after the last key,
 // and a chunk's scores are too many to keep (rows x keys x 4 bytes; the rows of a single
@@ -11,7 +11,7 @@
 // up its columns in registers, and no reduction across threads, no atomics and no order
 // that could change are needed; a unit (128 keys of a sequence and key head) stays in
 // shared memory while the rows' tiles pass by.  Rows are packed as in paged_chunk.cu
-// (token * G + head).  Two warpgroups take 64 columns each.  Bound by the exponentials
+// (token * G + head).  Four warpgroups take 32 columns each.  Bound by the exponentials
 // (128 x 128 of them against 128 x 128 x D products): the S buffers, four, keep the
 // tensor pipe ahead.
 #include "paged_chunk.h"
@@ -27,15 +27,18 @@ using namespace tiles;
 constexpr int NS = 4;                        // S buffers (and row parameters)
 constexpr int NQ = 4;                        // row tiles in shared memory
 constexpr int NK = 2;                        // key tiles
-constexpr int NUM_THREADS = 384;
-constexpr int WARP_LOAD = 8, WARP_MMA = 9, WARP_ROWS = 10;
+constexpr int NWG = 4;                       // warpgroups that take 128 / NWG columns each
+constexpr int CW = BM / NWG;
+constexpr int SUM_THREADS = 128 * NWG;
+constexpr int NUM_THREADS = SUM_THREADS + 128;
+constexpr int WARP_LOAD = 4 * NWG, WARP_MMA = WARP_LOAD + 1, WARP_ROWS = WARP_LOAD + 2;
 
 struct Params {
   Pool pool;
   int T, Hq, G, causal, tpc;
   int kbox, k_head, k_page;
   float scale_log2;
-  const float2* row_ml;                      // [T, Hq]
+  const float* row_b;                        // [T, Hq]: -(m + log2 l)
   float* sums;
   long long sums_sb, sums_sh;
   int* status;
@@ -43,6 +46,7 @@ struct Params {
 
 struct __align__(8) Barriers {
   uint64_t k_full[NK], k_free[NK], q_full[NQ], q_free[NQ], s_full[NS], s_free[NS], r_full[NS];
+  uint64_t part_full[2], part_free[2];
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -63,8 +67,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   __shared__ Barriers sb;
   __shared__ int before[chunk::MAX_BATCH + 1];   // units before each sequence
   __shared__ int3 seq[chunk::MAX_BATCH];         // s0, lq, kv
-  __shared__ float4 par[NS][BM / 2];             // (-m, -m', 1 / l, 1 / l') of column pairs
-  __shared__ float half_sum[2][BM];
+  __shared__ __align__(16) float par[NS][BM];    // -(m + log2 l) of the columns' rows
+  __shared__ float part_sum[2][NWG - 1][BM];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dsmem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ks = smem;
   uint8_t* qs = smem + NK * TILE_BYTES;
@@ -77,8 +81,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     for (int i = 0; i < NQ; ++i) { mbar_init(&sb.q_full[i], 1); mbar_init(&sb.q_free[i], 1); }
     for (int i = 0; i < NS; ++i) {
       mbar_init(&sb.s_full[i], 1);
-      mbar_init(&sb.s_free[i], 256);
+      mbar_init(&sb.s_free[i], SUM_THREADS);
       mbar_init(&sb.r_full[i], 32);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sb.part_full[i], SUM_THREADS - 128);
+      mbar_init(&sb.part_free[i], 128);
     }
     sb.abort_flag = 0;
     fence_mbar_init();
@@ -210,39 +218,35 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     if (ok)
       for (int t = max(0, k - NK); t < k; ++t) mbar_wait_drain(&sb.k_free[t % NK], (uint32_t)(t / NK) & 1u);
   } else if (warp == WARP_ROWS) {
-    // (-m, 1 / l) of a row tile's rows, in column pairs; fetched one tile ahead
+    // -(m + log2 l) of a row tile's rows, fetched one tile ahead; -inf (no weight) for a row that is none
     int i = 0;
     bool ok = true;
-    float2 next[4];
+    float next[4];
     for (int u = blockIdx.x; u < U && ok; u += gridDim.x) {
       const Unit x = unit(u);
       auto fetch = [&](int j) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = 4 * lane + e, t = r / p.G, tok = (x.first + j) * p.tpc + t;
-          // a row that is none: no weight
           next[e] = r < used && tok < x.s.lq && j < x.n
-                        ? __ldg(p.row_ml + (long long)(x.s.s0 + tok) * p.Hq + x.hk * p.G + (r - t * p.G))
-                        : make_float2(INFINITY, 0.f);
+                        ? __ldg(p.row_b + (long long)(x.s.s0 + tok) * p.Hq + x.hk * p.G + (r - t * p.G))
+                        : -INFINITY;
         }
       };
       fetch(0);
       for (int j = 0; j < x.n; ++j, ++i) {
         const int s = i % NS;
-        float2 now[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) now[e] = next[e];
+        const float4 now = make_float4(next[0], next[1], next[2], next[3]);
         fetch(j + 1);
         if (i >= NS && !(ok = wait(&sb.s_free[s], (uint32_t)(i / NS - 1) & 1u, RW_STATUS_TIMEOUT_LOAD))) break;
-        par[s][2 * lane] = make_float4(-now[0].x, -now[1].x, now[0].y, now[1].y);
-        par[s][2 * lane + 1] = make_float4(-now[2].x, -now[3].x, now[2].y, now[3].y);
+        *reinterpret_cast<float4*>(par[s] + 4 * lane) = now;
         mbar_arrive(&sb.r_full[s]);
       }
     }
-  } else if (warp < 8) {
-    const int w = warp >> 2;                   // columns [64 w, 64 w + 64)
+  } else if (warp < 4 * NWG) {
+    const int w = warp >> 2;                   // columns [CW w, CW w + CW)
     const int r = threadIdx.x & 127;           // the thread's key
-    const uint32_t t0 = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 64u * w;
+    const uint32_t t0 = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(CW * w);
     const uint64_t s2 = f2_pack(p.scale_log2, p.scale_log2);
     int i = 0, k = 0;
     bool ok = true;
@@ -256,48 +260,59 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         const int s = i % NS;
         ok = ok && wait(&sb.s_full[s], (uint32_t)(i / NS) & 1u, RW_STATUS_TIMEOUT_SOFTMAX) &&
              wait(&sb.r_full[s], (uint32_t)(i / NS) & 1u, RW_STATUS_TIMEOUT_SOFTMAX);
-        if (!ok) continue;
+        if (!ok) break;
         tc_fence_after();
-        uint32_t v[2][32];
-        tmem_ld32(t0 + 128u * s, v[0]);
-        tmem_ld32(t0 + 128u * s + 32, v[1]);
-        tmem_wait_ld();
-        reg_fence32(v[0]);
-        reg_fence32(v[1]);
         const int tok0 = (x.first + j) * p.tpc;
-        const bool masked = tok0 < all || tok0 + p.tpc > x.s.lq || used < BM;
-        if (masked) {
-          // columns [lo, hi) count; the scores of the others are whatever lies there
-          const int lo = (int)max(0ll, min((long long)BM, from - (long long)tok0 * p.G)) - 64 * w;
-          const int hi = min(used, (x.s.lq - tok0) * p.G) - 64 * w;
+        const bool masked = tok0 < all || tok0 + p.tpc > x.s.lq;  // (columns without a row hold 0 and have no weight)
+        // columns [lo, hi) count; the scores of the others are whatever lies there
+        const int lo = (int)max(0ll, min((long long)BM, from - (long long)tok0 * p.G)) - CW * w;
+        const int hi = min(used, (x.s.lq - tok0) * p.G) - CW * w;
+        const float4* pr = reinterpret_cast<const float4*>(par[s] + CW * w);
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < CW / 32; ++c) {
+          uint32_t v[32];
+          tmem_ld32(t0 + 128u * s + 32 * c, v);
+          tmem_wait_ld();
+          reg_fence32(v);
+          if (masked) {
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (32 * c + e < lo || 32 * c + e >= hi) v[c][e] = __float_as_uint(-INFINITY);
-        }
-        const float4* pr = par[s] + 32 * w;
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float4 q = pr[16 * c + e];
-            const uint64_t xv = ffma2(f2_pack(__uint_as_float(v[c][2 * e]), __uint_as_float(v[c][2 * e + 1])), s2,
-                                      f2_pack(q.x, q.y));
-            float a, b;
-            f2_unpack(xv, a, b);
-            acc[e & 1] = ffma2(f2_pack(fast_exp2(a), fast_exp2(b)), f2_pack(q.z, q.w), acc[e & 1]);
+              if (32 * c + e < lo || 32 * c + e >= hi) v[e] = __float_as_uint(-INFINITY);
           }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float4 q = pr[8 * c + e];
+            float a0, a1, a2, a3;
+            f2_unpack(ffma2(f2_pack(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1])), s2, f2_pack(q.x, q.y)),
+                      a0, a1);
+            f2_unpack(ffma2(f2_pack(__uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3])), s2,
+                            f2_pack(q.z, q.w)), a2, a3);
+            acc[0] = fadd2(acc[0], f2_pack(fast_exp2(a0), fast_exp2(a1)));
+            acc[1] = fadd2(acc[1], f2_pack(fast_exp2(a2), fast_exp2(a3)));
+          }
+        }
         tc_fence_before();
         mbar_arrive(&sb.s_free[s]);
       }
       float a, b;
       f2_unpack(fadd2(acc[0], acc[1]), a, b);
-      if (w == 1) half_sum[k & 1][r] = a + b;
-      named_bar_sync(1, 256);
-      if (w == 0 && ok && x.key0 + r < x.s.kv) {
-        float* dst = p.sums + x.b * p.sums_sb + x.hk * p.sums_sh + x.key0 + r;
-        *dst += (a + b) + half_sum[k & 1][r];
+      // the first warpgroup joins the others' sums while they go on
+      const int h = k & 1;
+      const uint32_t ph = (uint32_t)(k >> 1) & 1u;
+      if (w > 0) {
+        ok = ok && (k < 2 || wait(&sb.part_free[h], ph ^ 1u, RW_STATUS_TIMEOUT_SOFTMAX));
+        if (!ok) break;
+        part_sum[h][w - 1][r] = a + b;
+        mbar_arrive(&sb.part_full[h]);
+      } else {
+        ok = ok && wait(&sb.part_full[h], ph, RW_STATUS_TIMEOUT_SOFTMAX);
+        if (!ok) break;
+        float sum = a + b;
+#pragma unroll
+        for (int i = 0; i < NWG - 1; ++i) sum += part_sum[h][i][r];
+        mbar_arrive(&sb.part_free[h]);
+        // one thread of one CTA adds to a row's sum: an addition without a return value, whose order is no matter
+        if (x.key0 + r < x.s.kv) atomicAdd(p.sums + x.b * p.sums_sb + x.hk * p.sums_sh + x.key0 + r, sum);
       }
     }
   }
@@ -340,7 +355,7 @@ int launch(const rw_paged_t* cache, const Pool& pool, const chunk::Call& c, floa
   p.k_head = cache->Hkv == 1 ? 0 : (int)(cache->k_sh / kl.step);
   p.k_page = cache->num_pages == 1 ? 0 : (int)(cache->k_sp / kl.step);
   p.scale_log2 = c.scale_log2;
-  p.row_ml = c.row_ml;
+  p.row_b = c.row_b;
   p.sums = sums;
   p.sums_sb = sums_sb;
   p.sums_sh = sums_sh;
