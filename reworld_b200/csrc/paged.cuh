@@ -70,12 +70,16 @@ struct Num;
 
 template <>
 struct Num<false> {
+  static constexpr uint32_t EXP = 0x7F807F80u;  // exponent bits: all set in an infinity or NaN
+  static constexpr uint32_t ULP = 0x00800080u;  // their lowest ones
   static __device__ __forceinline__ float2 wide(uint32_t v) { return make_float2(bf16_lo(v), bf16_hi(v)); }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
 };
 
 template <>
 struct Num<true> {
+  static constexpr uint32_t EXP = 0x7C007C00u;
+  static constexpr uint32_t ULP = 0x04000400u;
   static __device__ __forceinline__ float2 wide(uint32_t v) {
     return __half22float2(*reinterpret_cast<const __half2*>(&v));
   }
@@ -85,6 +89,51 @@ struct Num<true> {
     return r;
   }
 };
+
+// Values of keys that only some rows of a tile see.  The weight of a key that a row does
+// not see is 0, but 0 times an infinity or NaN is NaN, and a token's value must not reach
+// the tokens before it.  So tiles with such keys are looked through before the second
+// product: values that are not finite are taken out (0), and, if there were any, added to
+// the rows that do see them afterwards (an infinity or NaN whatever its weight).
+//
+// has_nonfinite: sign bits of a word are set where its values are not finite (the magnitude
+// and one step of the exponent carry into the sign's place); other bits mean nothing.
+template <bool HALF>
+__device__ __forceinline__ uint32_t has_nonfinite(const uint4& v) {
+  const uint32_t u = Num<HALF>::ULP, m = 0x7FFF7FFFu;
+  return ((v.x & m) + u) | ((v.y & m) + u) | ((v.z & m) + u) | ((v.w & m) + u);
+}
+constexpr uint32_t SIGNS = 0x80008000u;
+
+template <bool HALF>
+__device__ __forceinline__ bool take_nonfinite(uint4& v) {
+  const uint32_t e = Num<HALF>::EXP;
+  const uint32_t a = __vcmpeq2(v.x & e, e), b = __vcmpeq2(v.y & e, e), c = __vcmpeq2(v.z & e, e),
+                 d = __vcmpeq2(v.w & e, e);
+  v.x &= ~a;
+  v.y &= ~b;
+  v.z &= ~c;
+  v.w &= ~d;
+  return (a | b | c | d) != 0u;
+}
+
+// add(c, x) for every value x that is not finite in channels [c0, c0 + n) of rows [from, to); n a multiple of 2.
+template <bool HALF, typename F>
+__device__ __forceinline__ void for_nonfinite(const Pool& p, int b, int hk, int from, int to, int c0, int n, F add) {
+#pragma unroll 1
+  for (int row = from; row < to; ++row) {
+    const long long pg = page_of(p, b, row, nullptr);
+    const uint8_t* src = p.v + pg * p.v_sp + (row & ((1 << p.page_shift) - 1)) * p.v_sl + hk * p.v_sh;
+#pragma unroll 1
+    for (int c = c0; c < c0 + n; c += 2) {
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(src + 2 * c), e = Num<HALF>::EXP;
+      const uint32_t m = __vcmpeq2(w & e, e);
+      const float2 x = Num<HALF>::wide(w);
+      if (m & 0xffffu) add(c, x.x);
+      if (m & 0xffff0000u) add(c + 1, x.y);
+    }
+  }
+}
 
 // Host: checks a rw_paged_t and makes the kernels' form of it.  RW_OK, or what is wrong.
 inline int make_pool(const rw_paged_t* a, Pool* p) {

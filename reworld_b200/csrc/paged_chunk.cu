@@ -17,11 +17,11 @@
 // Warps: two softmax warpgroups (tiles j even / odd, a row a thread), warp 8 loads q and keys,
 // warp 9 issues the MMAs, warp 10 loads the values, warp 11 plans.
 //
-// Pages: a tile is gathered by one TMA box a page (and 64 channels); page indices are read
-// one tile ahead.  Of the page that a sequence ends in,
-// the rows behind the end may hold anything: keys there are masked by selection, but a
-// weight of 0 times NaN is NaN, so the values of such a tile are not loaded by TMA; warp
-// 10 copies the rows that exist and writes zeros for the others.
+// Pages: a tile is gathered by one TMA box a page (and, of the values, 64 channels); page
+// indices are read one tile ahead.  Of the page that a sequence ends in, the rows behind
+// the end may hold anything.  Keys that a row does not see are masked by selection; of the
+// values of tiles that not every row sees whole, warp 11 zeroes the rows behind the end and
+// takes out what is not finite (paged.cuh) before the MMA warp gets them.
 //
 // Work: lengths are device data, so every CTA sums the key tiles of all units itself
 // (a few microseconds' latency, no host, no extra launch).  Pairs first take whole units
@@ -54,7 +54,6 @@ constexpr int SOFTMAX_THREADS = 256;
 constexpr int REG_SOFTMAX = 208, REG_OTHER = 88;
 static_assert(NWG * 128 * REG_SOFTMAX + 128 * REG_OTHER <= NUM_THREADS * 168, "register split exceeds the launch's");
 constexpr float RESCALE_THRESHOLD = 8.0f;    // log2 units
-constexpr int MAX_PARTS = 1024;              // slots of a launch (two a CTA or pair): checked by the host
 constexpr int MIN_SHARE = 12;                // cost of a share, where there is little work
 // What a unit costs beside its key tiles, in tiles: filling and draining the pipeline (q and
 // the first keys, the last softmax, the output) takes 5 to 8 us, a tile 0.75 to 0.9.
@@ -75,7 +74,8 @@ struct Seg {
   int kv0;
   int slot;              // -1: the whole unit
   int b, hk, tok0;       // unit's first token within the sequence
-  int s0, lq, kv, keys;  // keys: rows that any token of the unit sees
+  int s0, lq, kv;
+  int all;               // keys that every token of the unit sees
 };
 
 struct Params {
@@ -89,14 +89,16 @@ struct Params {
   float* lse;            // [T, Hq] or null
   float* row_b;          // [T, Hq]: -(m + log2 l) for the weight sums, or null
   float* scratch;        // [2 C] slots
-  int4* header;          // [2 C]: (b + 1 or 0, hk, tok0, unused)
+  int* dirty;            // [CTAs]: whether the CTA took out values that are not finite (join_kernel puts them back)
+  int4* header;          // [C]: the unit that the pair began and did not end: b, hk, tok0, parts (0: none)
   int kbox, vbox;        // rows of a TMA box: min(page, keys of a CTA), min(page, 128)
   int k_head, k_page;    // strides of head and page in the key map's last dimension
   int* status;
 };
 
 struct __align__(8) Barriers {
-  uint64_t pre_full, q_full, o_done, drain, v_tail, planned;
+  uint64_t pre_full, q_full, o_done, drain, planned;
+  uint64_t v_land[NSTAGE], v_ok[NSTAGE];
   uint64_t stage_full[NSTAGE], stage_free[NSTAGE];
   uint64_t s_full[NSBUF], p_ready[NSBUF], m_ready[NSBUF];
   uint32_t tmem_base;
@@ -333,9 +335,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     mbar_init(&sb.q_full, 1);
     mbar_init(&sb.o_done, 1);
     mbar_init(&sb.drain, 1);
-    mbar_init(&sb.v_tail, 32 * NCTA);
     mbar_init(&sb.planned, 1);
     for (int t = 0; t < NSTAGE; ++t) {
+      mbar_init(&sb.v_land[t], 1);
+      mbar_init(&sb.v_ok[t], 32 * NCTA);
       mbar_init(&sb.stage_full[t], 1);
       mbar_init(&sb.stage_free[t], 1);
     }
@@ -372,7 +375,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   __syncthreads();
 
   // ---- the planner's state (warp 11): its waves, then its share of the rest
-  long long t = 0, t1 = 0, before = 0;
+  long long t = 0, t1 = 0, before = 0, t_base = 0, t_rest = 1;
   int waves = 0, wave = 0, C = p.C;
   Walk wk{};
   bool in_tail = false;
@@ -396,8 +399,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         const long long e = min(t1, before + UNIT_COST + wk.n);
         s.kv0 = (int)max(0ll, t - before - UNIT_COST);
         s.n = (int)max(0ll, e - before - UNIT_COST) - s.kv0;
+        // a part: the unit's first one goes to the second slot of its pair (its share ends there), the others to the
+        // first slot of theirs (their shares begin inside the unit)
         s.slot = s.n == wk.n ? -1 : (s.kv0 > 0 ? 2 * pid : 2 * pid + 1);
         t = e;
+        if (even && lane == 0 && s.n > 0 && s.slot == 2 * pid + 1) {
+          // the last pair whose share meets the unit
+          const long long x = before + UNIT_COST + wk.n - 1 - t_base;
+          int c = (int)(x * C / t_rest);
+          while (c + 1 < C && t_rest * (c + 1) / C <= x) ++c;
+          while (c > 0 && t_rest * c / C > x) --c;
+          p.header[pid] = make_int4(wk.b, wk.hk, wk.rt * upt, c - pid + 1);
+        }
       }
     }
     if (s.n) {
@@ -407,8 +420,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       s.s0 = wk.s.s0;
       s.lq = wk.s.lq;
       s.kv = wk.s.kv;
-      s.keys = wk.keys;
-      if (even && lane == 0 && s.slot >= 0) p.header[s.slot] = make_int4(s.b + 1, s.hk, s.tok0, 0);
+      s.all = p.causal ? max(0, min(s.kv, s.kv - s.lq + s.tok0 + 1)) : s.kv;
     }
     if (lane == 0) {
       seg_sh[i & 1] = s;
@@ -420,22 +432,20 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     plan_sum(p, pl, lane);
     const long long N = pl.cost[p.pool.B];       // of all work
     const int U = pl.units[p.pool.B];
-    if (even && lane < 2) p.header[2 * pid + lane] = make_int4(0, 0, 0, 0);
-    __syncwarp();
+    if (even && lane == 0) p.header[pid] = make_int4(0, 0, 0, 0);
     if (N < (long long)C * MIN_SHARE) C = (int)min((long long)C, max((long long)U, (N + MIN_SHARE - 1) / MIN_SHARE));
     if (pid < C) {
       // about equal: no unit is over 1/8 longer than their mean
       if ((long long)pl.longest * U * 8 <= N * 9) waves = U / C;
-      long long t0 = 0;
       if (waves > 0 && waves * C < U) {
         const Walk f = walk_to_unit(p, pl, waves * C, upt);
-        t0 = cost_before(p, pl, f, upt, lane);
+        t_base = cost_before(p, pl, f, upt, lane);
       } else if (waves > 0) {
-        t0 = N;
+        t_base = N;
       }
-      const long long rest = N - t0;
-      t = t0 + rest * pid / C;
-      t1 = t0 + rest * (pid + 1) / C;
+      t_rest = N - t_base;
+      t = t_base + t_rest * pid / C;
+      t1 = t_base + t_rest * (pid + 1) / C;
     }
     plan_next(0);
   }
@@ -453,8 +463,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     tc_fence_after();
   };
   auto even_addr = [&](uint64_t* bar) { return NCTA == 2 ? mapa_shared(smem_u32(bar), 0) : smem_u32(bar); };
-  // whether the values of tile j (of the unit) are written by warp 10
-  auto ragged = [&](const Seg& sg, int j) { return sg.kv - j * BN < BN; };
+  // whether warp 11 looks through the values of tile j (of the unit): some row does not see all of it
+  auto checked = [&](const Seg& sg, int j) { return (j + 1) * BN > sg.all; };
 
   if (warp == WARP_LOAD) {
     setmaxnreg_dec<REG_OTHER>();
@@ -508,7 +518,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         bool ok = true;
         for (int j = 0; j < sg.n; ++j) {
           const int J = J0 + j, st = J % NSTAGE;
-          const bool has_k = j + NSBUF < sg.n, has_v = !ragged(sg, sg.kv0 + j);
+          const bool has_k = j + NSBUF < sg.n, has_v = !checked(sg, sg.kv0 + j);
           const int kn = page_at(sg, j + 1 + NSBUF);
           if (J >= NSTAGE &&
               !(ok = pwait_warp(&sb.stage_free[st], (uint32_t)(J / NSTAGE - 1) & 1u, cx, RW_STATUS_TIMEOUT_LOAD)))
@@ -549,7 +559,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     }
   } else if (warp == WARP_MMA) {
     setmaxnreg_dec<REG_OTHER>();
-    int J0 = 0, n_tail = 0;
+    int J0 = 0;
+    uint32_t phases = 0;                       // of v_ok
     for (int si = 0;; ++si) {
       const Seg sg = seg_sh[si & 1];
       if (sg.n == 0) break;
@@ -592,9 +603,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           const int J = J0 + j;
           if (!(ok = pwait_warp(&sb.p_ready[b], (uint32_t)(J / NSBUF) & 1u, cx, RW_STATUS_TIMEOUT_MMA))) break;
           if (!(ok = pwait_warp(&sb.stage_full[st], (uint32_t)(J / NSTAGE) & 1u, cx, RW_STATUS_TIMEOUT_MMA))) break;
-          if (ragged(sg, sg.kv0 + j)) {
-            if (!(ok = pwait_warp(&sb.v_tail, (uint32_t)n_tail & 1u, cx, RW_STATUS_TIMEOUT_MMA))) break;
-            ++n_tail;
+          if (checked(sg, sg.kv0 + j)) {
+            if (!(ok = pwait_warp(&sb.v_ok[st], (phases >> st) & 1u, cx, RW_STATUS_TIMEOUT_MMA))) break;
+            phases ^= 1u << st;
           }
           tc_fence_after();
           if (elect_one()) {
@@ -625,76 +636,84 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     for (int si = 0;; ++si) {
       const Seg sg = seg_sh[si & 1];
       if (sg.n == 0) break;
-      // values: 128 / vbox boxes a tile, up to the last tile where the sequence ends inside it
-      const bool tail = ragged(sg, sg.kv0 + sg.n - 1);
+      // values: 128 / vbox boxes a tile
       if (!aborted()) {
-        const int nvp = BN / p.vbox, n = tail ? sg.n - 1 : sg.n;
+        const int nvp = BN / p.vbox;
         const int mask = (1 << p.pool.page_shift) - 1;
         auto page_at = [&](int j) {
           const int row = (sg.kv0 + j) * BN + lane * p.vbox;
-          return lane < nvp && j < n ? paged::raw_page_of(p.pool, sg.b, row) : 0;
+          return lane < nvp && j < sg.n && row < sg.kv ? paged::raw_page_of(p.pool, sg.b, row) : 0;
         };
         int vp = page_at(0);
-        for (int j = 0; j < n; ++j) {
+        for (int j = 0; j < sg.n; ++j) {
           const int J = J0 + j, st = J % NSTAGE;
           const int vn = page_at(j + 1);
           if (J >= NSTAGE &&
               !pwait_warp(&sb.stage_free[st], (uint32_t)(J / NSTAGE - 1) & 1u, cx, RW_STATUS_TIMEOUT_LOAD))
             break;
-          const uint32_t bar = even_addr(&sb.stage_full[st]), dst = smem_u32(stages) + st * STAGE_BYTES;
+          // a tile that is looked through lands on this CTA's own barrier
+          const bool look = checked(sg, sg.kv0 + j);
+          const uint32_t bar = look ? smem_u32(&sb.v_land[st]) : even_addr(&sb.stage_full[st]);
+          const uint32_t dst = smem_u32(stages) + st * STAGE_BYTES;
+          if (look && lane == 0) mbar_expect_tx(&sb.v_land[st], HALF_TILE);
           const int row0 = ((sg.kv0 + j) * BN) & mask;
           vp = paged::checked_page(p.pool, vp, p.status);
+          __syncwarp();
           for_pages(vp, nvp, [&](int i, int pg) {
             load_4d<NCTA>(dst + i * p.vbox * 128, &tm_v, bar, 64 * (int)rank, sg.hk, nvp == 1 ? row0 : 0, pg);
           });
           vp = vn;
         }
       }
-      if (tail && !aborted()) {
-        const int j = sg.n - 1;                  // only a unit's last tile can be one
-        const int J = J0 + j, st = J % NSTAGE;
-        const int row0 = (sg.kv0 + j) * BN, rows = max(0, sg.kv - row0);
-        const int c = lane & 7, r0 = lane >> 3;
-        const uint8_t* src = p.pool.v + (long long)sg.hk * p.pool.v_sh + 128 * rank + 16 * c;
-        const int mask = (1 << p.pool.page_shift) - 1;
-        const bool ok = J < NSTAGE ||
-                        pwait_warp(&sb.stage_free[st], (uint32_t)(J / NSTAGE - 1) & 1u, cx, RW_STATUS_TIMEOUT_LOAD);
-        if (ok) {
-          uint8_t* dst = stages + st * STAGE_BYTES;
-#pragma unroll 1
-          for (int r8 = 0; r8 < BN; r8 += 32) {
-            uint4 v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int r = r8 + 4 * i + r0;
-              v[i] = make_uint4(0, 0, 0, 0);
-              if (r < rows) {
-                const long long pg = paged::page_of(p.pool, sg.b, row0 + r, nullptr);
-                v[i] = *reinterpret_cast<const uint4*>(src + pg * p.pool.v_sp + ((row0 + r) & mask) * p.pool.v_sl);
-              }
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int r = r8 + 4 * i + r0;
-              *reinterpret_cast<uint4*>(dst + r * 128 + ((c ^ (r & 7)) << 4)) = v[i];
-            }
-          }
-          fence_proxy_async_smem();
-          mbar_arrive_cluster(even_addr(&sb.v_tail));
-        }
-      }
-      __syncwarp();
       J0 += sg.n;
       boundary();
     }
   } else if (warp == WARP_PLAN) {
     setmaxnreg_dec<REG_OTHER>();
+    int J0 = 0;
+    uint32_t phases = 0;                       // of v_land
+    bool dirty = false;
     for (int si = 0;; ++si) {
-      const int n = seg_sh[si & 1].n;
-      if (n == 0) break;
+      const Seg sg = seg_sh[si & 1];
+      if (sg.n == 0) break;
       plan_next(si + 1);
+      // the values of the tiles that not every row sees whole: zeros behind the sequence's end, nothing that is not
+      // finite
+      for (int j = max(0, sg.all / BN - sg.kv0); j < sg.n; ++j) {
+        const int st = (J0 + j) % NSTAGE;
+        if (!pwait_warp(&sb.v_land[st], (phases >> st) & 1u, cx, RW_STATUS_TIMEOUT_LOAD)) break;
+        phases ^= 1u << st;
+        uint8_t* v = stages + st * STAGE_BYTES;
+        const int rows = max(0, sg.kv - (sg.kv0 + j) * BN), r0 = lane >> 3;
+        auto at = [&](int r) { return reinterpret_cast<uint4*>(v + r * 128 + (((lane & 7) ^ (r & 7)) << 4)); };
+#pragma unroll 1
+        for (int r = r0 + (max(0, rows - r0) + 3) / 4 * 4; r < BN; r += 4) *at(r) = make_uint4(0, 0, 0, 0);
+        uint32_t found = 0;
+        if (rows >= BN) {
+// (unrolled further, this loop cost the softmax loop 7 %: the kernel's code no longer fits where it did)
+#pragma unroll 2
+          for (int r = r0; r < BN; r += 4) found |= paged::has_nonfinite<HALF>(*at(r));
+        } else {
+#pragma unroll 1
+          for (int r = r0; r < rows; r += 4) found |= paged::has_nonfinite<HALF>(*at(r));
+        }
+        if (found & paged::SIGNS) {
+          dirty = true;
+#pragma unroll 1
+          for (int r = r0; r < rows; r += 4) {
+            uint4 x = *at(r);
+            if (paged::take_nonfinite<HALF>(x)) *at(r) = x;
+          }
+        }
+        fence_proxy_async_smem();
+        mbar_arrive_cluster(even_addr(&sb.v_ok[st]));
+      }
+      __syncwarp();
+      J0 += sg.n;
       boundary();
     }
+    dirty = __any_sync(0xffffffffu, dirty);
+    if (lane == 0) p.dirty[blockIdx.x] = dirty;
   } else {
     // ------------------------------------------------------------ softmax, then the output
     setmaxnreg_inc<REG_SOFTMAX>();
@@ -970,57 +989,79 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   }
 }
 
-// Joins the parts of the units that more than one pair worked on.  The parts of a unit
-// lie in consecutive used slots; the block of the first of them joins them, in the order
-// of the keys.  A thread has one row and 32 channels.
+// Row r of CTA `rank` of the unit of sequence b, key head hk and first token tok0: adds the values that are not finite
+// and that the row sees, of the tiles that chunk_kernel looked through, to channels [c0, c0 + 32) of its output.
+template <bool HALF, int D>
+__device__ __noinline__ void mend_row(const Params& p, const Seq& sq, int b, int hk, int tok0, int tok, int head, int c0) {
+  const int all = p.causal ? max(0, min(sq.kv, sq.kv - sq.lq + tok0 + 1)) : sq.kv;
+  const int lim = p.causal ? max(0, sq.kv - sq.lq + tok + 1) : sq.kv;
+  uint16_t* out = reinterpret_cast<uint16_t*>(p.out + (long long)(sq.s0 + tok) * p.o_sl + (long long)head * p.o_sh);
+  paged::for_nonfinite<HALF>(p.pool, b, hk, all / BN * BN, min(lim, sq.kv), c0, 32, [&](int c, float x) {
+    out[c] = (uint16_t)Num<HALF>::pack(Num<HALF>::wide(out[c]).x + x, 0.f);
+  });
+}
+
+constexpr int MEND_BLOCKS = 64;
+
+// Joins the parts of a unit that more than one pair worked on: the block of the pair that
+// began it, in the order of the keys.  A thread has one row and 32 channels.  If values
+// that are not finite were taken out somewhere, MEND_BLOCKS more go through all units and
+// put them back (otherwise they leave at once); the rows of joined units get theirs here.
 template <bool HALF, int D>
 __global__ void __launch_bounds__(BM) join_kernel(const __grid_constant__ Params p) {
   griddep_launch_dependents();
   griddep_wait();
-  constexpr int R = Shape<D>::NCTA * BM;
-  __shared__ int part[MAX_PARTS];
-  __shared__ int n_parts, n_before;
-  const int s = blockIdx.x, r = threadIdx.x;
-  const int4 h = __ldcg(p.header + s);
-  if (h.x == 0) return;
-  auto same = [&](const int4& o) { return o.x == h.x && o.y == h.y && o.z == h.z; };
-  // the unit's slots from s on, in order (a unit's used slots follow one another); none may come before s
-  if (r == 0) { n_parts = 0; n_before = 0; }
-  __syncthreads();
-  for (int o = r; o < 2 * p.C; o += BM) {
-    if (!same(__ldcg(p.header + o))) continue;
-    if (o < s) n_before = 1; else atomicAdd(&n_parts, 1);
-  }
-  __syncthreads();
-  if (n_before) return;
-  const int n = n_parts;
-  if (r < 32) {
-    // compaction by the first warp, in order
-    int at = 0;
-    for (int o0 = s; o0 < 2 * p.C && at < n; o0 += 32) {
-      const bool mine = o0 + r < 2 * p.C && same(__ldcg(p.header + o0 + r));
-      const unsigned m = __ballot_sync(0xffffffffu, mine);
-      if (mine) part[at + __popc(m & ((1u << r) - 1u))] = o0 + r;
-      at += __popc(m);
-    }
-  }
-  __syncthreads();
+  constexpr int NCTA = Shape<D>::NCTA;
+  constexpr int R = NCTA * BM;
+  constexpr long long SLOT = Shape<D>::SLOT_FLOATS;
+  const int pid = blockIdx.x, r = threadIdx.x;
   const int rank = blockIdx.y, row = rank * BM + r, c0 = 32 * blockIdx.z;
-  const Seq sq = paged::load_seq(p.pool, h.x - 1, p.T, nullptr);
   const int rtok = r / p.G, g = r - rtok * p.G;
+  auto any_dirty = [&]() {
+    int d = 0;
+    for (int i = r; i < NCTA * p.C; i += BM) d |= __ldcg(p.dirty + i);
+    return __syncthreads_or(d) != 0;
+  };
+  if (pid >= p.C) {
+    if (!any_dirty()) return;
+    const int upt = NCTA * p.tpc;
+    int u = 0;
+    for (int b = 0; b < p.pool.B; ++b) {
+      const Seq sq = paged::load_seq(p.pool, b, p.T, nullptr);
+      const int nu = units_of(p, sq, upt);
+      for (int i = 0; i < nu * p.pool.Hkv; ++i, ++u) {
+        if (u % MEND_BLOCKS != pid - p.C) continue;
+        const int hk = i / nu, tok0 = (i - hk * nu) * upt, tok = tok0 + rank * p.tpc + rtok;
+        int joined = 0;
+        for (int c = r; c < p.C; c += BM) {
+          const int4 h = __ldcg(p.header + c);
+          joined |= h.w > 0 && h.x == b && h.y == hk && h.z == tok0;
+        }
+        if (__syncthreads_or(joined)) continue;
+        if (r < p.tpc * p.G && tok < sq.lq) mend_row<HALF, D>(p, sq, b, hk, tok0, tok, hk * p.G + g, c0);
+      }
+    }
+    return;
+  }
+  const int4 h = __ldcg(p.header + pid);
+  const int n = min(h.w, p.C - pid);
+  if (n <= 0) return;
+  const bool mend = any_dirty();
+  const Seq sq = paged::load_seq(p.pool, h.x, p.T, nullptr);
   const int tok = h.z + rank * p.tpc + rtok;
   if (r >= p.tpc * p.G || tok >= sq.lq) return;
-  const float* ml = p.scratch + (long long)D * R + row;
+  // part i: slot 2 pid + 1, then 2 (pid + 1), 2 (pid + 2), ...
+  auto slot = [&](int i) { return p.scratch + (2LL * (pid + i) + (i == 0)) * SLOT + row; };
   float m = -INFINITY;
 #pragma unroll 8
-  for (int i = 0; i < n; ++i) m = fmaxf(m, __ldcg(ml + part[i] * Shape<D>::SLOT_FLOATS));
+  for (int i = 0; i < n; ++i) m = fmaxf(m, __ldcg(slot(i) + (long long)D * R));
   float acc[32], l = 0.f;
 #pragma unroll
   for (int e = 0; e < 32; ++e) acc[e] = 0.f;
   const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll 2
   for (int i = 0; i < n; ++i) {
-    const float* sl = p.scratch + part[i] * Shape<D>::SLOT_FLOATS + row;
+    const float* sl = slot(i);
     const float f = fast_exp2((__ldcg(sl + (long long)D * R) - base) * p.scale_log2);
     l += f * __ldcg(sl + (long long)D * R + R);
 #pragma unroll
@@ -1043,6 +1084,7 @@ __global__ void __launch_bounds__(BM) join_kernel(const __grid_constant__ Params
     if (p.lse) p.lse[at] = l != 0.f ? (m * p.scale_log2 + log2f(l)) * 0.6931471805599453f : -INFINITY;
     if (p.row_b) p.row_b[at] = l != 0.f ? -(m * p.scale_log2 + log2f(l)) : -INFINITY;
   }
+  if (mend) mend_row<HALF, D>(p, sq, h.x, h.y, h.z, tok, head, c0);
 }
 
 // ---------------------------------------------------------------- host
@@ -1076,7 +1118,7 @@ int grid_size(int D) {
 
 long long workspace_bytes(int D) {
   const long long C = grid_size(D);
-  return 2 * C * ((D == 128 ? Shape<128>::SLOT_FLOATS : Shape<64>::SLOT_FLOATS) * 4 + 16);
+  return C * (2 * 4 * (D == 128 ? Shape<128>::SLOT_FLOATS : Shape<64>::SLOT_FLOATS) + 32);
 }
 
 template <bool HALF, int D>
@@ -1100,7 +1142,7 @@ int launch_one(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& 
   cfg.attrs = attr;
   cfg.numAttrs = NCTA == 2 ? 2 : 1;
   if (cudaLaunchKernelEx(&cfg, chunk_kernel<HALF, D>, mq, mk, mv, p) != cudaSuccess) return RW_ERR_CUDA;
-  return launch_dependent(join_kernel<HALF, D>, dim3(2 * p.C, NCTA, D / 32), dim3(BM), 0, st, p) == cudaSuccess
+  return launch_dependent(join_kernel<HALF, D>, dim3(p.C + MEND_BLOCKS, NCTA, D / 32), dim3(BM), 0, st, p) == cudaSuccess
              ? RW_OK : RW_ERR_CUDA;
 }
 
@@ -1110,14 +1152,15 @@ int launch(const rw_paged_t* cache, const Pool& pool, const Call& c, void* works
   p.T = c.T; p.Hq = c.Hq; p.G = c.Hq / pool.Hkv; p.causal = c.causal;
   p.tpc = BM / p.G;
   p.C = grid_size(cache->D);
-  if (p.C < 1 || 2 * p.C > MAX_PARTS) return RW_ERR_CUDA;
+  if (p.C < 1) return RW_ERR_CUDA;
   p.scale_log2 = c.scale_log2;
   p.out = static_cast<uint8_t*>(c.out);
   p.o_sl = 2 * c.o_sl; p.o_sh = 2 * c.o_sh;
   p.lse = c.lse;
   p.row_b = c.row_b;
   p.header = static_cast<int4*>(workspace);
-  p.scratch = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 2LL * p.C * 16);
+  p.dirty = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + 16LL * p.C);
+  p.scratch = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 32LL * p.C);
   const int krows = cache->D == 128 ? Shape<128>::KROWS : Shape<64>::KROWS;
   p.kbox = cache->page_size < krows ? cache->page_size : krows;
   p.vbox = cache->page_size < BN ? cache->page_size : BN;

@@ -5,10 +5,11 @@
 // pages shared with other sequences stay whole and every row can move at once.
 //
 // select_kernel, one CTA for a sequence and key head: finds the smallest kept sum by
-// radix selection (four passes over the sums with an 8-bit histogram each; the sums,
-// 4 bytes a row, stay in L2), then one pass that numbers the kept rows with a running
-// scan and writes their indices and sums.  move_kernel copies the kept rows of k and v,
-// 16 bytes a thread; it is bound by memory (a kept row is read and written once).
+// radix selection (three passes over the sums, which stay in L2, with histograms of 11, 11
+// and 10 bits: 11 bits hold the exponent and three more, so that sums of a similar size
+// do not all meet in one counter), then numbers the kept rows with one scan for every
+// 16384 rows and writes their indices and sums.  move_kernel copies the kept rows of k and
+// v, 16 bytes a thread; it is bound by memory (a kept row is read and written once).
 #include "paged.cuh"
 
 namespace rw {
@@ -16,10 +17,8 @@ namespace evict {
 
 using paged::Pool;
 
-constexpr int THREADS = 1024;
-constexpr int WARPS = THREADS / 32;
-constexpr int PER = 4;               // rows of a thread in a step of the last pass
-constexpr int STEP = THREADS * PER;
+constexpr int BINS = 2048;
+constexpr int PER = 16;              // sums of a thread under way at once
 
 struct Params {
   Pool pool;
@@ -50,9 +49,35 @@ __device__ __forceinline__ int rows_of(const Params& p, int b, int* status) {
   return kv;
 }
 
-__global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__ Params p) {
-  __shared__ unsigned hist[WARPS][256];
+// Inclusive sums over the block of a value of every thread, in thread order; `all` is their total.
+template <int THREADS>
+__device__ __forceinline__ unsigned block_scan(unsigned x, unsigned* scan, unsigned* all) {
+  constexpr int WARPS = THREADS / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) scan[warp] = x;
+  __syncthreads();
+  // every warp sums up the warps' totals for itself
+  unsigned w = lane < WARPS ? scan[lane] : 0u;
+#pragma unroll
+  for (int o = 1; o < WARPS; o <<= 1) {
+    const unsigned y = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += y;
+  }
+  *all = __shfl_sync(0xffffffffu, w, WARPS - 1);
+  return x + (warp > 0 ? __shfl_sync(0xffffffffu, w, warp - 1) : 0u);
+}
+
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS, 1) select_kernel(const __grid_constant__ Params p) {
+  constexpr int WARPS = THREADS / 32, STEP = THREADS * PER, DIGITS = BINS / THREADS;
+  __shared__ unsigned hist[BINS];
   __shared__ unsigned scan[WARPS];
+  __shared__ unsigned count[PER * WARPS];    // kept (low half) and tied (high half) rows of every 32
   __shared__ unsigned s_digit, s_left;
   griddep_launch_dependents();
   griddep_wait();
@@ -73,46 +98,47 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__
     return;
   }
   const int lo = min(p.n_sink, kv), hi = kv - p.n_recent;   // rows [lo, hi) compete; lo <= hi since sink + recent <= keep < kv
-  unsigned need = (unsigned)(p.keep - p.n_sink - p.n_recent);
-  // ---- the need-th largest sum of [lo, hi): its bits from the top, 8 at a time
+  const unsigned need = (unsigned)(p.keep - p.n_sink - p.n_recent);
+  // ---- the need-th largest sum of [lo, hi): its bits from the top
   uint32_t prefix = 0;
   unsigned left = need;                      // of the rows with this prefix
   if (need > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = lane; i < 256; i += 32) hist[warp][i] = 0;
-      __syncwarp();
-      for (int i = lo + tid; i < hi; i += THREADS) {
-        const uint32_t o = order_of(x[i]);
-        if (shift == 24 || (o >> (shift + 8)) == prefix) atomicAdd(&hist[warp][(o >> shift) & 255u], 1u);
-      }
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const int bits = pass < 2 ? 11 : 10, shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
+      for (int i = tid; i < BINS; i += THREADS) hist[i] = 0;
       __syncthreads();
-      if (tid < 256) {
-        unsigned n = 0;
-        for (int w = 0; w < WARPS; ++w) n += hist[w][tid];
-        hist[0][tid] = n;
-      }
-      __syncthreads();
-      if (warp == 0) {
-        // rows with a larger digit than each: lane holds digits 8 lane .. 8 lane + 7
-        unsigned mine = 0;
-        for (int i = 0; i < 8; ++i) mine += hist[0][8 * lane + i];
-        unsigned above = mine;               // suffix sum over lanes
-        for (int o = 1; o < 32; o <<= 1) {
-          const unsigned y = __shfl_down_sync(0xffffffffu, above, o);
-          if (lane + o < 32) above += y;
+      for (int i0 = lo; i0 < hi; i0 += STEP) {
+        float v[PER];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          const int i = i0 + j * THREADS + tid;
+          v[j] = i < hi ? x[i] : 0.f;
         }
-        above -= mine;
-        for (int i = 7; i >= 0; --i) {
-          const unsigned n = hist[0][8 * lane + i];
-          if (above < left && left <= above + n) {
-            s_digit = 8 * lane + i;
-            s_left = left - above;
-          }
-          above += n;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          if (i0 + j * THREADS >= hi) break;
+          const uint32_t o = order_of(v[j]);
+          if (i0 + j * THREADS + tid < hi && (pass == 0 || (o >> (shift + bits)) == prefix))
+            atomicAdd(&hist[(o >> shift) & (BINS - 1u) & ((1u << bits) - 1u)], 1u);
         }
       }
       __syncthreads();
-      prefix = (prefix << 8) | s_digit;
+      // a thread has DIGITS digits, thread 0 the largest: how many rows have a larger one
+      unsigned n[DIGITS], mine = 0, all;
+#pragma unroll
+      for (int i = 0; i < DIGITS; ++i) mine += n[i] = hist[BINS - 1 - DIGITS * tid - i];
+      unsigned above = block_scan<THREADS>(mine, scan, &all) - mine;
+#pragma unroll
+      for (int i = 0; i < DIGITS; ++i) {
+        if (above < left && left <= above + n[i]) {
+          s_digit = BINS - 1 - DIGITS * tid - i;
+          s_left = left - above;
+        }
+        above += n[i];
+      }
+      __syncthreads();
+      prefix = (prefix << bits) | s_digit;
       left = s_left;
       __syncthreads();
     }
@@ -120,75 +146,65 @@ __global__ void __launch_bounds__(THREADS) select_kernel(const __grid_constant__
   // ---- number the kept rows: sink, recent, sums above the threshold, and the first `left` equal to it
   unsigned done_keep = 0, done_ties = 0;     // kept without the ties, ties seen, before this step
   for (int i0 = 0; i0 < kv; i0 += STEP) {
-    unsigned flag[PER], mine = 0;            // low half: kept without the ties, high half: ties (a step has 4096 rows)
-    float val[PER];
+    float v[PER];
+    unsigned keep_m[PER], tie_m[PER];        // of the warp's 32 rows
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      const int i = i0 + tid * PER + j;
-      flag[j] = 0;
-      val[j] = 0.f;
-      if (i < kv) {
-        val[j] = x[i];
-        if (i < lo || i >= hi) {
-          flag[j] = 1u;
-        } else if (need > 0) {
-          const uint32_t o = order_of(val[j]);
-          flag[j] = o > prefix ? 1u : (o == prefix ? 0x10000u : 0u);
-        }
-      }
-      mine += flag[j];
+      const int i = i0 + j * THREADS + tid;
+      v[j] = i < kv ? x[i] : 0.f;
     }
-    unsigned s = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned y = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += y;
-    }
-    if (lane == 31) scan[warp] = s;
-    __syncthreads();
-    if (warp == 0) {
-      unsigned w = scan[lane];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned y = __shfl_up_sync(0xffffffffu, w, o);
-        if (lane >= o) w += y;
-      }
-      scan[lane] = w;
-    }
-    __syncthreads();
-    unsigned before = s - mine + (warp > 0 ? scan[warp - 1] : 0u);
-    const unsigned total = scan[WARPS - 1];
-    unsigned nk = done_keep + (before & 0xffffu), nt = done_ties + (before >> 16);
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      const bool tie = flag[j] == 0x10000u;
-      if (flag[j] == 1u || (tie && nt < left)) {
+      const int i = i0 + j * THREADS + tid;
+      if (i0 + j * THREADS >= kv) {
+        if (lane == 0) count[j * WARPS + warp] = 0;
+        continue;
+      }
+      const uint32_t o = order_of(v[j]);
+      const bool fixed = i < kv && (i < lo || i >= hi), runs = i >= lo && i < hi && need > 0;
+      keep_m[j] = __ballot_sync(0xffffffffu, fixed || (runs && o > prefix));
+      tie_m[j] = __ballot_sync(0xffffffffu, runs && o == prefix);
+      if (lane == 0) count[j * WARPS + warp] = (unsigned)__popc(keep_m[j]) | ((unsigned)__popc(tie_m[j]) << 16);
+    }
+    __syncthreads();
+    // the groups of 32 in their order (at most 16384 rows a step: the halves do not run over); exclusive sums
+    unsigned all;
+    const unsigned mine = tid < PER * WARPS ? count[tid] : 0u;
+    const unsigned upto = block_scan<THREADS>(mine, scan, &all);
+    if (tid < PER * WARPS) count[tid] = upto - mine;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      if (i0 + j * THREADS >= kv) break;
+      const unsigned before = count[j * WARPS + warp], under = (1u << lane) - 1u;
+      const unsigned nk = done_keep + (before & 0xffffu) + __popc(keep_m[j] & under);
+      const unsigned nt = done_ties + (before >> 16) + __popc(tie_m[j] & under);
+      const bool tie = (tie_m[j] >> lane) & 1u;
+      if (((keep_m[j] >> lane) & 1u) || (tie && nt < left)) {
         const unsigned at = nk + min(nt, left);
-        kept[at] = i0 + tid * PER + j;
-        ns[at] = val[j];
+        kept[at] = i0 + j * THREADS + tid;
+        ns[at] = v[j];
       }
-      nk += flag[j] & 0xffffu;
-      nt += flag[j] >> 16;
     }
-    done_keep += total & 0xffffu;
-    done_ties += total >> 16;
+    done_keep += all & 0xffffu;
+    done_ties += all >> 16;
     __syncthreads();
   }
 }
 
-constexpr int MOVE_THREADS = 256;
+constexpr int MOVE_THREADS = 128;
 
 template <int D>
 __global__ void __launch_bounds__(MOVE_THREADS) move_kernel(const __grid_constant__ Params p) {
   constexpr int CH = D / 8;
-  constexpr int ROWS = 4;                    // rows of a thread, all loaded before the first is stored
+  constexpr int ROWS = 2;                    // rows of a thread, all loaded before the first is stored
   constexpr int RSTEP = MOVE_THREADS / CH;
   griddep_launch_dependents();
   griddep_wait();
-  const int hk = blockIdx.y, b = blockIdx.z;
+  const int hk = blockIdx.x, b = blockIdx.z;
   const int c = threadIdx.x % CH;
   const int n_new = min(rows_of(p, b, nullptr), p.keep);
-  const int j0 = blockIdx.x * (ROWS * RSTEP) + threadIdx.x / CH;
+  const int j0 = blockIdx.y * (ROWS * RSTEP) + threadIdx.x / CH;
   const int* kept = p.kept + ((long long)b * p.pool.Hkv + hk) * p.keep;
   const int mask = (1 << p.pool.page_shift) - 1;
   uint4 kr[ROWS], vr[ROWS];
@@ -215,8 +231,8 @@ __global__ void __launch_bounds__(MOVE_THREADS) move_kernel(const __grid_constan
       }
       uint8_t* kd = const_cast<uint8_t*>(p.pool.k) + pg * p.pool.k_sp + (j & mask) * p.pool.k_sl + hk * p.pool.k_sh;
       uint8_t* vd = const_cast<uint8_t*>(p.pool.v) + pg * p.pool.v_sp + (j & mask) * p.pool.v_sl + hk * p.pool.v_sh;
-      *reinterpret_cast<uint4*>(kd + 16 * c) = kr[i];
-      *reinterpret_cast<uint4*>(vd + 16 * c) = vr[i];
+      __stcs(reinterpret_cast<uint4*>(kd + 16 * c), kr[i]);
+      __stcs(reinterpret_cast<uint4*>(vd + 16 * c), vr[i]);
     }
   }
 }
@@ -245,11 +261,13 @@ extern "C" int rw_paged_evict(const rw_paged_t* cache, const float* sums, long l
   p.dst_table = dst_table; p.dst_stride = dst_stride; p.dst_width = dst_width;
   p.status = status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (launch_dependent(evict::select_kernel, dim3(p.pool.Hkv, cache->B), dim3(evict::THREADS), 0, st, p) !=
-      cudaSuccess)
+  // A short row needs few threads, and barriers cost less with few (evicting from 1000 rows 10.3 us, with 1024 threads 12.9; from 4000 rows 14.7 and 16.0).
+  const bool few = (long long)cache->table_width * cache->page_size <= 4096;
+  if (launch_dependent(few ? evict::select_kernel<256> : evict::select_kernel<1024>, dim3(p.pool.Hkv, cache->B),
+                       dim3(few ? 256 : 1024), 0, st, p) != cudaSuccess)
     return RW_ERR_CUDA;
-  const int rows = 4 * evict::MOVE_THREADS / (cache->D / 8);
-  const dim3 grid((keep + rows - 1) / rows, p.pool.Hkv, cache->B);
+  const int rows = 2 * evict::MOVE_THREADS / (cache->D / 8);
+  const dim3 grid(p.pool.Hkv, (keep + rows - 1) / rows, cache->B);
   auto kernel = cache->D == 128 ? evict::move_kernel<128> : evict::move_kernel<64>;
   return launch_dependent(kernel, grid, dim3(evict::MOVE_THREADS), 0, st, p) == cudaSuccess ? RW_OK : RW_ERR_CUDA;
 }

@@ -144,6 +144,7 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
   __shared__ long long base[THREADS + 1];
   __shared__ int come;
   __shared__ float sm_m[WARPS][RT], sm_l[WARPS][RT];
+  __shared__ int dirty;         // 1: the segment has values that are not finite (paged.cuh)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int grp = lane >> 2, quad = lane & 3;
   griddep_launch_dependents();
@@ -260,6 +261,9 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
       pg = nx;
     }
 
+    // keys that every row sees: tiles behind them are looked through for values that are not finite
+    const int all = p.causal ? min(en.keys, max(0, s.kv - s.lq + en.row0 / p.G + 1)) : en.keys;
+    if (tid == 0) dirty = 0;                 // (read after the barriers below)
     float o[D / 8][4];
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
@@ -277,6 +281,19 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
       const uint32_t ks = sbase + (uint32_t)((j - k0) % STAGES) * STAGE;
       const uint32_t vs = ks + TILE * PITCH;
       const int kw = warp * 16;              // this warp's keys of the tile
+      if (all < en.keys && (j + 1) * TILE > all) {
+        bool found = false;
+        for (int i = lane; i < 16 * CH; i += 32) {
+          uint4* at = reinterpret_cast<uint4*>(smem + (vs - sbase) + (kw + i / CH) * PITCH + 16 * (i % CH));
+          uint4 x = *at;
+          if (paged::take_nonfinite<HALF>(x)) {
+            *at = x;
+            found = true;
+          }
+        }
+        if (found) dirty = 1;
+        __syncwarp();
+      }
       float sc[2][4];
 #pragma unroll
       for (int i = 0; i < 2; ++i) sc[i][0] = sc[i][1] = sc[i][2] = sc[i][3] = 0.f;
@@ -400,6 +417,12 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
         v.x += f * x.x;
         v.y += f * x.y;
         ll += f * sm_l[w][r];
+      }
+      if (dirty) {
+        // taken-out values go to the rows that see them
+        const int lim = p.causal ? max(0, s.kv - s.lq + (en.row0 + r) / p.G + 1) : s.kv;
+        paged::for_nonfinite<HALF>(p.pool, b, hk, max(all / TILE, k0) * TILE, min(lim, k1 * TILE), c, 2,
+                                   [&](int ch, float x) { (ch == c ? v.x : v.y) += x; });
       }
       if (whole) {
         put(r, c, v, mm, ll);

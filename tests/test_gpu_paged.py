@@ -190,6 +190,50 @@ def test_large_and_infinite_scores(cuda, lq):
     assert torch.isfinite(out.float()).all()
 
 
+@pytest.mark.parametrize("dtype,D,hq,hkv", [(BF, 128, 4, 4), (FP, 64, 6, 2), (BF, 128, 8, 1)])
+@pytest.mark.parametrize("lqs,lens", [([5, 3], [40, 200]), ([300, 17], [300, 900]), ([2, 260], [1500, 2000])])
+def test_values_of_later_tokens_that_are_not_finite(cuda, dtype, D, hq, hkv, lqs, lens):
+    """Infinities and NaN in a token's key and value reach that token and those behind it, no other."""
+    from reworld_b200 import paged_attention
+    k, v, table, kv, g = _cache(cuda, lens, 16, hkv, D, dtype, 12)
+    s = _starts(cuda, lqs)
+    q = torch.randn(sum(lqs), hq, D, generator=g, device=cuda).to(dtype)
+    ref, lref = paged_attention(q, k, v, table, s, kv, max_q_len=max(lqs), return_lse=True)
+    inf, nan = float("inf"), float("nan")
+    for b, (lq, n) in enumerate(zip(lqs, lens)):
+        # the last token's value, one in the middle, and the last token's key
+        for tok, ch, x in ((lq - 1, 3, nan), (lq // 2, 5, inf), (lq // 2, D - 1, -inf), (lq // 2 + 1, 5, -inf)):
+            row = n - lq + min(tok, lq - 1)
+            v[int(table[b, row // 16]), row % 16, :, ch] = x
+        row = n - 1
+        k[int(table[b, row // 16]), row % 16, 0, 1] = nan
+    out, lse = paged_attention(q, k, v, table, s, kv, max_q_len=max(lqs), return_lse=True)
+    torch.cuda.synchronize()
+    _status_clean()
+    G, t = hq // hkv, 0
+    for lq in lqs:
+        mid, last = lq // 2, lq - 1
+        for i in range(lq):
+            got, want = out[t + i].float(), ref[t + i].float().clone()
+            if i >= mid:
+                want[:, 5], want[:, D - 1] = inf, -inf
+            if i >= min(mid + 1, last):
+                want[:, 5] = nan if min(mid + 1, last) != mid else -inf
+            if i >= last:
+                want[:, 3] = nan
+                want[:G] = nan                           # its key was NaN too
+            assert torch.equal(torch.isnan(got), torch.isnan(want)), (i, lq)
+            ok = torch.isfinite(want)
+            assert torch.equal(got[~ok & ~torch.isnan(want)], want[~ok & ~torch.isnan(want)])
+            # the rest differs by nothing: the same sums, with zeros in the places of what was taken out...
+            if i < mid:
+                assert torch.equal(got, want), i
+        t += lq
+    # ...and the weights did not see the values at all
+    rows = torch.isfinite(lse)
+    assert torch.equal(lse[rows], lref[rows])
+
+
 def test_strided_inputs_and_output(cuda):
     from reworld_b200 import paged_attention
     k, v, table, kv, g = _cache(cuda, [100, 50], 16, 2, 128, BF, 4)
