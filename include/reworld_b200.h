@@ -439,11 +439,11 @@ int rw_paged_rotary_store(const rw_paged_t* cache, const void* k, const void* v,
  * softmax(q[t, h] k^T * softmax_scale) v over key head h / (Hq / Hkv), fp32
  * statistics and accumulation, one rounding of the output.  causal != 0: token i
  * of a sequence with lq new tokens sees rows 0 .. kv - lq + i, otherwise all kv.
- * A row that sees nothing gets zeros and lse -inf.  What lies in a page behind
- * the rows that a token sees has no effect, NaN included.  lse ([T, Hq] fp32,
+ * A row that sees nothing gets zeros and lse -inf.  What a token does not see has
+ * no effect on it, infinities and NaN in later rows included.  lse ([T, Hq] fp32,
  * may be NULL): natural logarithm of the sum of exp(score).  Hq / Hkv <= 128.
- * max_q_len: no sequence has more new tokens (rows of a longer one are not
- * computed).  Rows of out and lse behind the last sequence stay as they were.
+ * max_q_len: no sequence has more new tokens (the rows of a longer one are
+ * undefined).  Rows of out and lse behind the last sequence stay as they were.
  * sums (may be NULL): fp32 [B, Hkv, >= table_width * page_size] with element strides
  * sums_sb, sums_sh; sums[b, g, j] += the weights that the rows of key head g's group
  * gave to cached row j.  The order of the additions is fixed.

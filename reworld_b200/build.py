@@ -2,18 +2,24 @@
 
 Each .cu file under csrc/ is compiled with nvcc for `-gencode
 arch=compute_100a,code=sm_100a` and the objects are linked into one shared
-library that the package loads with ctypes.  Run `python reworld_b200/build.py`
+library that the package loads with ctypes.  csrc/paged_bind.cpp (argument checks
+of paged.py on torch's C++ tensors, no device code) becomes a Python module beside
+it, linked to that library.  Run `python reworld_b200/build.py`
 (by path: importing the package requires the library to exist) or call build().
 """
 import concurrent.futures
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_lib")
 LIB_NAME = "libreworld_b200.so"
+BIND_NAME = "paged_bind.so"
+CXX = os.environ.get("CXX", "g++")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]
@@ -34,11 +40,40 @@ def lib_path():
     return os.path.join(OUT_DIR, LIB_NAME)
 
 
+def bind_path():
+    return os.path.join(OUT_DIR, BIND_NAME)
+
+
+def _compile_bind(obj):
+    """Compiles paged_bind.cpp to `obj` and returns the command that links it."""
+    # found, not imported: a build needs torch's headers and libraries only
+    torch_dir = list(importlib.util.find_spec("torch").submodule_search_locations)[0]
+    inc = os.path.join(torch_dir, "include")
+    lib = os.path.join(torch_dir, "lib")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")
+    cmd = [CXX, "-O2", "-std=c++20", "-fPIC", "-fvisibility=hidden", "-w", "-c", os.path.join(CSRC, "paged_bind.cpp"),
+           "-o", obj, "-isystem", inc, "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"), "-isystem", cuda,
+           "-isystem", sysconfig.get_paths()["include"]]
+    _run(cmd)
+    return [CXX, "-shared", "-o", bind_path() + ".tmp", obj, "-L" + lib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+           "-L" + OUT_DIR, "-lreworld_b200",
+           # (the CUDA runtime that torch loads)
+           "-Wl,--copy-dt-needed-entries", "-Wl,-rpath," + lib, "-Wl,-rpath,$ORIGIN"]
+
+
+def _run(cmd):
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{' '.join(cmd)} failed:\n{r.stdout}\n{r.stderr}")
+
+
 def build(force=False, verbose=False):
-    """Compiles csrc/*.cu into _lib/libreworld_b200.so (skipped when up to date)."""
+    """Compiles csrc/*.cu into _lib/libreworld_b200.so and csrc/paged_bind.cpp into
+    _lib/paged_bind.so (skipped when up to date)."""
     os.makedirs(OUT_DIR, exist_ok=True)
     out = lib_path()
-    if not force and os.path.exists(out) and os.path.getmtime(out) >= _newest_input_mtime():
+    newest = _newest_input_mtime()
+    if not force and all(os.path.exists(f) and os.path.getmtime(f) >= newest for f in (out, bind_path())):
         return out
     objs = []
 
@@ -55,14 +90,19 @@ def build(force=False, verbose=False):
         return obj
 
     with concurrent.futures.ThreadPoolExecutor(max_workers=os.cpu_count() or 4) as ex:
+        bind_obj = os.path.join(OUT_DIR, "paged_bind.o")
+        bind = ex.submit(_compile_bind, bind_obj)
         objs = list(ex.map(compile_one, _sources()))
+        link_bind = bind.result()
     tmp = out + ".tmp"
     cmd = [NVCC, *ARCH, "-shared", "-o", tmp, *objs, "-cudart=static"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, out)
-    for o in objs:
+    _run(link_bind)
+    os.replace(bind_path() + ".tmp", bind_path())
+    for o in objs + [bind_obj]:
         os.remove(o)
     return out
 
