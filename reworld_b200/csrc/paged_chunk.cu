@@ -29,6 +29,8 @@
 // if the units are about equal; what does not fill a wave, or all of it if they are not,
 // is one sequence of tiles of which every pair takes an equal share, and the parts of
 // units that more than one pair worked on are joined by join_kernel.
+#include <algorithm>
+
 #include "paged.cuh"
 #include "paged_chunk.h"
 #include "paged_tiles.cuh"
@@ -1153,6 +1155,12 @@ int launch(const rw_paged_t* cache, const Pool& pool, const Call& c, void* works
   p.tpc = BM / p.G;
   p.C = grid_size(cache->D);
   if (p.C < 1) return RW_ERR_CUDA;
+  // no more CTAs than the work can be dealt to: units by the tokens, tiles by the table's width
+  const long long upt = (cache->D == 128 ? Shape<128>::NCTA : Shape<64>::NCTA) * p.tpc;
+  const long long units = pool.Hkv * std::min(pool.B * ((c.longest + upt - 1) / upt), c.T / upt + pool.B);
+  const long long tiles = ((long long)cache->table_width * cache->page_size + BN - 1) / BN;
+  const long long cost = units * (UNIT_COST + std::max(1ll, tiles));
+  p.C = (int)std::max(1ll, std::min((long long)p.C, std::max(units, (cost + MIN_SHARE - 1) / MIN_SHARE)));
   p.scale_log2 = c.scale_log2;
   p.out = static_cast<uint8_t*>(c.out);
   p.o_sl = 2 * c.o_sl; p.o_sh = 2 * c.o_sh;

@@ -14,7 +14,7 @@ struct Call {
   void* out;
   float* lse;
   float* row_b;
-  int T, Hq, causal;
+  int T, Hq, longest, causal;         // longest: the most new tokens of a sequence
   long long q_sl, q_sh, o_sl, o_sh;  // element strides
   float scale_log2;
   int* status;

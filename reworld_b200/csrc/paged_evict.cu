@@ -99,6 +99,17 @@ __global__ void __launch_bounds__(THREADS, 1) select_kernel(const __grid_constan
   }
   const int lo = min(p.n_sink, kv), hi = kv - p.n_recent;   // rows [lo, hi) compete; lo <= hi since sink + recent <= keep < kv
   const unsigned need = (unsigned)(p.keep - p.n_sink - p.n_recent);
+  // a short row's sums are read once
+  const bool once = kv <= STEP;
+  float v[PER];
+  auto fetch = [&](int i0) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int i = i0 + j * THREADS + tid;
+      v[j] = i < kv ? x[i] : 0.f;
+    }
+  };
+  if (once) fetch(0);
   // ---- the need-th largest sum of [lo, hi): its bits from the top
   uint32_t prefix = 0;
   unsigned left = need;                      // of the rows with this prefix
@@ -108,19 +119,15 @@ __global__ void __launch_bounds__(THREADS, 1) select_kernel(const __grid_constan
       const int bits = pass < 2 ? 11 : 10, shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
       for (int i = tid; i < BINS; i += THREADS) hist[i] = 0;
       __syncthreads();
-      for (int i0 = lo; i0 < hi; i0 += STEP) {
-        float v[PER];
+      for (int i0 = 0; i0 < hi; i0 += STEP) {
+        if (!once) fetch(i0);
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
           const int i = i0 + j * THREADS + tid;
-          v[j] = i < hi ? x[i] : 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
           if (i0 + j * THREADS >= hi) break;
           const uint32_t o = order_of(v[j]);
-          if (i0 + j * THREADS + tid < hi && (pass == 0 || (o >> (shift + bits)) == prefix))
-            atomicAdd(&hist[(o >> shift) & (BINS - 1u) & ((1u << bits) - 1u)], 1u);
+          if (i >= lo && i < hi && (pass == 0 || (o >> (shift + bits)) == prefix))
+            atomicAdd(&hist[(o >> shift) & ((1u << bits) - 1u)], 1u);
         }
       }
       __syncthreads();
@@ -146,13 +153,8 @@ __global__ void __launch_bounds__(THREADS, 1) select_kernel(const __grid_constan
   // ---- number the kept rows: sink, recent, sums above the threshold, and the first `left` equal to it
   unsigned done_keep = 0, done_ties = 0;     // kept without the ties, ties seen, before this step
   for (int i0 = 0; i0 < kv; i0 += STEP) {
-    float v[PER];
     unsigned keep_m[PER], tie_m[PER];        // of the warp's 32 rows
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int i = i0 + j * THREADS + tid;
-      v[j] = i < kv ? x[i] : 0.f;
-    }
+    if (!once) fetch(i0);
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       const int i = i0 + j * THREADS + tid;

@@ -48,7 +48,7 @@ struct Params {
   float scale_log2;
   float* part;                  // [2 C][16 * D + 32]: O, then m, then l
   int* counters;                // [B * nrt * Hkv], zero before and after
-  int* header;                  // [2 C]: 1 + the unit of every part, 0: none (join_kernel joins); null: the last CTA joins
+  int2* header;                 // [B * nrt * Hkv]: first slot and parts of every unit (join_kernel joins); null: the last CTA joins
   // raw scores (log2 units) and (m, 1 / l) of every row, for the weight sums; null otherwise
   float* scores;                // [B * Hkv * nrt * 16][cap]
   float2* row_ml;               // [B * Hkv * nrt * 16]
@@ -173,7 +173,6 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
   }
   const long long N = base[THREADS];
   const int C = (int)max(1ll, min((long long)gridDim.x, N / p.min_tiles)), cta = blockIdx.x;
-  if (p.header && tid < 2) p.header[2 * cta + tid] = 0;
   if (cta >= C) return;
   const long long t0 = N * cta / C, t1 = N * (cta + 1) / C;
   if (t0 >= t1) return;
@@ -398,7 +397,16 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
     __syncthreads();
 
     const bool whole = k0 == 0 && k1 == n_tiles;
-    if (p.header && !whole && tid == 0) p.header[2 * cta + (t == t0 ? 0 : 1)] = 1 + e * p.pool.Hkv + hk;
+    // largest c with N c / C <= x: the CTA that has tile x
+    auto owner = [&](long long x) {
+      long long c = (x * C) / N;
+      while (c + 1 < C && N * (c + 1) / C <= x) ++c;
+      while (c > 0 && N * c / C > x) --c;
+      return (int)c;
+    };
+    if (p.header && k0 == 0 && tid == 0)
+      p.header[(long long)e * p.pool.Hkv + hk] =
+          make_int2(2 * cta + (t == t0 ? 0 : 1), whole ? 0 : owner(u1 - 1) - cta + 1);
     float* slot = p.part + (long long)(2 * cta + (t == t0 ? 0 : 1)) * SLOT;
     auto put = [&](int r, int c, float2 v, float mm, float ll) { put_row<HALF>(p, en, b, hk, r, c, v, mm, ll); };
     // 2 channels of a row a thread and step
@@ -436,12 +444,6 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
     }
     if (!whole && !p.header) {
       // the CTAs whose shares meet the unit: the one that holds tile u0 to the one that holds u1 - 1
-      auto owner = [&](long long x) {        // largest c with N c / C <= x
-        long long c = (x * C) / N;
-        while (c + 1 < C && N * (c + 1) / C <= x) ++c;
-        while (c > 0 && N * c / C > x) --c;
-        return (int)c;
-      };
       const int ca = owner(u0), cb = owner(u1 - 1);
       int* counter = p.counters + (long long)e * p.pool.Hkv + hk;
       __threadfence();
@@ -513,62 +515,55 @@ constexpr int JOIN_GROUPS = 8;
 // Parts a unit, above which this kernel joins: 2 units of 8 parts 18.4 us without and 20.5 with it, 24 units of 12
 // parts 38.9 and 34.8 (4000 rows), 4 units of 74 parts 86 and 74, 1 unit of 296 parts 86 and 51.
 constexpr int WIDE_JOIN = 10;
-constexpr int MAX_PARTS = 2048;
+constexpr int MAX_PARTS = 1024;  // CTAs of a launch: checked by the host
 
 template <bool HALF, int D>
-__global__ void __launch_bounds__(JOIN_GROUPS * D / 4) join_kernel(const __grid_constant__ Params p, int C) {
+__global__ void __launch_bounds__(JOIN_GROUPS * D / 4) join_kernel(const __grid_constant__ Params p) {
   constexpr int SLOT = RT * D + 2 * RT;
   constexpr int NT = JOIN_GROUPS * D / 4;
-  __shared__ int part[MAX_PARTS];
   __shared__ float fac[MAX_PARTS];
-  __shared__ int n_sh;
-  __shared__ float red[2];
+  __shared__ float red[2][NT / 32];
   __shared__ float4 acc[JOIN_GROUPS][D / 4];
   griddep_launch_dependents();
   griddep_wait();
-  const int u = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+  const int u = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int e = u / p.pool.Hkv, hk = u - e * p.pool.Hkv;
+  const int2 h = __ldcg(p.header + u);         // (not written, and not used, where the unit has no rows)
   const Entry en = load_entry(p, e, nullptr);
   if (r >= en.rows) return;
-  if (tid < 32) {
-    int n = 0;
-#pragma unroll 4
-    for (int o0 = 0; o0 < 2 * C; o0 += 32) {
-      const bool mine = o0 + lane < 2 * C && __ldcg(p.header + o0 + lane) == u + 1;
-      const unsigned m = __ballot_sync(0xffffffffu, mine);
-      if (mine) part[n + __popc(m & ((1u << lane) - 1u))] = o0 + lane;
-      n += __popc(m);
-    }
-    __syncwarp();
-    float mm = -INFINITY;
-    for (int i = lane; i < n; i += 32) {
-      fac[i] = __ldcg(p.part + (long long)part[i] * SLOT + RT * D + r);
-      mm = fmaxf(mm, fac[i]);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-    const float bs = mm == -INFINITY ? 0.f : mm;
-    float ll = 0.f;
-    for (int i = lane; i < n; i += 32) {
-      fac[i] = fast_exp2(fac[i] - bs);
-      ll += fac[i] * __ldcg(p.part + (long long)part[i] * SLOT + RT * D + RT + r);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
-    if (lane == 0) {
-      n_sh = n;
-      red[0] = mm;
-      red[1] = ll;
-    }
-  }
-  __syncthreads();
-  const int n = n_sh;
+  const int n = min(h.y, MAX_PARTS);
   if (n == 0) return;                          // one CTA did it all, and wrote it
+  // part 0 may be in its CTA's second slot, the others are in the first slots of the CTAs that follow
+  auto slot = [&](int i) { return p.part + (i == 0 ? (long long)h.x : 2LL * (h.x / 2 + i)) * SLOT; };
+  float mm = -INFINITY;
+  for (int i = tid; i < n; i += NT) {
+    fac[i] = __ldcg(slot(i) + RT * D + r);
+    mm = fmaxf(mm, fac[i]);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+  if (lane == 0) red[0][warp] = mm;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NT / 32; ++i) mm = fmaxf(mm, red[0][i]);
+  const float bs = mm == -INFINITY ? 0.f : mm;
+  float ll = 0.f;
+  for (int i = tid; i < n; i += NT) {
+    fac[i] = fast_exp2(fac[i] - bs);
+    ll += fac[i] * __ldcg(slot(i) + RT * D + RT + r);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
+  if (lane == 0) red[1][warp] = ll;
+  __syncthreads();
+  ll = 0.f;
+#pragma unroll
+  for (int i = 0; i < NT / 32; ++i) ll += red[1][i];
   const int g = tid / (D / 4), c = 4 * (tid % (D / 4));
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
+#pragma unroll 10
   for (int i = g; i < n; i += JOIN_GROUPS) {
-    const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part + (long long)part[i] * SLOT + r * D + c));
+    const float4 x = __ldcg(reinterpret_cast<const float4*>(slot(i) + r * D + c));
     const float f = fac[i];
     v.x += f * x.x;
     v.y += f * x.y;
@@ -587,8 +582,8 @@ __global__ void __launch_bounds__(JOIN_GROUPS * D / 4) join_kernel(const __grid_
     v.w += x.w;
   }
   const int b = e / p.nrt;
-  put_row<HALF>(p, en, b, hk, r, c, make_float2(v.x, v.y), red[0], red[1]);
-  put_row<HALF>(p, en, b, hk, r, c + 2, make_float2(v.z, v.w), red[0], red[1]);
+  put_row<HALF>(p, en, b, hk, r, c, make_float2(v.x, v.y), mm, ll);
+  put_row<HALF>(p, en, b, hk, r, c + 2, make_float2(v.z, v.w), mm, ll);
 }
 
 // sums[b, hk, j] += sum over the rows of exp2(score - m) / l, rows in their order.
@@ -647,7 +642,7 @@ inline Layout layout(int D, int C, int B, int Hkv, int nrt, long long cap, bool 
   Layout l;
   l.part = 0;
   l.header = (2LL * C * (RT * D + 2 * RT) * 4 + 255) & ~255LL;
-  l.ml = (l.header + 8LL * C + 255) & ~255LL;
+  l.ml = (l.header + 8LL * B * Hkv * nrt + 255) & ~255LL;
   const long long lines = (long long)B * Hkv * nrt * RT;
   l.scores = l.ml + (sums ? (lines * 8 + 255) & ~255LL : 0);
   l.total = l.scores + (sums ? lines * cap * 4 : 0);
@@ -663,7 +658,7 @@ int launch_rows(const Params& p, int C, cudaStream_t stream) {
     return RW_ERR_CUDA;
   if (!p.header) return RW_OK;
   const dim3 grid(p.pool.B * p.nrt * p.pool.Hkv, std::min(RT, p.T * p.G));
-  return launch_dependent(join_kernel<HALF, D>, grid, dim3(JOIN_GROUPS * D / 4), 0, stream, p, C) == cudaSuccess
+  return launch_dependent(join_kernel<HALF, D>, grid, dim3(JOIN_GROUPS * D / 4), 0, stream, p) == cudaSuccess
              ? RW_OK : RW_ERR_CUDA;
 }
 
@@ -697,7 +692,7 @@ extern "C" int rw_paged_attn(const rw_paged_t* cache, const void* q, void* out, 
     if (!workspace || !aligned16(workspace) || workspace_bytes < parts + (sums ? 4LL * T * Hq : 0))
       return RW_ERR_INVALID_ARG;
     float* rb = sums ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + parts) : nullptr;
-    const chunk::Call c{q, out, lse, rb, T, Hq, causal != 0, q_sl, q_sh, o_sl, o_sh, scale_log2, status};
+    const chunk::Call c{q, out, lse, rb, T, Hq, max_q_len < T ? max_q_len : T, causal != 0, q_sl, q_sh, o_sl, o_sh, scale_log2, status};
     const int rc = chunk::launch(cache, p.pool, c, workspace, st);
     return rc != RW_OK || !sums ? rc : weigh::launch(cache, p.pool, c, sums, sums_sb, sums_sh, st);
   }
@@ -705,7 +700,7 @@ extern "C" int rw_paged_attn(const rw_paged_t* cache, const void* q, void* out, 
   // would need a workspace for a chunk's scores)
   if (rows::on_tensor_tiles(cache->B, nrt) && sums) return RW_ERR_UNSUPPORTED;
   const int C = rows::grid_size(cache->D);
-  if (C == 0 || 2 * C > rows::MAX_PARTS) return RW_ERR_CUDA;
+  if (C == 0 || C > rows::MAX_PARTS) return RW_ERR_CUDA;
   const rows::Layout lay = rows::layout(cache->D, C, cache->B, p.pool.Hkv, (int)nrt, cap, sums != nullptr);
   if (!workspace || !aligned16(workspace) || workspace_bytes < lay.total || !counters ||
       n_counters < rows::counters_needed(cache->B, p.pool.Hkv, (int)nrt))
@@ -717,22 +712,25 @@ extern "C" int rw_paged_attn(const rw_paged_t* cache, const void* q, void* out, 
   p.q_sl = 2 * q_sl; p.q_sh = 2 * q_sh; p.o_sl = 2 * o_sl; p.o_sh = 2 * o_sh;
   p.T = T; p.Hq = Hq; p.G = G; p.nrt = (int)nrt; p.causal = causal != 0;
   p.min_tiles = 1;
+  // no more CTAs than there can be tiles: the others would only cost their launch
+  const long long most = nrt * cache->B * p.pool.Hkv * std::max(1ll, (cap + rows::TILE - 1) / rows::TILE);
+  const int ctas = (int)std::min((long long)C, most);
   p.scale_log2 = scale_log2;
   p.part = reinterpret_cast<float*>(ws + lay.part);
   p.counters = counters;
   // Where a unit can have many parts (CTAs a unit, tiles of a unit), they are joined by a kernel of their own; where
   // it has few, by the last CTA that comes to it, without another launch.
   if (std::min((long long)C / (cache->B * p.pool.Hkv * nrt), cap / rows::TILE) > rows::WIDE_JOIN)
-    p.header = reinterpret_cast<int*>(ws + lay.header);
+    p.header = reinterpret_cast<int2*>(ws + lay.header);
   p.scores = sums ? reinterpret_cast<float*>(ws + lay.scores) : nullptr;
   p.row_ml = sums ? reinterpret_cast<float2*>(ws + lay.ml) : nullptr;
   p.cap = cap;
   p.status = status;
   int rc;
   if (cache->dtype == RW_DTYPE_FP16)
-    rc = cache->D == 128 ? rows::launch_rows<true, 128>(p, C, st) : rows::launch_rows<true, 64>(p, C, st);
+    rc = cache->D == 128 ? rows::launch_rows<true, 128>(p, ctas, st) : rows::launch_rows<true, 64>(p, ctas, st);
   else
-    rc = cache->D == 128 ? rows::launch_rows<false, 128>(p, C, st) : rows::launch_rows<false, 64>(p, C, st);
+    rc = cache->D == 128 ? rows::launch_rows<false, 128>(p, ctas, st) : rows::launch_rows<false, 64>(p, ctas, st);
   if (rc != RW_OK || !sums || cap == 0) return rc;
   rows::SumParams sp{};
   sp.pool = p.pool;

@@ -346,6 +346,9 @@ int launch(const rw_paged_t* cache, const Pool& pool, const chunk::Call& c, floa
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return RW_ERR_CUDA;
+  const long long units = (long long)pool.B * pool.Hkv * (((long long)cache->table_width * cache->page_size + BM - 1) / BM);
+  if (units == 0) return RW_OK;
+  if (units < sms) sms = (int)units;
   Params p{};
   p.pool = pool;
   p.T = c.T; p.Hq = c.Hq; p.G = c.Hq / pool.Hkv; p.causal = c.causal;
