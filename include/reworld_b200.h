@@ -447,16 +447,15 @@ int rw_paged_rotary_store(const rw_paged_t* cache, const void* k, const void* v,
  * sums (may be NULL): fp32 [B, Hkv, >= table_width * page_size] with element strides
  * sums_sb, sums_sh; sums[b, g, j] += the weights that the rows of key head g's group
  * gave to cached row j.  The order of the additions is fixed.
- * counters: n_counters ints of device memory, zeroed once; every call leaves them
- * zero.  workspace: 16-byte aligned, rw_paged_attn_workspace_bytes(...) bytes,
- * which also tells the counters needed.  Calls that overlap on the GPU need
- * counters and workspaces of their own. */
+ * workspace: device memory, 16-byte aligned, rw_paged_attn_workspace_bytes(...)
+ * bytes, contents of no matter; calls that overlap on the GPU need workspaces of
+ * their own.  (cache_rows: table_width * page_size; with_sums: sums != NULL.) */
 int rw_paged_attn(const rw_paged_t* cache, const void* q, void* out, float* lse, int T, int Hq, int max_q_len,
                   long long q_sl, long long q_sh, long long o_sl, long long o_sh, int causal, float softmax_scale,
-                  float* sums, long long sums_sb, long long sums_sh, int* counters, long long n_counters,
-                  void* workspace, long long workspace_bytes, int* status, void* stream);
+                  float* sums, long long sums_sb, long long sums_sh, void* workspace, long long workspace_bytes,
+                  int* status, void* stream);
 long long rw_paged_attn_workspace_bytes(int T, int Hq, int Hkv, int D, int B, int max_q_len, long long cache_rows,
-                                        int with_sums, long long* n_counters);
+                                        int with_sums);
 
 /* Eviction by accumulated attention weight.  Of the kv rows of every sequence and
  * key head, the first n_sink and the last n_recent are kept and, of the others,

@@ -92,8 +92,8 @@ _SIGNATURES = {
     "rw_paged_rotary_store": (c_int, [ctypes.POINTER(RwPaged)] + [c_vp] * 4 + [c_int] * 2 + [c_ll] * 8 + [c_vp]
                               + [c_int] * 3 + [c_vp] * 3),
     "rw_paged_attn": (c_int, [ctypes.POINTER(RwPaged)] + [c_vp] * 3 + [c_int] * 3 + [c_ll] * 4 + [c_int, c_float, c_vp]
-                      + [c_ll] * 2 + [c_vp, c_ll, c_vp, c_ll, c_vp, c_vp]),
-    "rw_paged_attn_workspace_bytes": (c_ll, [c_int] * 6 + [c_ll, c_int, ctypes.POINTER(c_ll)]),
+                      + [c_ll] * 2 + [c_vp, c_ll, c_vp, c_vp]),
+    "rw_paged_attn_workspace_bytes": (c_ll, [c_int] * 6 + [c_ll, c_int]),
     "rw_paged_evict": (c_int, [ctypes.POINTER(RwPaged), c_vp, c_ll, c_ll, c_vp, c_ll, c_vp, c_vp] + [c_int] * 3
                        + [c_vp, c_ll, c_int, c_vp, c_vp]),
     "rw_error_string": (ctypes.c_char_p, [c_int]),

@@ -5,7 +5,7 @@
 // file holds no computation: it checks the arguments, allocates what is returned, keeps the
 // workspaces and calls the C entry points of include/reworld_b200.h on the current stream.
 //
-// Workspaces and counters are kept for each stream, since calls on different streams may
+// Workspaces are kept for each stream, since calls on different streams may
 // overlap; a call that is captured into a graph gets its own, of the graph's memory, so
 // graphs share nothing.  The interpreter lock is held throughout, so that two host threads
 // that use one stream cannot put their launches between each other's.
@@ -187,20 +187,14 @@ int* status_word(int device) {
   return word[device];
 }
 
-struct Scratch {
-  Tensor bytes, counters;
-};
-
-Scratch scratch_for(const Tensor& like, cudaStream_t stream, int64_t bytes, int64_t counters) {
-  const auto opt = like.options().requires_grad(false);
+Tensor scratch_for(const Tensor& like, cudaStream_t stream, int64_t bytes) {
+  const auto opt = like.options().requires_grad(false).dtype(at::kByte);
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
-    return {at::empty({bytes}, opt.dtype(at::kByte)), at::zeros({counters}, opt.dtype(at::kInt))};
+    return at::empty({bytes}, opt);
   // never destroyed: at exit the device may be gone before it
-  static auto* kept = new std::map<std::pair<int, cudaStream_t>, Scratch>();
-  Scratch& s = (*kept)[{like.device().index(), stream}];
-  if (!s.bytes.defined() || s.bytes.numel() < bytes) s.bytes = at::empty({bytes}, opt.dtype(at::kByte));
-  if (!s.counters.defined() || s.counters.numel() < counters)
-    s.counters = at::zeros({std::max<int64_t>(counters, 1 << 14)}, opt.dtype(at::kInt));
+  static auto* kept = new std::map<std::pair<int, cudaStream_t>, Tensor>();
+  Tensor& s = (*kept)[{like.device().index(), stream}];
+  if (!s.defined() || s.numel() < bytes) s = at::empty({bytes}, opt);
   return s;
 }
 
@@ -316,13 +310,11 @@ py::object attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pag
     const int dev = k_pages.device().index();
     cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev).stream();
     const int t = count(T, "tokens"), h = count(Hq, "heads");
-    long long counters = 0;
-    const long long need = rw_paged_attn_workspace_bytes(t, h, c.Hkv, c.D, c.B, (int)longest, rows, w.ptr != nullptr,
-                                                         &counters);
-    const Scratch s = scratch_for(k_pages, stream, need, counters);
+    const long long need = rw_paged_attn_workspace_bytes(t, h, c.Hkv, c.D, c.B, (int)longest, rows, w.ptr != nullptr);
+    const Tensor ws = scratch_for(k_pages, stream, need);
     check_code(rw_paged_attn(&c, hq.ptr, ho.ptr, return_lse ? lse.data_ptr<float>() : nullptr, t, h, (int)longest,
-                             hq.sl, hq.sh, ho.sl, ho.sh, causal, (float)scale, w.ptr, w.sb, w.sh,
-                             s.counters.data_ptr<int>(), counters, s.bytes.data_ptr(), need, status_word(dev), stream),
+                             hq.sl, hq.sh, ho.sl, ho.sh, causal, (float)scale, w.ptr, w.sb, w.sh, ws.data_ptr(),
+                             need, status_word(dev), stream),
                "rw_paged_attn");
   }
   if (return_lse) return py::make_tuple(y, lse);

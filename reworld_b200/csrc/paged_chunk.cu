@@ -1107,7 +1107,7 @@ int value_map(CUtensorMap* m, const rw_paged_t* c, int rows) {
 
 bool supported(const rw_paged_t* c) {
   // coordinates are 32-bit, and a row's stride of 16 has to fit a map's
-  return c->B <= MAX_BATCH && key_lines(c).lines < (1ll << 31) && c->k_sl < (1ll << 35);
+  return key_lines(c).lines < (1ll << 31) && c->k_sl < (1ll << 35);
 }
 
 int grid_size(int D) {

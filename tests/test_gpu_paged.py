@@ -157,6 +157,10 @@ def test_chunks_pages_and_layouts(cuda, page, layout):
     _run(cuda, [150, 31], [333, 500], 4, 2, 128, BF, page=page, layout=layout)
 
 
+def test_chunks_of_many_sequences(cuda):
+    _run(cuda, [(i % 3) + 3 for i in range(1100)], [(13 * i) % 90 + 5 for i in range(1100)], 4, 1, 64, BF, max_q=5)
+
+
 def test_chunk_rows_that_see_nothing(cuda):
     """More new tokens than rows: the first ones see none; sequences without rows or tokens."""
     _run(cuda, [40, 10, 0, 200], [25, 0, 100, 60], 4, 2, 128, BF)

@@ -31,8 +31,7 @@ BAD_POOLS = [
 def test_every_entry_point_refuses_a_bad_cache(bad, code):
     lib, pg = _native.lib(), _pg(**bad)
     assert lib.rw_paged_rotary_store(pg, p, p, None, None, 4, 0, *([128] * 8), None, 0, 0, 0, None, None, None) == code
-    assert lib.rw_paged_attn(pg, p, p, None, 4, 4, 1, *([128] * 4), 1, 0.1, None, 0, 0, p, 1 << 20, p, 1 << 40, None,
-                             None) == code
+    assert lib.rw_paged_attn(pg, p, p, None, 4, 4, 1, *([128] * 4), 1, 0.1, None, 0, 0, p, 1 << 40, None, None) == code
     assert lib.rw_paged_evict(pg, p, 64, 32, p, 64, p, p, 16, 0, 0, p, 1, 1, None, None) == code
 
 
@@ -75,8 +74,8 @@ def test_attention_refusals():
     s4 = [512, 128] * 2
     big = 1 << 40
 
-    def call(pg=None, q=p, out=p, T=4, Hq=4, mq=1, st=s4, scale=0.1, cnt=p, nc=1 << 20, ws=p, wb=big, sums=None, ss=(0, 0)):
-        return fn(pg or _pg(), q, out, None, T, Hq, mq, *st, 1, scale, sums, *ss, cnt, nc, ws, wb, None, None)
+    def call(pg=None, q=p, out=p, T=4, Hq=4, mq=1, st=s4, scale=0.1, ws=p, wb=big, sums=None, ss=(0, 0)):
+        return fn(pg or _pg(), q, out, None, T, Hq, mq, *st, 1, scale, sums, *ss, ws, wb, None, None)
 
     assert call(T=0) == 0 and call(mq=0) == 0 and call(pg=_pg(B=0)) == 0
     assert call(q=None) == -1 and call(out=ctypes.c_void_p(8)) == -1
@@ -106,11 +105,10 @@ def test_evict_refusals():
 
 def test_workspace_of_odd_questions():
     fn = _native.lib().rw_paged_attn_workspace_bytes
-    n = ctypes.c_longlong(-1)
     for args in ((0, 8, 2, 128, 1, 1, 64, 0), (1, 8, 3, 128, 1, 1, 64, 0), (1, 8, 2, 96, 1, 1, 64, 0),
                  (1, 8, 2, 128, 0, 1, 64, 0), (1, 8, 2, 128, 1, 0, 64, 0), (1, 8, 2, 128, 1, 1, -1, 0)):
-        assert fn(*args, n) == 0 and n.value == 0
-    assert fn(1, 8, 2, 128, 1, 1, 64, 0, None) >= 0
+        assert fn(*args) == 0
+    assert fn(1, 8, 2, 128, 1, 1, 64, 0) >= 0
 
 
 def test_python_calls_reject_cpu_tensors():
