@@ -30,6 +30,12 @@ struct Pool {
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }
 
+// a / b of counts: in 32 bits where they fit (a 64-bit division is a subroutine of some 100 dependent
+// instructions, which a plan made by one warp shows).
+__device__ __forceinline__ long long div_count(long long a, long long b) {
+  return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+}
+
 // Tokens [s0, s0 + lq) and cached rows of a sequence, within the call's T tokens and
 // the table's width.
 struct Seq {

@@ -244,7 +244,7 @@ __device__ __forceinline__ Walk walk_to_unit(const Params& p, const Plan& pl, in
 }
 // Whole warp: cost of the units before that one.
 __device__ __forceinline__ long long cost_before(const Params& p, const Plan& pl, const Walk& w, int upt, int lane) {
-  long long sum = 0, all = (pl.cost[w.b + 1] - pl.cost[w.b]) / p.pool.Hkv;
+  long long sum = 0, all = paged::div_count(pl.cost[w.b + 1] - pl.cost[w.b], p.pool.Hkv);
   int keys;
   for (int rt = lane; rt < w.rt; rt += 32) sum += UNIT_COST + tiles_of(p, w.s, rt, upt, &keys);
 #pragma unroll
@@ -262,8 +262,8 @@ __device__ __forceinline__ Walk walk_to_cost(const Params& p, const Plan& pl, lo
   }
   w.b = lo;
   enter(p, w, upt);
-  const long long each = (pl.cost[lo + 1] - pl.cost[lo]) / p.pool.Hkv;
-  w.hk = (int)((t - pl.cost[lo]) / each);
+  const long long each = paged::div_count(pl.cost[lo + 1] - pl.cost[lo], p.pool.Hkv);
+  w.hk = (int)paged::div_count(t - pl.cost[lo], each);
   long long at = pl.cost[lo] + each * w.hk;
   for (int r0 = 0; r0 < w.nu; r0 += 32) {
     int keys;
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   __syncthreads();
 
   // ---- the planner's state (warp 11): its waves, then its share of the rest
-  long long t = 0, t1 = 0, before = 0, t_base = 0, t_rest = 1;
+  long long t = 0, t1 = 0, before = 0, t_base = 0, share = 1;  // pair c has [t_base + c share, t_base + (c + 1) share)
   int waves = 0, wave = 0, C = p.C;
   Walk wk{};
   bool in_tail = false;
@@ -407,10 +407,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         t = e;
         if (even && lane == 0 && s.n > 0 && s.slot == 2 * pid + 1) {
           // the last pair whose share meets the unit
-          const long long x = before + UNIT_COST + wk.n - 1 - t_base;
-          int c = (int)(x * C / t_rest);
-          while (c + 1 < C && t_rest * (c + 1) / C <= x) ++c;
-          while (c > 0 && t_rest * c / C > x) --c;
+          const int c = (int)paged::div_count(before + UNIT_COST + wk.n - 1 - t_base, share);
           p.header[pid] = make_int4(wk.b, wk.hk, wk.rt * upt, c - pid + 1);
         }
       }
@@ -435,7 +432,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const long long N = pl.cost[p.pool.B];       // of all work
     const int U = pl.units[p.pool.B];
     if (even && lane == 0) p.header[pid] = make_int4(0, 0, 0, 0);
-    if (N < (long long)C * MIN_SHARE) C = (int)min((long long)C, max((long long)U, (N + MIN_SHARE - 1) / MIN_SHARE));
+    if (N < (long long)C * MIN_SHARE)
+      C = (int)min((long long)C, max((long long)U, paged::div_count(N + MIN_SHARE - 1, MIN_SHARE)));
     if (pid < C) {
       // about equal: no unit is over 1/8 longer than their mean
       if ((long long)pl.longest * U * 8 <= N * 9) waves = U / C;
@@ -445,9 +443,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       } else if (waves > 0) {
         t_base = N;
       }
-      t_rest = N - t_base;
-      t = t_base + t_rest * pid / C;
-      t1 = t_base + t_rest * (pid + 1) / C;
+      share = max(1ll, paged::div_count(N - t_base + C - 1, C));
+      t = min(N, t_base + share * pid);
+      t1 = min(N, t + share);
     }
     plan_next(0);
   }
@@ -725,28 +723,32 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const uint32_t tO = tmem + lane_base;
     const float sl2 = p.scale_log2;
     const uint32_t p_ready0 = even_addr(&sb.p_ready[0]);
-    const int rtok = r / p.G, rg = r - rtok * p.G;   // the row's token (of the CTA's) and head (of the group's)
     int J0 = 0;
     for (int si = 0;; ++si) {
-      const Seg sg = seg_sh[si & 1];
-      if (sg.n == 0) break;
+      // Only what the tiles' loop needs is held through it; the rest is read, or worked out, again behind it (held
+      // in registers it was spilled, inside the loop).
+      const Seg& sg = seg_sh[si & 1];
+      const int n = sg.n, kv0 = sg.kv0;
+      if (n == 0) break;
       const uint32_t sph = (uint32_t)si & 1u;
-      const int tok = sg.tok0 + (int)rank * p.tpc + rtok;  // within the sequence
-      const bool there = r < used && tok < sg.lq;
-      // keys of the row; a row without a token takes them all (its values go nowhere)
-      const int lim = there ? (p.causal ? max(0, sg.kv - sg.lq + tok + 1) : sg.kv) : sg.kv;
-      // keys that every row of the CTA sees
-      const int all = p.causal ? max(0, min(sg.kv, sg.kv - sg.lq + sg.tok0 + (int)rank * p.tpc + 1)) : sg.kv;
+      int lim, all;
+      {
+        const int rtok = r / p.G, tok = sg.tok0 + (int)rank * p.tpc + rtok;
+        // keys of the row; a row without a token takes them all (its values go nowhere)
+        lim = p.causal && r < used && tok < sg.lq ? max(0, sg.kv - sg.lq + tok + 1) : sg.kv;
+        // keys that every row of the CTA sees
+        all = p.causal ? max(0, min(sg.kv, sg.kv - sg.lq + sg.tok0 + (int)rank * p.tpc + 1)) : sg.kv;
+      }
       bool ok = !aborted();
       float m_base = -INFINITY;
       uint64_t l2 = 0ull;
-      for (int j = w; j < sg.n && ok; j += NWG) {
+      for (int j = w; j < n && ok; j += NWG) {
         const int J = J0 + j;
         const int b = J % NSBUF;
         const uint32_t tS = tmem + lane_base + 128u + 128u * b;
         if (!(ok = pwait_warp(&sb.s_full[b], (uint32_t)(J / NSBUF) & 1u, cx, RW_STATUS_TIMEOUT_SOFTMAX))) break;
         tc_fence_after();
-        const int key0 = (sg.kv0 + j) * BN;
+        const int key0 = (kv0 + j) * BN;
         const bool masked = key0 + BN > all;
         const int cut = lim - key0;              // columns from here on are not seen
         auto load_half = [&](int h, uint32_t (&v)[2][32], const bool mask) {
@@ -909,6 +911,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       if (ok) ok = pwait_warp(&sb.o_done, sph, cx, RW_STATUS_TIMEOUT_SOFTMAX);
       tc_fence_after();
       constexpr int CW = D / NWG;                  // channels of a warpgroup
+      int r_again = r;
+      asm volatile("" : "+r"(r_again));
+      const int rtok = r_again / p.G, rg = r_again - rtok * p.G;  // the row's token (of the CTA's) and head (of the group's)
+      const int tok = sg.tok0 + (int)rank * p.tpc + rtok;         // within the sequence
+      const bool there = r < used && tok < sg.lq;
       if (ok && sg.slot >= 0) {
         float* base = p.scratch + (long long)sg.slot * Shape<D>::SLOT_FLOATS;
         constexpr int R = NCTA * BM;
@@ -970,7 +977,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
         fence_proxy_async_smem();                  // read before the next segment's loads go there
       }
-      J0 += sg.n;
+      J0 += n;
       boundary();
     }
   }

@@ -6,7 +6,7 @@
 // products an element at most.  What decides is that all SMs read all the time, however
 // ragged the lengths are.  So the work is one sequence of key tiles (64 keys of one
 // sequence and key head), in the order (sequence, head, tile), and CTA c of C
-// takes the share [c N / C, (c + 1) N / C) of its N tiles; lengths are read on the
+// takes the c-th share of ceil(N / C) of its N tiles; lengths are read on the
 // device, nothing is planned on the host.  A share covers the end of one unit (the
 // tiles of one sequence and head), whole units, and the beginning of another.
 // Units that lie in one share are written out directly; the others leave their
@@ -176,7 +176,9 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
   const long long N = base[THREADS];
   const int C = (int)max(1ll, min((long long)gridDim.x, N)), cta = blockIdx.x;  // (no share without a tile)
   if (cta >= C) return;
-  const long long t1 = N * (cta + 1) / C;
+  const long long share = paged::div_count(N + C - 1, C);
+  if (share * cta >= N) return;  // (the last CTAs may find nothing left)
+  const long long t1 = min(N, share * (cta + 1));
   // The segments of the share, one ahead, by thread 0: seg[i & 1] is segment i (n == 0: there is none).
   auto advance = [&](int i) {
     Seg s;
@@ -189,7 +191,7 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
       s.en = plan.en;
       s.n_tiles = tiles_of(s.en);
       s.b = plan.e;
-      s.hk = (int)((plan.t - plan.ebase) / s.n_tiles);
+      s.hk = (int)paged::div_count(plan.t - plan.ebase, s.n_tiles);
       s.u0 = plan.ebase + (long long)s.hk * s.n_tiles;
       s.k0 = (int)(plan.t - s.u0);
       s.n = (int)(min(t1, s.u0 + s.n_tiles) - plan.t);
@@ -200,7 +202,7 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
     seg[i & 1] = s;
   };
   if (tid == 0) {
-    const long long t0 = N * cta / C;
+    const long long t0 = share * cta;
     int lo = 0, hi = THREADS - 1;
     while (lo < hi) {   // last thread whose run of entries begins at or before t0
       const int mid = (lo + hi + 1) >> 1;
@@ -419,11 +421,9 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
     if (k0 == 0 && tid == 0) {
       int parts = 0;
       if (!whole) {
-        const long long x = sg.u0 + sg.n_tiles - 1;  // the CTA that has the unit's last tile
-        long long c = (x * C) / N;
-        while (c + 1 < C && N * (c + 1) / C <= x) ++c;
-        while (c > 0 && N * c / C > x) --c;
-        parts = (int)c - cta + 1;
+        // up to the CTA that has the unit's last tile
+        const int c = (int)paged::div_count(sg.u0 + sg.n_tiles - 1, share);
+        parts = c - cta + 1;
       }
       p.header[(long long)b * p.pool.Hkv + hk] = make_int2(my_slot, parts);
     }
