@@ -11,8 +11,9 @@
 // work item is two 16-byte chunks of one head that hold 8 whole pairs (chunks i and
 // i + rot / 16, or 2i and 2i + 1), so both layouts need the same 64 bytes of table,
 // and 128 / (D / 16) heads are under way in a CTA at once; a thread keeps its place in
-// the head, so the table is read once a token.  Tokens are dealt to CTAs in runs, so
-// that the sequence of a token is searched for only when a run leaves it.
+// the head, so the table is read once a token.
+#include <algorithm>
+
 #include "paged.cuh"
 
 namespace rw {
@@ -174,8 +175,11 @@ inline int launch(Params& p, int dtype, void* stream) {
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return RW_ERR_CUDA;
-  const int most = sms * 12;             // resident CTAs of this size
-  p.run = p.T <= most ? 1 : (p.T + most - 1) / most;
+  // A token a CTA: the SMs' scheduler covers one token's chain of loads (sequence, page, table) with others.  Where
+  // there are many tokens, three, so that they share the search for the sequence: 4 x 2640 tokens of 24 + 48 heads
+  // 65.9 us with 1, 65.3 with 2, 65.6 with 3, 70.0 with 4 (72 with one wave of CTAs), of 24 + 8 heads 37.2, 34.6,
+  // 32.9, 35.9; 4 x 700 tokens of 24 + 48 heads 20.5, 23.1, 21.6, 25.7.
+  p.run = std::min(3, std::max(1, p.T / (sms * 16)));
   const int grid = (p.T + p.run - 1) / p.run;
   auto kernel = dtype == RW_DTYPE_FP16 ? rotary_kernel<true> : rotary_kernel<false>;
   return launch_dependent(kernel, dim3(grid), dim3(THREADS), 0, static_cast<cudaStream_t>(stream), p) == cudaSuccess
