@@ -460,6 +460,9 @@ def _evict_case(cuda, lens, page, hkv, D, keep, sink, recent, dtype=BF, sums=Non
     ([100], 16, 2, 64, 1, 1, 0),
     ([100, 77], 32, 2, 64, 50, 0, 50),
     ([8192, 8193, 4096], 256, 2, 64, 4095, 3, 5),
+    ([40000, 20000, 33, 0], 64, 1, 64, 9000, 16, 100),   # several CTAs a unit
+    ([70000], 256, 2, 64, 65000, 0, 0),
+    ([17000], 128, 1, 64, 500, 0, 500),
 ])
 @pytest.mark.parametrize("layout", ["rows", "heads"])
 def test_evict(cuda, lens, page, hkv, D, keep, sink, recent, layout):
@@ -483,6 +486,7 @@ def test_evict_ties_and_special_sums(cuda, kind):
         x[..., 2::7] = float("nan")
         return x
     _evict_case(cuda, [5000, 700], 16, 2, 64, 600, 2, 10, sums=sums)
+    _evict_case(cuda, [30000], 64, 2, 64, 8000, 2, 10, sums=lambda cap, g: sums(cap, g)[:1])
 
 
 # ------------------------------------------------------------------ together
