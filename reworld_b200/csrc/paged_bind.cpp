@@ -189,7 +189,8 @@ int* status_word(int device) {
 
 Tensor scratch_for(const Tensor& like, cudaStream_t stream, int64_t bytes) {
   const auto opt = like.options().requires_grad(false).dtype(at::kByte);
-  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
+  // (a large one is not worth keeping: its allocation is nothing beside the call)
+  if (bytes > (64 << 20) || c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
     return at::empty({bytes}, opt);
   // never destroyed: at exit the device may be gone before it
   static auto* kept = new std::map<std::pair<int, cudaStream_t>, Tensor>();

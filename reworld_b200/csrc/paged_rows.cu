@@ -49,8 +49,8 @@ struct Params {
   float* part;                  // [2 C][16 * D + 32]: O, then m, then l
   int2* header;                 // [B * Hkv]: first slot and parts of every unit (0: written whole)
   // raw scores (log2 units) and (m, 1 / l) of every row, for the weight sums; null otherwise
-  float* scores;                // [B * Hkv * 16][cap]
-  float2* row_ml;               // [B * Hkv * 16]
+  float* scores;                // [B * Hkv * rows_most][cap]
+  float2* row_ml;               // [B * Hkv * rows_most]
   float* sums;
   long long sums_sb, sums_sh;
   long long cap;
@@ -89,14 +89,14 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
 // A sequence, its rows of a key head, and what the last of them sees.
 struct Entry {
   Seq s;
-  int rows;   // 0..16 (a sequence with more is one with more than max_q_len tokens)
+  int rows;   // 0..rows_most (a sequence with more is one with more than max_q_len tokens)
   int keys;   // keys that any of the rows sees
 };
 
 __device__ __forceinline__ Entry load_entry(const Params& p, int b, int* status) {
   Entry n;
   n.s = paged::load_seq(p.pool, b, p.T, status);
-  n.rows = (int)min((long long)RT, (long long)n.s.lq * p.G);
+  n.rows = (int)min((long long)p.rows_most, (long long)n.s.lq * p.G);
   n.keys = 0;
   if (n.rows > 0) n.keys = p.causal ? max(0, n.s.kv - n.s.lq + (n.rows - 1) / p.G + 1) : n.s.kv;
   return n;
@@ -127,7 +127,7 @@ __device__ __forceinline__ void put_row(const Params& p, const Entry& en, int b,
       p.lse[(long long)(en.s.s0 + tok) * p.Hq + hk * p.G + g] =
           ll != 0.f ? (mm + log2f(ll)) * 0.6931471805599453f : -INFINITY;
     if (p.row_ml) {
-      const long long line = ((long long)b * p.pool.Hkv + hk) * RT + r;
+      const long long line = ((long long)b * p.pool.Hkv + hk) * p.rows_most + r;
       p.row_ml[line] = make_float2(mm == -INFINITY ? 0.f : mm, inv);
     }
   }
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const int r = grp + 8 * x;
-            const long long line = ((long long)b * p.pool.Hkv + hk) * RT + r;
+            const long long line = ((long long)b * p.pool.Hkv + hk) * p.rows_most + r;
             if (r < en.rows && key0 + 8 * i < p.cap)
               *reinterpret_cast<float2*>(p.scores + line * p.cap + key0 + 8 * i) =
                   make_float2(sc[i][2 * x], sc[i][2 * x + 1]);
@@ -574,7 +574,7 @@ __global__ void __launch_bounds__(JOIN_GROUPS * D / 4) join_sums_kernel(const __
   for (int r = tid >> 5; r < rows; r += NT / 32) {
     float2 x;
     if (h.y == 0) {
-      x = __ldcg(p.row_ml + unit * RT + r);
+      x = __ldcg(p.row_ml + unit * p.rows_most + r);
     } else {
       float mm = -INFINITY, ll = 0.f;
       const float* at = p.part + RT * D + r;
@@ -592,7 +592,7 @@ __global__ void __launch_bounds__(JOIN_GROUPS * D / 4) join_sums_kernel(const __
   }
   __syncthreads();
   float* dst = p.sums + b * p.sums_sb + hk * p.sums_sh;
-  const float* sc = p.scores + unit * RT * p.cap;
+  const float* sc = p.scores + unit * p.rows_most * p.cap;
   // 4 keys a thread (a key tile's scores are there to its end): one wave of blocks
   for (int j = 4 * (blockIdx.x * NT + tid); j < en.keys; j += 4 * gridDim.x * NT) {
     float4 add = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -638,12 +638,12 @@ struct Layout {
   long long part, header, ml, scores, total;  // byte offsets
 };
 
-inline Layout layout(int D, int C, int B, int Hkv, long long cap, bool sums) {
+inline Layout layout(int D, int C, int B, int Hkv, long long rows, long long cap, bool sums) {
   Layout l;
   l.part = 0;
   l.header = (2LL * C * (RT * D + 2 * RT) * 4 + 255) & ~255LL;
   l.ml = (l.header + 8LL * B * Hkv + 255) & ~255LL;
-  const long long lines = (long long)B * Hkv * RT;
+  const long long lines = (long long)B * Hkv * rows;
   l.scores = l.ml + (sums ? (lines * 8 + 255) & ~255LL : 0);
   l.total = l.scores + (sums ? lines * cap * 4 : 0);
   return l;
@@ -668,7 +668,7 @@ int run_rows(const rw_paged_t* cache, const Pool& pool, const chunk::Call& c, lo
   const int C = grid_size(cache->D);
   if (C == 0 || C > MAX_PARTS) return RW_ERR_CUDA;
   if (cap == 0) sums = nullptr;
-  const Layout lay = layout(cache->D, C, cache->B, pool.Hkv, cap, sums != nullptr);
+  const Layout lay = layout(cache->D, C, cache->B, pool.Hkv, rows, cap, sums != nullptr);
   if (!workspace || !aligned16(workspace) || workspace_bytes < lay.total) return RW_ERR_INVALID_ARG;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   Params p{};
@@ -750,7 +750,7 @@ extern "C" long long rw_paged_attn_workspace_bytes(int T, int Hq, int Hkv, int D
   using namespace rw;
   if (T < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || B < 1 || max_q_len < 1 || (D != 64 && D != 128) || cache_rows < 0)
     return 0;
-  if (rows::few_rows((long long)std::min(max_q_len, T) * (Hq / Hkv)))
-    return rows::layout(D, rows::grid_size(D), B, Hkv, cache_rows, with_sums != 0).total;
+  const long long rows = (long long)std::min(max_q_len, T) * (Hq / Hkv);
+  if (rows::few_rows(rows)) return rows::layout(D, rows::grid_size(D), B, Hkv, rows, cache_rows, with_sums != 0).total;
   return chunk::workspace_bytes(D) + (with_sums ? 4LL * T * Hq : 0);
 }
