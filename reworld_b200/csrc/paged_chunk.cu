@@ -598,9 +598,28 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           }
           __syncwarp();
         }
-        int b = J0 % NSBUF, st = J0 % NSTAGE;
-        for (int j = 0; j < sg.n && ok; ++j) {
-          const int J = J0 + j;
+        int b = J0 % NSBUF, st = J0 % NSTAGE, J = J0, j = 0;
+        // The tiles that have a QK to issue behind them and whose values nobody looks through: this thread has about
+        // 1000 clocks a tile, and waits and commits take 100 each, so their loop asks nothing else (with the questions
+        // of the last tiles in it, 2640 tokens over 34320 rows took 5 % longer).
+        const int plain = min(sg.n - NSBUF, sg.all / BN - sg.kv0);
+        uint32_t pb = (uint32_t)(J0 / NSBUF) & 1u, ps = (uint32_t)(J0 / NSTAGE) & 1u;
+        for (; j < plain && ok; ++j, ++J) {
+          if (!(ok = pwait_warp(&sb.p_ready[b], pb, cx, RW_STATUS_TIMEOUT_MMA))) break;
+          if (!(ok = pwait_warp(&sb.stage_full[st], ps, cx, RW_STATUS_TIMEOUT_MMA))) break;
+          tc_fence_after();
+          if (elect_one()) {
+            issue_pv(tmem, tmem + 128u + 128u * b, dv_st + st * STAGE_DESC, j > 0);
+            issue_qk(tmem + 128u + 128u * b, dq, dk_st + st * STAGE_DESC);
+            commit_n<NCTA>(&sb.s_full[b]);
+            commit_n<NCTA>(&sb.stage_free[st]);
+          }
+          __syncwarp();
+          if (++b == NSBUF) { b = 0; pb ^= 1u; }
+          if (++st == NSTAGE) { st = 0; ps ^= 1u; }
+        }
+#pragma unroll 1
+        for (; j < sg.n && ok; ++j, ++J) {
           if (!(ok = pwait_warp(&sb.p_ready[b], (uint32_t)(J / NSBUF) & 1u, cx, RW_STATUS_TIMEOUT_MMA))) break;
           if (!(ok = pwait_warp(&sb.stage_full[st], (uint32_t)(J / NSTAGE) & 1u, cx, RW_STATUS_TIMEOUT_MMA))) break;
           if (checked(sg, sg.kv0 + j)) {
