@@ -57,9 +57,10 @@ constexpr int REG_SOFTMAX = 208, REG_OTHER = 88;
 static_assert(NWG * 128 * REG_SOFTMAX + 128 * REG_OTHER <= NUM_THREADS * 168, "register split exceeds the launch's");
 constexpr float RESCALE_THRESHOLD = 8.0f;    // log2 units
 constexpr int MIN_SHARE = 12;                // cost of a share, where there is little work
-// What a unit costs beside its key tiles, in tiles: filling and draining the pipeline (q and
-// the first keys, the last softmax, the output) takes 5 to 8 us, a tile 0.75 to 0.9.
-constexpr int UNIT_COST = 7;
+// What a unit costs beside its key tiles, in tiles: filling and draining the pipeline (q and the first keys, the last
+// softmax, the output) takes 5 to 8 us, a tile 0.75 to 0.9.  4 ragged chunks of up to 701 tokens 140.5 us dealt out with
+// 3, 131.8 with 7, 131.7 with 11; 16 of up to 300 tokens 233, 198 and 196; 3 prompts of head dim 64 53.1, 51.2 and 50.5.
+constexpr int UNIT_COST = 10;
 
 template <int D>
 struct Shape {
