@@ -57,8 +57,9 @@ def _compile_bind(obj):
     _run(cmd)
     return [CXX, "-shared", "-o", bind_path() + ".tmp", obj, "-L" + lib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
            "-L" + OUT_DIR, "-lreworld_b200",
-           # (the CUDA runtime that torch loads)
-           "-Wl,--copy-dt-needed-entries", "-Wl,-rpath," + lib, "-Wl,-rpath,$ORIGIN"]
+           # the C++ and CUDA runtimes that torch loads: a second, static C++ runtime (a compiler that comes with
+           # libstdc++.a alone takes that) is mixed with torch's, and the first formatted message ends the process
+           "-l:libstdc++.so.6", "-Wl,--copy-dt-needed-entries", "-Wl,-rpath," + lib, "-Wl,-rpath,$ORIGIN"]
 
 
 def _run(cmd):

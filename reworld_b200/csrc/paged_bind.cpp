@@ -122,7 +122,7 @@ Table table_of(const Tensor& t, const char* name, const Tensor& like) {
 
 rw_paged_t cache_of(const Tensor& k, const Tensor& v, const Tensor& block_table, const Tensor& kv_lens,
                     const Tensor* q_starts) {
-  CHECK_VALUE(k.is_cuda(), "a paged cache lives on a CUDA device");
+  CHECK_VALUE(k.is_cuda(), "a paged cache lives on a CUDA device, not on ", k.device());
   const int code = dtype_code(k.scalar_type());
   CHECK_VALUE(code >= 0, "a paged cache is bf16 or fp16");
   CHECK_VALUE(k.dim() == 4 && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() && v.device() == k.device(),
@@ -202,7 +202,8 @@ Tensor scratch_for(const Tensor& like, cudaStream_t stream, int64_t bytes) {
 Tensor rotary(const Tensor& x, const Tensor& table, const Tensor& positions, bool interleaved,
               const optional<Tensor>& out) {
   const int code = dtype_code(x.scalar_type());
-  CHECK_VALUE(x.is_cuda() && code >= 0 && x.dim() == 3, "rotary runs on bf16 or fp16 CUDA tensors [T, heads, D]");
+  CHECK_VALUE(x.is_cuda() && code >= 0 && x.dim() == 3, "rotary runs on bf16 or fp16 CUDA tensors [T, heads, D], not on ",
+              x.scalar_type(), " ", x.sizes(), " on ", x.device());
   const int64_t T = x.size(0), H = x.size(1), D = x.size(2);
   TORCH_CHECK_NOT_IMPLEMENTED(D == 64 || D == 128, "head_dim ", D, ": the rotary kernel has 64 and 128");
   const RotaryTable tab = rotary_of(table, D, x);

@@ -152,3 +152,13 @@ def test_rotary_table():
                 dict(scaling=("other", 2.0))):
         with pytest.raises(ValueError):
             paged.rotary_table(**{"max_pos": 8, "rotary_dim": 32, "device": "cpu", **bad})
+
+
+def test_refusals_say_what_was_given():
+    """Messages are formatted in C++, which takes one C++ runtime in the process."""
+    z = torch.zeros(1, 8, 2, 128, dtype=torch.bfloat16)
+    n = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="not on cpu"):
+        paged.paged_attention(z[0], z, z, n[None], n, n)
+    with pytest.raises(ValueError, match=r"BFloat16 \[8, 2, 128\] on cpu"):
+        paged.rotary(z[0], torch.zeros(4, 64, 2), n)
