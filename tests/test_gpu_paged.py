@@ -251,6 +251,141 @@ def test_strided_inputs_and_output(cuda):
     assert torch.equal(paged_attention(odd, k, v, table, s, kv), paged_attention(odd.clone(), k, v, table, s, kv))
 
 
+@pytest.mark.parametrize("lq", [1, 60])
+def test_pools_and_tables_as_views(cuda, lq):
+    """Keys and values of a page beside one another in one tensor, a block table inside a wider one, one
+    page, one head: the strides that a view has, not those that its shape suggests."""
+    from reworld_b200 import paged_attention, paged_evict, paged_rotary_store
+    k, v, table, kv, g = _cache(cuda, [200, 130], 16, 2, 128, BF, 13)
+    both = torch.full((k.shape[0], 2, 16, 3, 160), float("nan"), dtype=BF, device=cuda)
+    ks, vs = both[:, 0, :, :2, :128], both[:, 1, :, 1:, 16:144]
+    ks.copy_(k)
+    vs.copy_(v)
+    wide = torch.full((2, table.shape[1] + 5), -7, dtype=torch.int32, device=cuda)
+    wide[:, 2:2 + table.shape[1]] = table
+    ts = wide[:, 2:2 + table.shape[1]]
+    s = _starts(cuda, [lq, lq])
+    q = torch.randn(2 * lq, 8, 128, generator=g, device=cuda).to(BF)
+    w, ws = (torch.zeros(2, 2, 16 * table.shape[1], device=cuda) for _ in range(2))
+    a = paged_attention(q, k, v, table, s, kv, max_q_len=lq, weight_sums=w)
+    b = paged_attention(q, ks, vs, ts, s, kv, max_q_len=lq, weight_sums=ws)
+    assert torch.equal(a, b) and torch.equal(w, ws)
+    kn, vn = (torch.randn(2 * lq, 2, 128, generator=g, device=cuda).to(BF) for _ in range(2))
+    for kk, vv, tt in ((k, v, table), (ks, vs, ts)):
+        paged_rotary_store(kn, vn, kk, vv, tt, s, kv)
+    free = [i for i in range(k.shape[0]) if i not in set(table.flatten().tolist())][:2]
+    dst = torch.tensor(free, dtype=torch.int32, device=cuda).view(2, 1)
+    for kk, vv, tt in ((k, v, table), (ks, vs, ts)):
+        paged_evict(kk, vv, tt, kv, w, 10, dst)
+    assert torch.equal(torch.nan_to_num(k, 5.0), torch.nan_to_num(ks, 5.0))
+    assert torch.equal(torch.nan_to_num(v, 5.0), torch.nan_to_num(vs, 5.0))
+    one = torch.zeros(1, 1, dtype=torch.int32, device=cuda)
+    n = torch.tensor([min(16, lq + 3)], dtype=torch.int32, device=cuda)
+    lq = min(lq, 16)
+    page = both[:1, 0, :, :1, :128].copy_(torch.randn(1, 16, 1, 128, generator=g, device=cuda))
+    got = paged_attention(q[:lq], page, page, one, _starts(cuda, [lq]), n, max_q_len=lq)
+    want = op.attention(q[:lq], page, page, one, torch.tensor([0, lq]), n, True, 1 / math.sqrt(128))
+    _check(got, None, None, want, BF, 128, 16)
+    _status_clean()
+
+
+def test_two_threads_on_one_stream(cuda):
+    """Calls of several launches from two host threads that share a stream, and its workspace."""
+    import threading
+    from reworld_b200 import paged_attention
+    k, v, table, kv, g = _cache(cuda, [3000, 2500], 16, 2, 64, BF, 14)
+    qs = [torch.randn(n, 8, 64, generator=g, device=cuda).to(BF) for n in (2, 140)]
+    ss = [_starts(cuda, [1, 1]), _starts(cuda, [70, 70])]
+    want = [paged_attention(q, k, v, table, s, kv, max_q_len=q.shape[0] // 2) for q, s in zip(qs, ss)]
+    bad = []
+
+    def work(i):
+        for _ in range(60):
+            o = paged_attention(qs[i], k, v, table, ss[i], kv, max_q_len=qs[i].shape[0] // 2)
+            bad.append(not torch.equal(o, want[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for x in threads:
+        x.start()
+    for x in threads:
+        x.join()
+    assert len(bad) == 120 and not any(bad)
+    _status_clean()
+
+
+def test_nothing_to_do(cuda):
+    from reworld_b200 import paged_attention, paged_evict, paged_rotary_store, rotary, rotary_table
+    k, v, table, kv, g = _cache(cuda, [30], 16, 2, 64, BF, 15)
+    q = torch.randn(3, 4, 64, generator=g, device=cuda).to(BF)
+    none = torch.zeros(0, dtype=torch.int32, device=cuda)
+    out = torch.full_like(q, 3.0)
+    paged_attention(q, k, v, table, _starts(cuda, [3]), kv, max_q_len=0, out=out)
+    paged_attention(q, k, v, table[:0], _starts(cuda, []), none, out=out)
+    assert (out == 3.0).all()
+    o, lse = paged_attention(q[:0], k, v, table, _starts(cuda, [0]), kv, return_lse=True)
+    assert o.shape == (0, 4, 64) and lse.shape == (0, 4)
+    assert paged_rotary_store(q[:0, :2], q[:0, :2], k, v, table, _starts(cuda, [0]), kv, q=q[:0]).shape == (0, 4, 64)
+    assert rotary(q[:0], rotary_table(8, 32, device=cuda), none).shape == (0, 4, 64)
+    kept, lens, sums = paged_evict(k, v, table[:0], none, torch.zeros(0, 2, 32, device=cuda), 8,
+                                   torch.zeros(0, 1, dtype=torch.int32, device=cuda))
+    assert kept.shape == (0, 2, 8) and lens.shape == (0,) and sums.shape == (0, 2, 32)
+    # a table without pages: every row sees nothing
+    empty = torch.zeros(1, 0, dtype=torch.int32, device=cuda)
+    w = torch.ones(1, 2, 4, device=cuda)
+    for mq in (1, 3):
+        out, lse = paged_attention(q, k, v, empty, _starts(cuda, [mq]), torch.zeros_like(kv), max_q_len=mq, weight_sums=w,
+                                   return_lse=True)
+        assert not out[:mq].any() and (lse[:mq] == -math.inf).all() and (w == 1).all()
+    _status_clean()
+
+
+def test_refusals_on_device_tensors(cuda):
+    from reworld_b200 import paged_attention, paged_evict, paged_rotary_store, rotary, rotary_table
+    k, v, table, kv, g = _cache(cuda, [30, 40], 16, 2, 64, BF, 16)
+    q = torch.randn(6, 4, 64, generator=g, device=cuda).to(BF)
+    s = _starts(cuda, [3, 3])
+    w = torch.zeros(2, 2, table.shape[1] * 16, device=cuda)
+
+    def attend(q=q, k=k, v=v, t=table, s=s, kv=kv, **kw):
+        return paged_attention(q, k, v, t, s, kv, **kw)
+
+    for bad in (dict(q=q.half()), dict(q=q[:, :3]), dict(q=q[..., :32]), dict(q=q[0]), dict(v=v[:, :8]), dict(v=v.half()),
+                dict(t=table.long()), dict(t=table[:1]), dict(s=s.long()), dict(s=s[:2]), dict(kv=kv.long()),
+                dict(kv=kv.cpu()), dict(s=s.cpu()), dict(softmax_scale=0.0), dict(softmax_scale=float("nan")),
+                dict(max_q_len=-1), dict(out=q), dict(out=q[:3]), dict(out=q.half()), dict(weight_sums=w[:, :1]),
+                dict(weight_sums=w.half()), dict(weight_sums=w[..., :-1]), dict(weight_sums=w[:1].expand(2, 2, w.shape[2])),
+                dict(out=torch.zeros(1, 4, 64, dtype=BF, device=cuda).expand(6, 4, 64)), dict(k=k[..., ::2], v=v[..., ::2]),
+                dict(k=k.transpose(2, 3), v=v.transpose(2, 3))):
+        with pytest.raises((ValueError, NotImplementedError)):
+            attend(**bad)
+    for bad in (dict(k=k[:, :12], v=v[:, :12]), dict(k=k[..., :32].contiguous(), v=v[..., :32].contiguous())):
+        with pytest.raises(NotImplementedError):
+            attend(**bad)
+    with pytest.raises(NotImplementedError):
+        attend(q=torch.zeros(6, 258, 64, dtype=BF, device=cuda))
+    buf = torch.zeros(12, 4, 64, dtype=BF, device=cuda)
+    tab = rotary_table(64, 32, device=cuda)
+    pos = torch.zeros(6, dtype=torch.int32, device=cuda)
+    for bad in (dict(out=buf[3:9]), dict(table=tab.half()), dict(table=tab[:, :5]), dict(positions=pos.long()),
+                dict(positions=pos[:5]), dict(table=rotary_table(64, 128, device=cuda))):
+        with pytest.raises(ValueError):
+            rotary(**{**dict(x=buf[:6], table=tab, positions=pos), **bad})
+    kn = torch.zeros(6, 2, 64, dtype=BF, device=cuda)
+    for bad in (dict(k=kn[:5]), dict(v=kn.half()), dict(q=q[:5]), dict(q_out=q), dict(q=kn, q_out=kn[:, :1]),
+                dict(positions=pos[:2]), dict(q=q, q_out=torch.zeros(6, 5, 64, dtype=BF, device=cuda)),
+                dict(q=torch.zeros_like(kn), q_out=kn)):
+        with pytest.raises(ValueError):
+            paged_rotary_store(**{**dict(k=kn, v=kn, k_pages=k, v_pages=v, block_table=table, q_starts=s, kv_lens=kv),
+                                  **bad})
+    dst = torch.zeros(2, 1, dtype=torch.int32, device=cuda)
+    for bad in (dict(keep=0), dict(keep=17), dict(n_sink=-1), dict(n_sink=5, n_recent=6), dict(dst_table=dst[:1]),
+                dict(dst_table=dst.long()), dict(weight_sums=w[:1])):
+        with pytest.raises(ValueError):
+            paged_evict(**{**dict(k_pages=k, v_pages=v, block_table=table, kv_lens=kv, weight_sums=w, keep=10,
+                                  dst_table=dst), **bad})
+    _status_clean()
+
+
 def test_another_stream_and_two_graphs(cuda):
     """Calls on two streams at once, and two captured graphs replayed at once with new lengths."""
     from reworld_b200 import paged_attention
