@@ -258,10 +258,10 @@ __global__ void __launch_bounds__(MOVE_THREADS) move_kernel(const __grid_constan
   constexpr int RSTEP = MOVE_THREADS / CH;
   griddep_launch_dependents();
   griddep_wait();
-  const int hk = blockIdx.x, b = blockIdx.z;
+  const int hk = blockIdx.x % p.pool.Hkv, b = blockIdx.y;
   const int c = threadIdx.x % CH;
   const int n_new = min(rows_of(p, b, nullptr), p.keep);
-  const int j0 = blockIdx.y * (ROWS * RSTEP) + threadIdx.x / CH;
+  const int j0 = blockIdx.x / p.pool.Hkv * (ROWS * RSTEP) + threadIdx.x / CH;
   const int* kept = p.kept + ((long long)b * p.pool.Hkv + hk) * p.keep;
   const int mask = (1 << p.pool.page_shift) - 1;
   uint4 kr[ROWS], vr[ROWS];
@@ -310,6 +310,9 @@ extern "C" int rw_paged_evict(const rw_paged_t* cache, const float* sums, long l
   if (cache->B == 0) return RW_OK;
   if (!sums || !new_sums || !kept || !new_lens || !dst_table) return RW_ERR_INVALID_ARG;
   if ((long long)dst_width * cache->page_size < keep || new_cap < keep) return RW_ERR_CAPACITY;
+  const int rows = 2 * evict::MOVE_THREADS / (cache->D / 8);   // of a block of move_kernel
+  const long long blocks = ((long long)keep + rows - 1) / rows;
+  if (blocks * p.pool.Hkv > 0x7fffffffll) return RW_ERR_CAPACITY;
   p.sums = sums;
   p.sums_sb = sums_sb; p.sums_sh = sums_sh;
   p.new_sums = new_sums; p.new_cap = new_cap;
@@ -349,8 +352,7 @@ extern "C" int rw_paged_evict(const rw_paged_t* cache, const float* sums, long l
     if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess)
       return RW_ERR_CUDA;
   }
-  const int rows = 2 * evict::MOVE_THREADS / (cache->D / 8);
-  const dim3 grid(p.pool.Hkv, (keep + rows - 1) / rows, cache->B);
+  const dim3 grid((unsigned)(blocks * p.pool.Hkv), cache->B);
   auto kernel = cache->D == 128 ? evict::move_kernel<128> : evict::move_kernel<64>;
   return launch_dependent(kernel, grid, dim3(evict::MOVE_THREADS), 0, st, p) == cudaSuccess ? RW_OK : RW_ERR_CUDA;
 }

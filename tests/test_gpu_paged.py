@@ -386,6 +386,39 @@ def test_refusals_on_device_tensors(cuda):
     _status_clean()
 
 
+@pytest.mark.parametrize("lq,hkv,layout", [(1, 2, "rows"), (40, 2, "rows"), (40, 2, "heads")])
+def test_pages_behind_eight_gigabytes(cuda, lq, hkv, layout):
+    """The same pages at the end of a pool whose offsets pass 32 bits, in bytes and in elements."""
+    from reworld_b200 import paged_attention, paged_evict, paged_rotary_store
+    page, D, n = 256, 128, 700
+    k, v, table, kv, g = _cache(cuda, [n], page, hkv, D, BF, 3, layout, spare=4)
+    few = k.shape[0]
+    total = 2 ** 33 // (page * hkv * D * 2) + few + 5
+    shape = (total, page, hkv, D) if layout == "rows" else (total, hkv, page, D)
+    big = [torch.empty(shape, dtype=BF, device=cuda) for _ in range(2)]
+    if layout == "heads":
+        big = [t.transpose(1, 2) for t in big]
+    assert (total - few) * big[0].stride(0) >= 2 ** 32
+    for t, s in zip(big, (k, v)):
+        t[total - few:] = s
+    far = table + (total - few)
+    starts = _starts(cuda, [lq])
+    q, nk, nv = ((torch.randn(lq, h, D, generator=g, device=cuda)).to(BF) for h in (4 * hkv, hkv, hkv))
+    got = []
+    free = torch.tensor([i for i in range(few) if i not in table.flatten().tolist()][:2], dtype=torch.int32, device=cuda)
+    for kp, vp, tb, at in ((k, v, table, 0), (*big, far, total - few)):
+        w = torch.zeros(1, hkv, table.shape[1] * page, device=cuda)
+        paged_rotary_store(nk, nv, kp, vp, tb, starts, kv)
+        o = paged_attention(q, kp, vp, tb, starts, kv, max_q_len=lq, weight_sums=w)
+        kept, lens, sums = paged_evict(kp, vp, tb, kv, w, 300, (free + at)[None], 4, 50)
+        pages = (kp[at:at + few].clone(), vp[at:at + few].clone())
+        got.append((o, w, kept, lens, sums, *pages))
+    torch.cuda.synchronize()
+    _status_clean()
+    for a, b in zip(*got):
+        assert torch.equal(torch.nan_to_num(a.float(), 77.0), torch.nan_to_num(b.float(), 77.0))
+
+
 def test_another_stream_and_two_graphs(cuda):
     """Calls on two streams at once, and two captured graphs replayed at once with new lengths."""
     from reworld_b200 import paged_attention
@@ -602,6 +635,10 @@ def _evict_case(cuda, lens, page, hkv, D, keep, sink, recent, dtype=BF, sums=Non
 @pytest.mark.parametrize("layout", ["rows", "heads"])
 def test_evict(cuda, lens, page, hkv, D, keep, sink, recent, layout):
     _evict_case(cuda, lens, page, hkv, D, keep, sink, recent, layout=layout)
+
+
+def test_evict_keeps_over_a_million_rows(cuda):
+    _evict_case(cuda, [1100000, 5], 1024, 1, 128, 1060000, 4, 1000)
 
 
 @pytest.mark.parametrize("kind", ["equal", "zeros", "few values", "signs and specials", "close"])
