@@ -187,33 +187,34 @@ __device__ __forceinline__ void plan_own(const Params& p, Plan& pl, int upt, int
     }
     if (lane == 0) {
       pl.cost[b + 1] = sum * p.pool.Hkv;
-      pl.units[b + 1] = nu * p.pool.Hkv;
+      pl.units[b + 1] = (int)min(0x7fffffffll, (long long)nu * p.pool.Hkv);
       atomicMax(&pl.longest, top);
     }
   }
 }
-__device__ __forceinline__ void plan_sum(const Params& p, Plan& pl, int lane) {
-  long long ct = 0;
-  int cu = 0;
+// Number of units.  Sequences whose starts go up have far fewer than an int counts; others are reported (load_seq).
+__device__ __forceinline__ long long plan_sum(const Params& p, Plan& pl, int lane) {
+  long long ct = 0, cu = 0;
   for (int b0 = 0; b0 < p.pool.B; b0 += 32) {
     const int b = b0 + lane;
     long long t = b < p.pool.B ? pl.cost[b + 1] : 0;
-    int u = b < p.pool.B ? pl.units[b + 1] : 0;
+    long long u = b < p.pool.B ? pl.units[b + 1] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long y = __shfl_up_sync(0xffffffffu, t, o);
-      const int z = __shfl_up_sync(0xffffffffu, u, o);
+      const long long z = __shfl_up_sync(0xffffffffu, u, o);
       if (lane >= o) { t += y; u += z; }
     }
     if (b < p.pool.B) {
       pl.cost[b + 1] = ct + t;
-      pl.units[b + 1] = cu + u;
+      pl.units[b + 1] = (int)(cu + u);
     }
     ct += __shfl_sync(0xffffffffu, t, 31);
     cu += __shfl_sync(0xffffffffu, u, 31);
   }
   if (lane == 0) { pl.cost[0] = 0; pl.units[0] = 0; }
   __syncwarp();
+  return cu;
 }
 
 // Where a walker over the units in the order (sequence, head, row tile) stands.
@@ -429,15 +430,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     __syncwarp();
   };
   if (warp == WARP_PLAN) {
-    plan_sum(p, pl, lane);
+    const long long U = plan_sum(p, pl, lane);
     const long long N = pl.cost[p.pool.B];       // of all work
-    const int U = pl.units[p.pool.B];
     if (even && lane == 0) p.header[pid] = make_int4(0, 0, 0, 0);
     if (N < (long long)C * MIN_SHARE)
-      C = (int)min((long long)C, max((long long)U, paged::div_count(N + MIN_SHARE - 1, MIN_SHARE)));
-    if (pid < C) {
+      C = (int)min((long long)C, max(U, paged::div_count(N + MIN_SHARE - 1, MIN_SHARE)));
+    if (pid < C && U <= 0x7fffffffll) {
       // about equal: no unit is over 1/8 longer than their mean
-      if ((long long)pl.longest * U * 8 <= N * 9) waves = U / C;
+      if ((long long)pl.longest * U * 8 <= N * 9) waves = (int)paged::div_count(U, C);
       if (waves > 0 && waves * C < U) {
         const Walk f = walk_to_unit(p, pl, waves * C, upt);
         t_base = cost_before(p, pl, f, upt, lane);

@@ -108,24 +108,30 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   for (int b = threadIdx.x; b < p.pool.B; b += NUM_THREADS) {
     const Seq s = paged::load_seq(p.pool, b, p.T, nullptr);
     seq[b] = make_int3(s.s0, s.lq, s.kv);
-    before[b + 1] = s.lq > 0 ? (s.kv + BM - 1) / BM * p.pool.Hkv : 0;
+    before[b + 1] = s.lq > 0 ? (int)min(0x7fffffffll, (long long)((s.kv + BM - 1) / BM) * p.pool.Hkv) : 0;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   if (warp == 0) {
-    int c = 0;
+    long long c = 0;
     for (int b0 = 0; b0 < p.pool.B; b0 += 32) {
-      int u = b0 + lane < p.pool.B ? before[b0 + lane + 1] : 0;
+      long long u = b0 + lane < p.pool.B ? before[b0 + lane + 1] : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int z = __shfl_up_sync(0xffffffffu, u, o);
+        const long long z = __shfl_up_sync(0xffffffffu, u, o);
         if (lane >= o) u += z;
       }
-      if (b0 + lane < p.pool.B) before[b0 + lane + 1] = c + u;
+      if (b0 + lane < p.pool.B) before[b0 + lane + 1] = (int)(c + u);
       c += __shfl_sync(0xffffffffu, u, 31);
     }
-    if (lane == 0) before[0] = 0;
+    if (lane == 0) {
+      before[0] = 0;
+      if (c >= 0x7fffffffll) {   // (as many as that would take hours)
+        report_status(p.status, RW_STATUS_BAD_SLOT);
+        before[p.pool.B] = 0;
+      }
+    }
   }
   __syncthreads();
   const uint32_t tmem = sb.tmem_base;
