@@ -448,7 +448,7 @@ int rw_paged_rotary_store(const rw_paged_t* cache, const void* k, const void* v,
  * sums_sb, sums_sh; sums[b, g, j] += the weights that the rows of key head g's group
  * gave to cached row j.  The order of the additions is fixed.
  * workspace: device memory, 16-byte aligned, rw_paged_attn_workspace_bytes(...)
- * bytes, contents of no matter; calls that overlap on the GPU need workspaces of
+ * bytes (0: it may be null), contents of no matter; calls that overlap on the GPU need workspaces of
  * their own.  (cache_rows: table_width * page_size; with_sums: sums != NULL.) */
 int rw_paged_attn(const rw_paged_t* cache, const void* q, void* out, float* lse, int T, int Hq, int max_q_len,
                   long long q_sl, long long q_sh, long long o_sl, long long o_sh, int causal, float softmax_scale,

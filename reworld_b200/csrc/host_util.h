@@ -100,6 +100,17 @@ inline bool ensure_smem_attr(const void* func, int bytes, std::atomic<unsigned l
   return true;
 }
 
+// cudaFuncSetAttribute(NonPortableClusterSizeAllowed), as above: clusters of more than 8.
+inline bool ensure_cluster_attr(const void* func, std::atomic<unsigned long long>* done_mask) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  const unsigned long long bit = 1ull << dev;
+  if (done_mask->load(std::memory_order_acquire) & bit) return true;
+  if (cudaFuncSetAttribute(func, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return false;
+  done_mask->fetch_or(bit, std::memory_order_release);
+  return true;
+}
+
 inline bool stride_ok(long long s) { return s > 0 && (s % 8) == 0 && s < (1ll << 38); }
 
 }  // namespace rw

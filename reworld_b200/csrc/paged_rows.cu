@@ -16,7 +16,14 @@
 // In a CTA each of the 4 warps takes 16 keys of a 64-key tile with a running maximum and
 // sum of its own (mma.sync m16n8k16 feeds far more than memory delivers here: a tile of
 // 32 KB costs a warp 32 MMAs), so the warps only meet for the loads; the 4 states are
-// joined when the unit's tiles are done.  Keys and values come through a ring of 3 stages
+// joined when the unit's tiles are done.
+//
+// A short call is bound by its launches and the loads that wait for one another.  Where the
+// device holds a cluster of CTAs for every unit, and a CTA then has few tiles of the longest
+// unit there can be, the cluster joins its parts through distributed shared memory, and adds
+// the weights, whose scores it still has: one launch, no plan and no scratch.
+//
+// Keys and values come through a ring of 3 stages
 // of 16-byte cp.async; rows behind the last visible one are filled with zeros, never
 // read, so what a page holds there (NaN included) does not matter.
 #include <algorithm>
@@ -44,6 +51,7 @@ struct Params {
   float* lse;                   // [T, Hq] natural logarithm, or null
   long long q_sl, q_sh, o_sl, o_sh;  // byte strides
   int T, Hq, G, causal;
+  int cs, pitch;                // CLUSTER: CTAs of a unit, keys of a CTA at most
   int rows_most;                // rows of a sequence and key head at most
   float scale_log2;
   float* part;                  // [2 C][16 * D + 32]: O, then m, then l
@@ -109,6 +117,11 @@ struct Seg {
   long long u0;
 };
 
+// Keys that every row sees: tiles behind them are looked through for values that are not finite.
+__device__ __forceinline__ int keys_of_all(const Params& p, const Entry& n) {
+  return p.causal ? min(n.keys, max(0, n.s.kv - n.s.lq + 1)) : n.keys;
+}
+
 // Tiles of an entry: at least one while it has rows, so that rows that see nothing are written too.
 __device__ __forceinline__ int tiles_of(const Entry& n) {
   return n.rows > 0 ? max(1, (n.keys + TILE - 1) / TILE) : 0;
@@ -133,7 +146,22 @@ __device__ __forceinline__ void put_row(const Params& p, const Entry& en, int b,
   }
 }
 
-template <bool HALF, int D>
+__device__ __forceinline__ float ld_cluster(uint32_t a) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+  return v;
+}
+
+constexpr int MAX_CLUSTER = 16;
+constexpr int CLUSTER_TILES = 16;  // of a CTA at most
+
+// CLUSTER: the CTAs of a cluster share the tiles of one unit.
+template <bool HALF, int D, bool CLUSTER>
 __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant__ Params p) {
   constexpr int PITCH = 2 * D;               // bytes of a row in shared memory
   constexpr int CH = D / 8;                  // 16-byte chunks of a row
@@ -146,39 +174,63 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
   __shared__ Seg seg[2];
   __shared__ struct { long long t, ebase; Entry en; int e; } plan;
   __shared__ float sm_m[WARPS][RT], sm_l[WARPS][RT];
+  __shared__ float2 ml[CLUSTER ? RT : 1];  // m and 1 / l of every row
   __shared__ int dirty;         // 1: the segment has values that are not finite (paged.cuh)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int grp = lane >> 2, quad = lane & 3;
   griddep_launch_dependents();
   griddep_wait();
 
-  // ---- tiles before every thread's run of entries, and of all
-  const int NE = p.pool.B;
-  const int run = (NE + THREADS - 1) / THREADS;
-  {
-    long long mine = 0;
-    for (int e = tid * run; e < min(NE, (tid + 1) * run); ++e)
-      mine += (long long)tiles_of(load_entry(p, e, blockIdx.x == 0 ? p.status : nullptr)) * p.pool.Hkv;
-    long long x = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
+  const int cta = blockIdx.x;
+  const int rank = CLUSTER ? cta % p.cs : 0;
+  long long share = 1, t1 = 0;
+  if constexpr (CLUSTER) {
+    const int unit = cta / p.cs;
+    Seg s;
+    s.b = unit / p.pool.Hkv;
+    s.hk = unit - s.b * p.pool.Hkv;
+    s.en = load_entry(p, s.b, cta % (p.cs * p.pool.Hkv) == 0 && tid == 0 ? p.status : nullptr);
+    if (s.en.rows == 0) return;              // (with the whole cluster)
+    s.n_tiles = tiles_of(s.en);
+    const int per = (s.n_tiles + p.cs - 1) / p.cs;
+    s.k0 = min(rank * per, s.n_tiles);
+    s.n = min(per, s.n_tiles - s.k0);
+    s.all = keys_of_all(p, s.en);
+    s.u0 = 0;
+    if (tid == 0) {
+      seg[0] = s;
+      seg[1].n = 0;
+      dirty = 0;
     }
-    __shared__ long long wsum[WARPS];
-    if (lane == 31) wsum[warp] = x;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) x += wsum[w];
-    base[tid] = x - mine;
-    if (tid == THREADS - 1) base[THREADS] = x;
-    __syncthreads();
+  } else {
+    // ---- tiles before every thread's run of entries, and of all
+    const int NE = p.pool.B;
+    const int run = (NE + THREADS - 1) / THREADS;
+    {
+      long long mine = 0;
+      for (int e = tid * run; e < min(NE, (tid + 1) * run); ++e)
+        mine += (long long)tiles_of(load_entry(p, e, blockIdx.x == 0 ? p.status : nullptr)) * p.pool.Hkv;
+      long long x = mine;
+  #pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      __shared__ long long wsum[WARPS];
+      if (lane == 31) wsum[warp] = x;
+      __syncthreads();
+      for (int w = 0; w < warp; ++w) x += wsum[w];
+      base[tid] = x - mine;
+      if (tid == THREADS - 1) base[THREADS] = x;
+      __syncthreads();
+    }
+    const long long N = base[THREADS];
+    const int C = (int)max(1ll, min((long long)gridDim.x, N));  // (no share without a tile)
+    if (cta >= C) return;
+    share = paged::div_count(N + C - 1, C);
+    if (share * cta >= N) return;  // (the last CTAs may find nothing left)
+    t1 = min(N, share * (cta + 1));
   }
-  const long long N = base[THREADS];
-  const int C = (int)max(1ll, min((long long)gridDim.x, N)), cta = blockIdx.x;  // (no share without a tile)
-  if (cta >= C) return;
-  const long long share = paged::div_count(N + C - 1, C);
-  if (share * cta >= N) return;  // (the last CTAs may find nothing left)
-  const long long t1 = min(N, share * (cta + 1));
   // The segments of the share, one ahead, by thread 0: seg[i & 1] is segment i (n == 0: there is none).
   auto advance = [&](int i) {
     Seg s;
@@ -195,14 +247,14 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
       s.u0 = plan.ebase + (long long)s.hk * s.n_tiles;
       s.k0 = (int)(plan.t - s.u0);
       s.n = (int)(min(t1, s.u0 + s.n_tiles) - plan.t);
-      // keys that every row sees: tiles behind them are looked through for values that are not finite
-      s.all = p.causal ? min(s.en.keys, max(0, s.en.s.kv - s.en.s.lq + 1)) : s.en.keys;
+      s.all = keys_of_all(p, s.en);
       plan.t += s.n;
     }
     seg[i & 1] = s;
   };
-  if (tid == 0) {
+  if (!CLUSTER && tid == 0) {
     const long long t0 = share * cta;
+    const int run = (p.pool.B + THREADS - 1) / THREADS;
     int lo = 0, hi = THREADS - 1;
     while (lo < hi) {   // last thread whose run of entries begins at or before t0
       const int mid = (lo + hi + 1) >> 1;
@@ -253,8 +305,8 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
   for (int si = 0;; ++si) {
     const Seg& sg = seg[si & 1];
     const int n = sg.n;
-    if (n == 0) break;
-    if (tid == 0) advance(si + 1);           // (read behind the barriers below)
+    if (!CLUSTER && n == 0) break;
+    if (!CLUSTER && tid == 0) advance(si + 1);  // (read behind the barriers below)
     const Entry en = sg.en;
     const Seq s = en.s;
     const int hk = sg.hk, b = sg.b, k0 = sg.k0, all = sg.all;
@@ -335,7 +387,17 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
           sc[i][x] = v;
           mx[x >> 1] = fmaxf(mx[x >> 1], v);
         }
-      if (p.scores) {
+      if (CLUSTER && p.sums) {
+        float* sc_sh = reinterpret_cast<float*>(smem + STAGES * STAGE) + k * TILE + kw + 2 * quad;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            if (grp + 8 * x < en.rows)
+              *reinterpret_cast<float2*>(sc_sh + (grp + 8 * x) * p.pitch + 8 * i) =
+                  make_float2(sc[i][2 * x], sc[i][2 * x + 1]);
+      }
+      if (!CLUSTER && p.scores) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -398,7 +460,7 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
     __syncthreads();                         // the last tile's stage is free: it takes the warps' states
 
     // ---- join the warps: fo[warp][16][D], 16-byte chunks of a row in another order for every row
-    float* fo = reinterpret_cast<float*>(smem + ((J0 + n - 1) % STAGES) * STAGE);
+    float* fo = reinterpret_cast<float*>(smem + (CLUSTER ? 0 : ((J0 + n - 1) % STAGES) * STAGE));
     auto at = [&](int w, int r, int c) { return fo + (w * RT + r) * D + (((c >> 2) ^ (r & 7)) << 2) + (c & 3); };
     if (quad == 0) {
 #pragma unroll
@@ -414,11 +476,11 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
         *reinterpret_cast<float2*>(at(warp, grp + 8 * x, 8 * i + 2 * quad)) = make_float2(o[i][2 * x], o[i][2 * x + 1]);
     __syncthreads();
 
-    const bool whole = n == sg.n_tiles;
+    const bool whole = !CLUSTER && n == sg.n_tiles;
     // the parts of a unit: the first in the second slot of its CTA if that has a segment before it, the others in the
     // first slots of the CTAs that follow
     const int my_slot = 2 * cta + (si > 0 ? 1 : 0);
-    if (k0 == 0 && tid == 0) {
+    if (!CLUSTER && k0 == 0 && tid == 0) {
       int parts = 0;
       if (!whole) {
         // up to the CTA that has the unit's last tile
@@ -427,7 +489,7 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
       }
       p.header[(long long)b * p.pool.Hkv + hk] = make_int2(my_slot, parts);
     }
-    float* slot = p.part + (long long)my_slot * SLOT;
+    float* slot = CLUSTER ? reinterpret_cast<float*>(smem + STAGE) : p.part + (long long)my_slot * SLOT;
     auto put = [&](int r, int c, float2 v, float mm, float ll) { put_row<HALF>(p, en, b, hk, r, c, v, mm, ll); };
     // 2 channels of a row a thread and step
     for (int i = tid; i < en.rows * (D / 2); i += THREADS) {
@@ -461,6 +523,79 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
           slot[RT * D + RT + r] = ll;
         }
       }
+    }
+    if constexpr (CLUSTER) {
+      constexpr int KEYS = CLUSTER_TILES * TILE / THREADS;   // of a thread, whose sums are read meanwhile
+      float* dst = p.sums + b * p.sums_sb + hk * p.sums_sh + k0 * TILE + tid;
+      const int keys = min(n * TILE, en.keys - k0 * TILE) - tid;
+      float old[KEYS];
+      if (p.sums) {
+#pragma unroll
+        for (int i = 0; i < KEYS; ++i) old[i] = i * THREADS < keys ? dst[i * THREADS] : 0.f;
+      }
+      cluster_sync();
+      auto part = [&](int i, int at) { return mapa_shared(sbase + STAGE + 4 * at, (uint32_t)i); };
+      // (m, l, and with them channels c, c + 1) of row r over the cluster, 8 parts' loads under way at once
+      auto join = [&](int r, int c, bool with_o, float& mm, float& ll, float2& v) {
+        mm = -INFINITY;
+        ll = 0.f;
+        v = make_float2(0.f, 0.f);
+#pragma unroll 1
+        for (int w0 = 0; w0 < p.cs; w0 += 8) {
+          float pm[8], pl[8];
+          float2 px[8];
+#pragma unroll
+          for (int w = 0; w < 8; ++w) {
+            pm[w] = -INFINITY;
+            pl[w] = 0.f;
+            px[w] = make_float2(0.f, 0.f);
+            if (w0 + w < p.cs) {
+              pm[w] = ld_cluster(part(w0 + w, RT * D + r));
+              pl[w] = ld_cluster(part(w0 + w, RT * D + RT + r));
+              if (with_o) px[w] = ld_cluster2(part(w0 + w, r * D + c));
+            }
+          }
+          float top = mm;
+#pragma unroll
+          for (int w = 0; w < 8; ++w) top = fmaxf(top, pm[w]);
+          const float bs = top == -INFINITY ? 0.f : top, f0 = fast_exp2(mm - bs);
+          v.x *= f0;
+          v.y *= f0;
+          ll *= f0;
+          mm = top;
+#pragma unroll
+          for (int w = 0; w < 8; ++w) {
+            const float f = fast_exp2(pm[w] - bs);
+            v.x += f * px[w].x;
+            v.y += f * px[w].y;
+            ll += f * pl[w];
+          }
+        }
+      };
+      float mm, ll;
+      float2 v;
+      for (int i = rank * THREADS + tid; i < en.rows * (D / 2); i += p.cs * THREADS) {
+        const int r = i / (D / 2), c = 2 * (i % (D / 2));
+        join(r, c, true, mm, ll, v);
+        put(r, c, v, mm, ll);
+      }
+      if (p.sums) {
+        if (tid < en.rows) {
+          join(tid, 0, false, mm, ll, v);
+          ml[tid] = make_float2(mm == -INFINITY ? 0.f : mm, ll != 0.f ? 1.f / ll : 0.f);
+        }
+        __syncthreads();
+        const float* sc_sh = reinterpret_cast<const float*>(smem + STAGES * STAGE) + tid;
+#pragma unroll
+        for (int i = 0; i < KEYS; ++i)
+          if (i * THREADS < keys) {
+            float add = 0.f;
+            for (int r = 0; r < en.rows; ++r) add += fast_exp2(sc_sh[r * p.pitch + i * THREADS] - ml[r].x) * ml[r].y;
+            dst[i * THREADS] = old[i] + add;
+          }
+      }
+      cluster_sync();                        // no CTA leaves while another may read its part
+      break;
     }
     J0 += n;
     __syncthreads();                         // the warps' states are read
@@ -649,12 +784,65 @@ inline Layout layout(int D, int C, int B, int Hkv, long long rows, long long cap
   return l;
 }
 
+// A launch of the CLUSTER kernel: CTAs of a unit (0: units are shared out among all CTAs instead), keys of a CTA at most,
+// dynamic shared memory.
+//
+// A cluster saves a second launch, the plan and what goes through scratch: 3 to 6 us, with weights 9.  What it may lose
+// is that its CTAs have more tiles than an equal share of all CTAs would be, 0.6 to 0.9 us each with a head of 128, half
+// of that with 64.  By cluster and by shares, us: 8 heads of 128, 500 rows 6.1 and 9.2, 4000 rows 10.6 and 14.1, 8000
+// rows (8 tiles a CTA) 14.9 and 17.1, 16000 rows (16 tiles) 24.0 and 21.2; 2 heads of 64, 511 rows 5.1 and 8.2, 16000
+// rows 14.9 and 19.2; 32 ragged sequences x 8 heads, up to 500 rows 15.4 and 26.5, up to 1000 rows 23.9 and 31.9; 128
+// of them 68.8 and 79.5, with equal lengths 104 and 98.  With weights: 8 heads, 500 rows 7.2 and 17.2, 8000 rows 17.9
+// and 21.3, 16000 rows 27.7 and 26.9.
+struct Clusters {
+  int cs, pitch, bytes;
+};
+inline Clusters clusters_for(int D, long long units, long long rows, long long cap, bool sums) {
+  const long long tiles = std::max(1ll, (cap + TILE - 1) / TILE);
+  const int all = grid_size(D), sm = D == 128 ? 2 : 4;
+  for (int cs = MAX_CLUSTER; cs >= 1; cs /= 2) {
+    const long long per = (tiles + cs - 1) / cs;
+    if (per > CLUSTER_TILES) break;
+    const long long bytes = STAGES * 4 * TILE * D + (sums ? 4 * rows * per * TILE : 0);
+    // as many CTAs as are resident together, by shared memory (4 KB of it is static, or the system's)
+    const long long most = std::min((long long)sm, (220 << 10) / (bytes + 4096)) * (all / sm);
+    if (cs > 1 && (cs / 2 >= tiles || units * cs > most)) continue;
+    if (per <= 1024 / D + units * tiles / all && units < (1 << 30)) return {cs, (int)per * TILE, (int)bytes};
+    break;
+  }
+  return {0, 0, 0};
+}
+
 template <bool HALF, int D>
-int launch_rows(const Params& p, int C, cudaStream_t stream) {
+int launch_cluster(const Params& p, int bytes, cudaStream_t stream) {
+  static std::atomic<unsigned long long> done{0}, done_size{0};
+  constexpr int MOST = STAGES * 4 * TILE * D + 4 * RT * CLUSTER_TILES * TILE;
+  const void* kernel = reinterpret_cast<const void*>(rows_kernel<HALF, D, true>);
+  if (!ensure_smem_attr(kernel, MOST, &done) || !ensure_cluster_attr(kernel, &done_size)) return RW_ERR_CUDA;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(p.pool.B * p.pool.Hkv * p.cs));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.cs;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, rows_kernel<HALF, D, true>, p) == cudaSuccess ? RW_OK : RW_ERR_CUDA;
+}
+
+template <bool HALF, int D>
+int launch_rows(const Params& p, int C, int cluster_bytes, cudaStream_t stream) {
+  if (p.cs) return launch_cluster<HALF, D>(p, cluster_bytes, stream);
   static std::atomic<unsigned long long> done{0};
   const int bytes = STAGES * 2 * TILE * 2 * D;
-  if (!ensure_smem_attr(reinterpret_cast<const void*>(rows_kernel<HALF, D>), bytes, &done)) return RW_ERR_CUDA;
-  if (launch_dependent(rows_kernel<HALF, D>, dim3(C), dim3(THREADS), bytes, stream, p) != cudaSuccess)
+  if (!ensure_smem_attr(reinterpret_cast<const void*>(rows_kernel<HALF, D, false>), bytes, &done)) return RW_ERR_CUDA;
+  if (launch_dependent(rows_kernel<HALF, D, false>, dim3(C), dim3(THREADS), bytes, stream, p) != cudaSuccess)
     return RW_ERR_CUDA;
   constexpr int NT = JOIN_GROUPS * D / 4;
   const unsigned bx = p.sums ? (unsigned)std::min(1024ll, (p.cap + 4 * NT - 1) / (4 * NT)) : (unsigned)p.rows_most;
@@ -667,9 +855,10 @@ int run_rows(const rw_paged_t* cache, const Pool& pool, const chunk::Call& c, lo
   const long long cap = (long long)cache->table_width * cache->page_size;
   const int C = grid_size(cache->D);
   if (C == 0 || C > MAX_PARTS) return RW_ERR_CUDA;
+  const Clusters cl = clusters_for(cache->D, (long long)cache->B * pool.Hkv, rows, cap, sums != nullptr);
   if (cap == 0) sums = nullptr;
   const Layout lay = layout(cache->D, C, cache->B, pool.Hkv, rows, cap, sums != nullptr);
-  if (!workspace || !aligned16(workspace) || workspace_bytes < lay.total) return RW_ERR_INVALID_ARG;
+  if (cl.cs == 0 && (!workspace || !aligned16(workspace) || workspace_bytes < lay.total)) return RW_ERR_INVALID_ARG;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   Params p{};
   p.pool = pool;
@@ -679,11 +868,15 @@ int run_rows(const rw_paged_t* cache, const Pool& pool, const chunk::Call& c, lo
   p.q_sl = 2 * c.q_sl; p.q_sh = 2 * c.q_sh; p.o_sl = 2 * c.o_sl; p.o_sh = 2 * c.o_sh;
   p.T = c.T; p.Hq = c.Hq; p.G = c.Hq / pool.Hkv; p.causal = c.causal;
   p.rows_most = (int)rows;
+  p.cs = cl.cs;
+  p.pitch = cl.pitch;
   p.scale_log2 = c.scale_log2;
-  p.part = reinterpret_cast<float*>(ws + lay.part);
-  p.header = reinterpret_cast<int2*>(ws + lay.header);
-  p.scores = sums ? reinterpret_cast<float*>(ws + lay.scores) : nullptr;
-  p.row_ml = sums ? reinterpret_cast<float2*>(ws + lay.ml) : nullptr;
+  if (cl.cs == 0) {
+    p.part = reinterpret_cast<float*>(ws + lay.part);
+    p.header = reinterpret_cast<int2*>(ws + lay.header);
+    p.scores = sums ? reinterpret_cast<float*>(ws + lay.scores) : nullptr;
+    p.row_ml = sums ? reinterpret_cast<float2*>(ws + lay.ml) : nullptr;
+  }
   p.sums = sums;
   p.sums_sb = sums_sb; p.sums_sh = sums_sh;
   p.cap = cap;
@@ -692,8 +885,8 @@ int run_rows(const rw_paged_t* cache, const Pool& pool, const chunk::Call& c, lo
   const long long most = (long long)cache->B * pool.Hkv * std::max(1ll, (cap + TILE - 1) / TILE);
   const int ctas = (int)std::min((long long)C, most);
   if (cache->dtype == RW_DTYPE_FP16)
-    return cache->D == 128 ? launch_rows<true, 128>(p, ctas, st) : launch_rows<true, 64>(p, ctas, st);
-  return cache->D == 128 ? launch_rows<false, 128>(p, ctas, st) : launch_rows<false, 64>(p, ctas, st);
+    return cache->D == 128 ? launch_rows<true, 128>(p, ctas, cl.bytes, st) : launch_rows<true, 64>(p, ctas, cl.bytes, st);
+  return cache->D == 128 ? launch_rows<false, 128>(p, ctas, cl.bytes, st) : launch_rows<false, 64>(p, ctas, cl.bytes, st);
 }
 
 // The chunk kernels plan MAX_BATCH sequences a launch.
@@ -751,6 +944,7 @@ extern "C" long long rw_paged_attn_workspace_bytes(int T, int Hq, int Hkv, int D
   if (T < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || B < 1 || max_q_len < 1 || (D != 64 && D != 128) || cache_rows < 0)
     return 0;
   const long long rows = (long long)std::min(max_q_len, T) * (Hq / Hkv);
+  if (rows::few_rows(rows) && rows::clusters_for(D, (long long)B * Hkv, rows, cache_rows, with_sums != 0).cs) return 0;
   if (rows::few_rows(rows)) return rows::layout(D, rows::grid_size(D), B, Hkv, rows, cache_rows, with_sums != 0).total;
   return chunk::workspace_bytes(D) + (with_sums ? 4LL * T * Hq : 0);
 }

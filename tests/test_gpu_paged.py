@@ -136,6 +136,29 @@ def test_single_tokens_batches(cuda, batch):
     _run(cuda, [1] * batch, [(37 * i) % 211 + 1 for i in range(batch)], 4, 2, 64, FP, sums=batch < 200)
 
 
+def _widen(table, wide):
+    """Few rows over a long table are shared out among all CTAs, over a short one they are a cluster's."""
+    return torch.nn.functional.pad(table, (0, 1250 - table.shape[1])) if wide else table
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("lqs,lens,hq,hkv,D", [
+    ([1], [575], 8, 2, 64),                              # nine tiles
+    ([1], [64], 8, 8, 128),
+    ([1, 1, 1, 1], [1000, 0, 37, 640], 12, 4, 128),
+    ([3, 0, 2, 3, 3, 1], [511, 200, 300, 2, 65, 1], 8, 2, 128),
+    ([16], [1024], 3, 3, 64),
+    ([4, 2], [1100, 700], 4, 1, 128),
+    ([1], [8100], 4, 4, 128),
+    ([2], [16000], 2, 1, 64),
+    ([1] * 40, [(97 * i) % 500 for i in range(40)], 16, 8, 128),
+    ([2] * 90, [(97 * i) % 900 for i in range(90)], 8, 8, 64),
+])
+def test_few_rows_by_clusters_and_by_shares(cuda, wide, dtype, lqs, lens, hq, hkv, D):
+    _run(cuda, lqs, lens, hq, hkv, D, dtype, width=1250 if wide else None, causal=lqs[0] != 3)
+
+
 @pytest.mark.parametrize("dtype", [BF, FP])
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("lqs,lens,hq,hkv,D", [
@@ -178,12 +201,13 @@ def test_max_q_len_is_a_bound_and_may_be_left_out(cuda):
     assert torch.equal(a, b)
 
 
-@pytest.mark.parametrize("lq", [1, 40])
-def test_large_and_infinite_scores(cuda, lq):
+@pytest.mark.parametrize("lq,wide", [(1, False), (1, True), (40, False)])
+def test_large_and_infinite_scores(cuda, lq, wide):
     """Scores far apart (one weight is 1), masked rows of the largest finite values."""
     from reworld_b200 import paged_attention
     k, v, table, kv, g = _cache(cuda, [300], 16, 2, 128, BF, 3)
     pages = table[0].tolist()
+    table = _widen(table, wide)
     big = torch.finfo(BF).max
     k[pages[-1], 300 % 16:], v[pages[-1], 300 % 16:] = big, -big     # behind the last row
     q = (100 * torch.randn(lq, 4, 128, generator=g, device=cuda)).to(BF)
@@ -195,11 +219,14 @@ def test_large_and_infinite_scores(cuda, lq):
 
 
 @pytest.mark.parametrize("dtype,D,hq,hkv", [(BF, 128, 4, 4), (FP, 64, 6, 2), (BF, 128, 8, 1)])
-@pytest.mark.parametrize("lqs,lens", [([5, 3], [40, 200]), ([300, 17], [300, 900]), ([2, 260], [1500, 2000])])
-def test_values_of_later_tokens_that_are_not_finite(cuda, dtype, D, hq, hkv, lqs, lens):
+@pytest.mark.parametrize("lqs,lens,wide", [([5, 3], [40, 200], False), ([5, 3], [40, 200], True), ([2, 2], [700, 1900], False),
+                                           ([2, 2], [700, 1900], True), ([300, 17], [300, 900], False),
+                                           ([2, 260], [1500, 2000], False)])
+def test_values_of_later_tokens_that_are_not_finite(cuda, dtype, D, hq, hkv, lqs, lens, wide):
     """Infinities and NaN in a token's key and value reach that token and those behind it, no other."""
     from reworld_b200 import paged_attention
     k, v, table, kv, g = _cache(cuda, lens, 16, hkv, D, dtype, 12)
+    table = _widen(table, wide)
     s = _starts(cuda, lqs)
     q = torch.randn(sum(lqs), hq, D, generator=g, device=cuda).to(dtype)
     ref, lref = paged_attention(q, k, v, table, s, kv, max_q_len=max(lqs), return_lse=True)
@@ -294,6 +321,7 @@ def test_two_threads_on_one_stream(cuda):
     import threading
     from reworld_b200 import paged_attention
     k, v, table, kv, g = _cache(cuda, [3000, 2500], 16, 2, 64, BF, 14)
+    table = _widen(table, True)
     qs = [torch.randn(n, 8, 64, generator=g, device=cuda).to(BF) for n in (2, 140)]
     ss = [_starts(cuda, [1, 1]), _starts(cuda, [70, 70])]
     want = [paged_attention(q, k, v, table, s, kv, max_q_len=q.shape[0] // 2) for q, s in zip(qs, ss)]
@@ -419,11 +447,13 @@ def test_pages_behind_eight_gigabytes(cuda, lq, hkv, layout):
         assert torch.equal(torch.nan_to_num(a.float(), 77.0), torch.nan_to_num(b.float(), 77.0))
 
 
-def test_another_stream_and_two_graphs(cuda):
+@pytest.mark.parametrize("wide", [False, True])
+def test_another_stream_and_two_graphs(cuda, wide):
     """Calls on two streams at once, and two captured graphs replayed at once with new lengths."""
     from reworld_b200 import paged_attention
     lens = [3000, 4000]
     k, v, table, kv, g = _cache(cuda, lens, 16, 2, 128, BF, 5)
+    table = _widen(table, wide)
     s = _starts(cuda, [1, 1])
     qs = [torch.randn(2, 8, 128, generator=g, device=cuda).to(BF) for _ in range(2)]
     ws = [torch.zeros(2, 2, table.shape[1] * 16, device=cuda) for _ in range(2)]
@@ -460,9 +490,11 @@ def test_another_stream_and_two_graphs(cuda):
     _status_clean()
 
 
-def test_bad_pages_and_lengths_are_reported_and_stay_in_bounds(cuda):
+@pytest.mark.parametrize("wide", [False, True])
+def test_bad_pages_and_lengths_are_reported_and_stay_in_bounds(cuda, wide):
     from reworld_b200 import _native, paged_attention, paged_rotary_store
     k, v, table, kv, g = _cache(cuda, [60], 16, 2, 128, BF, 6)
+    table = _widen(table, wide)
     q = torch.randn(1, 4, 128, generator=g, device=cuda).to(BF)
     s = _starts(cuda, [1])
     for bad_table, bad_kv, bad_s in ((table + 100000, kv, s), (table - 100000, kv, s), (table, kv + 100000, s),
