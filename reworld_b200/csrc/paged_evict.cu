@@ -5,13 +5,17 @@
 // pages shared with other sequences stay whole and every row can move at once.
 //
 // select_kernel, a cluster of one to eight CTAs for a sequence and key head: finds the smallest kept sum by
-// radix selection (three passes over the sums, which stay in L2, with histograms of 11, 11
+// radix selection (three passes over the sums, which stay in registers or L2, with histograms of 11, 11
 // and 10 bits: 11 bits hold the exponent and three more, so that sums of a similar size
 // do not all meet in one counter), then numbers the kept rows with one scan for every
 // 16384 rows and writes their indices and sums.  Each CTA of the cluster has its part of
-// the rows; they add up one another's histograms and counts through distributed shared
-// memory (64 units of 32768 rows leave more than half of the SMs idle otherwise).  move_kernel copies the kept rows of k and
+// the rows; through distributed shared memory each adds up its slice of the histograms, and
+// the one whose slice has the threshold tells the others (all of them adding up all of the histograms
+// took 5 us a pass with eight CTAs).  move_kernel copies the kept rows of k and
 // v, 16 bytes a thread; it is bound by memory (a kept row is read and written once).
+//
+// 64 units of 32768 rows of 128 channels, half kept: 199 us, 1.09 GB, 5.5 TB/s; 8 units of 1000 rows: 7.2 us,
+// the chain of the selection's barriers and the second launch.
 #include "paged.cuh"
 
 namespace rw {
@@ -21,6 +25,7 @@ using paged::Pool;
 
 constexpr int BINS = 2048;
 constexpr int PER = 16;              // sums of a thread under way at once
+constexpr int MAX_CLUSTER = 8;
 
 struct Params {
   Pool pool;
@@ -81,14 +86,17 @@ __device__ __forceinline__ unsigned ld_cluster(const unsigned* p, int rank) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(p), (uint32_t)rank)) : "memory");
   return v;
 }
+__device__ __forceinline__ void st_cluster(unsigned* p, int rank, unsigned v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_shared(smem_u32(p), (uint32_t)rank)), "r"(v) : "memory");
+}
 
 template <int THREADS, bool CLUSTER>
 __global__ void __launch_bounds__(THREADS, 1) select_kernel(const __grid_constant__ Params p) {
   constexpr int WARPS = THREADS / 32, STEP = THREADS * PER, DIGITS = BINS / THREADS;
   __shared__ unsigned hist[BINS];
   __shared__ unsigned scan[WARPS];
-  __shared__ unsigned count[PER * WARPS];    // kept (low half) and tied (high half) rows of every 32
   __shared__ unsigned s_digit, s_left, s_keep, s_ties;
+  __shared__ unsigned s_slice[MAX_CLUSTER];  // counts of the CTAs' parts of the histogram
   griddep_launch_dependents();
   griddep_wait();
   const int cs = CLUSTER ? p.cs : 1, rank = CLUSTER ? blockIdx.x % cs : 0;
@@ -98,8 +106,23 @@ __global__ void __launch_bounds__(THREADS, 1) select_kernel(const __grid_constan
   int* kept = p.kept + ((long long)b * p.pool.Hkv + hk) * p.keep;
   float* ns = p.new_sums + ((long long)b * p.pool.Hkv + hk) * p.new_cap;
   const int n_new = min(kv, p.keep);
-  if (blockIdx.x == 0 && tid == 0) p.new_lens[b] = n_new;
+  // this CTA's rows [begin, end); a short part's sums are read once.  A warp has 32 * pe rows of a step, 32 at a time
+  const int part = (kv + cs - 1) / cs, begin = min(kv, rank * part), end = min(kv, begin + part);
+  const bool once = end - begin <= STEP;
+  const int pe = once ? (end - begin + THREADS - 1) / THREADS : PER;
+  const int own = warp * (32 * pe) + lane;
+  float v[PER];
+  auto fetch = [&](int i0) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int i = i0 + own + 32 * j;
+      v[j] = j < pe && i < end ? x[i] : 0.f;
+    }
+  };
+  if (once) fetch(begin);
+  if (tid == 0) s_keep = s_ties = 0;
   const int first = rank * THREADS + tid, step = cs * THREADS;
+  if (blockIdx.x == 0 && tid == 0) p.new_lens[b] = n_new;
   for (long long i = n_new + first; i < p.new_cap; i += step) ns[i] = 0.f;
   for (int i = n_new + first; i < p.keep; i += step) kept[i] = -1;
   if (kv <= p.keep) {
@@ -111,26 +134,11 @@ __global__ void __launch_bounds__(THREADS, 1) select_kernel(const __grid_constan
   }
   const int lo = min(p.n_sink, kv), hi = kv - p.n_recent;   // rows [lo, hi) compete; lo <= hi since sink + recent <= keep < kv
   const unsigned need = (unsigned)(p.keep - p.n_sink - p.n_recent);
-  // this CTA's rows [begin, end); a short part's sums are read once
-  const int per = (kv + cs - 1) / cs, begin = min(kv, rank * per), end = min(kv, begin + per);
-  const bool once = end - begin <= STEP;
-  auto sync_all = [&]() {
-    if constexpr (CLUSTER) cluster_sync(); else __syncthreads();
-  };
-  float v[PER];
-  auto fetch = [&](int i0) {
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int i = i0 + j * THREADS + tid;
-      v[j] = i < end ? x[i] : 0.f;
-    }
-  };
-  if (once) fetch(begin);
-  if (tid == 0) s_keep = s_ties = 0;
   // ---- the need-th largest sum of [lo, hi): its bits from the top
   uint32_t prefix = 0;
   unsigned left = need;                      // of the rows with this prefix
   if (need > 0) {
+    const unsigned span = (unsigned)max(0, min(hi, end) - lo);
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
       const int bits = pass < 2 ? 11 : 10, shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
@@ -140,60 +148,85 @@ __global__ void __launch_bounds__(THREADS, 1) select_kernel(const __grid_constan
         if (!once) fetch(i0);
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-          const int i = i0 + j * THREADS + tid;
-          if (i0 + j * THREADS >= end) break;
+          if (j >= pe) break;
           const uint32_t o = order_of(v[j]);
-          if (i < end && i >= lo && i < hi && (pass == 0 || (o >> (shift + bits)) == prefix))
+          if ((unsigned)(i0 + own + 32 * j - lo) < span && (pass == 0 || (o >> (shift + bits)) == prefix))
             atomicAdd(&hist[(o >> shift) & ((1u << bits) - 1u)], 1u);
         }
       }
-      sync_all();
-      // a thread has DIGITS digits, thread 0 the largest: how many rows have a larger one
-      unsigned n[DIGITS], mine = 0, all;
+      if constexpr (CLUSTER) {
+        // a CTA adds up its slice of the cluster's histograms, a thread a digit, thread 0 the largest
+        const int slice = BINS / cs;
+        cluster_sync();
+        unsigned n = 0, all;
+        const int digit = slice * (rank + 1) - 1 - tid;
+        if (tid < slice) {
+          unsigned m[MAX_CLUSTER];
 #pragma unroll
-      for (int i = 0; i < DIGITS; ++i) n[i] = hist[BINS - 1 - DIGITS * tid - i];
-      for (int c = 1; c < cs; ++c) {
+          for (int c = 0; c < MAX_CLUSTER; ++c) m[c] = c < cs ? ld_cluster(&hist[digit], c) : 0u;
 #pragma unroll
-        for (int i = 0; i < DIGITS; ++i) n[i] += ld_cluster(&hist[BINS - 1 - DIGITS * tid - i], (rank + c) % cs);
-      }
-#pragma unroll
-      for (int i = 0; i < DIGITS; ++i) mine += n[i];
-      unsigned above = block_scan<THREADS>(mine, scan, &all) - mine;
-#pragma unroll
-      for (int i = 0; i < DIGITS; ++i) {
-        if (above < left && left <= above + n[i]) {
-          s_digit = BINS - 1 - DIGITS * tid - i;
-          s_left = left - above;
+          for (int c = 0; c < MAX_CLUSTER; ++c) n += m[c];
         }
-        above += n[i];
+        const unsigned upto = block_scan<THREADS>(n, scan, &all);
+        if (tid < cs) st_cluster(&s_slice[rank], tid, all);
+        cluster_sync();
+        unsigned above = upto - n;
+        for (int c = rank + 1; c < cs; ++c) above += s_slice[c];
+        if (above < left && left <= above + n)
+          for (int c = 0; c < cs; ++c) {
+            st_cluster(&s_digit, c, (unsigned)digit);
+            st_cluster(&s_left, c, left - above);
+          }
+        cluster_sync();
+      } else {
+        __syncthreads();
+        // a thread has DIGITS digits, thread 0 the largest: how many rows have a larger one
+        unsigned n[DIGITS], mine = 0, all;
+#pragma unroll
+        for (int i = 0; i < DIGITS; ++i) mine += n[i] = hist[BINS - 1 - DIGITS * tid - i];
+        unsigned above = block_scan<THREADS>(mine, scan, &all) - mine;
+#pragma unroll
+        for (int i = 0; i < DIGITS; ++i) {
+          if (above < left && left <= above + n[i]) {
+            s_digit = BINS - 1 - DIGITS * tid - i;
+            s_left = left - above;
+          }
+          above += n[i];
+        }
+        __syncthreads();
       }
-      __syncthreads();
       prefix = (prefix << bits) | s_digit;
       left = s_left;
-      sync_all();                            // the histograms are read
+      __syncthreads();                       // (they are read)
     }
   }
-  // what a row is: 1 kept whatever the ties, 2 tied, 0 neither
-  auto kind = [&](int i, float s) {
-    if (i >= end) return 0;
-    if (i < lo || i >= hi) return 1;
-    if (need == 0) return 0;
-    const uint32_t o = order_of(s);
-    return o > prefix ? 1 : (o == prefix ? 2 : 0);
+  // What a thread's rows of a step are, two bits each: 1 kept whatever the ties, 2 tied, 0 neither.
+  unsigned code = 0;
+  auto classify = [&](int i0) {
+    code = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      if (j >= pe) break;
+      const int i = i0 + own + 32 * j;
+      const uint32_t o = order_of(v[j]);
+      unsigned is = o > prefix ? 1u : (o == prefix ? 2u : 0u);
+      if (need == 0) is = 0u;
+      if (i < lo || i >= hi) is = 1u;
+      if (i < end) code |= is << (2 * j);
+    }
+    return (unsigned)(__popc(code & 0x55555555u) | (__popc(code & 0xAAAAAAAAu) << 16));
   };
   // ---- number the kept rows: sink, recent, sums above the threshold, and the first `left` equal to it
   unsigned done_keep = 0, done_ties = 0;     // kept without the ties, ties seen, before this step
+  unsigned mine = 0;                         // kept (low half) and tied (high half) rows of the thread in the step
   if constexpr (CLUSTER) {
     // those of the CTAs before this one
     unsigned k = 0, e = 0;
     for (int i0 = begin; i0 < end; i0 += STEP) {
       if (!once) fetch(i0);
-#pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        const int is = kind(i0 + j * THREADS + tid, v[j]);
-        k += is == 1;
-        e += is == 2;
-      }
+      mine = classify(i0);
+      k += mine & 0xffffu;
+      e += mine >> 16;
     }
     k = __reduce_add_sync(0xffffffffu, k);
     e = __reduce_add_sync(0xffffffffu, e);
@@ -209,38 +242,28 @@ __global__ void __launch_bounds__(THREADS, 1) select_kernel(const __grid_constan
     }
   }
   for (int i0 = begin; i0 < end; i0 += STEP) {
-    unsigned keep_m[PER], tie_m[PER];        // of the warp's 32 rows
     if (!once) fetch(i0);
+    if (!CLUSTER || !once) mine = classify(i0);
+    // (at most 16384 rows a step: the halves do not run over)
+    const unsigned in_warp = __reduce_add_sync(0xffffffffu, mine);
+    if (lane == 0) scan[warp] = in_warp;
+    __syncthreads();
+    unsigned w = lane < WARPS ? scan[lane] : 0u;
+    const unsigned all = __reduce_add_sync(0xffffffffu, w), before = __reduce_add_sync(0xffffffffu, lane < warp ? w : 0u);
+    unsigned nk = done_keep + (before & 0xffffu), nt = done_ties + (before >> 16);
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      if (i0 + j * THREADS >= end) {
-        if (lane == 0) count[j * WARPS + warp] = 0;
-        continue;
-      }
-      const int is = kind(i0 + j * THREADS + tid, v[j]);
-      keep_m[j] = __ballot_sync(0xffffffffu, is == 1);
-      tie_m[j] = __ballot_sync(0xffffffffu, is == 2);
-      if (lane == 0) count[j * WARPS + warp] = (unsigned)__popc(keep_m[j]) | ((unsigned)__popc(tie_m[j]) << 16);
-    }
-    __syncthreads();
-    // the groups of 32 in their order (at most 16384 rows a step: the halves do not run over); exclusive sums
-    unsigned all;
-    const unsigned mine = tid < PER * WARPS ? count[tid] : 0u;
-    const unsigned upto = block_scan<THREADS>(mine, scan, &all);
-    if (tid < PER * WARPS) count[tid] = upto - mine;
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      if (i0 + j * THREADS >= end) break;
-      const unsigned before = count[j * WARPS + warp], under = (1u << lane) - 1u;
-      const unsigned nk = done_keep + (before & 0xffffu) + __popc(keep_m[j] & under);
-      const unsigned nt = done_ties + (before >> 16) + __popc(tie_m[j] & under);
-      const bool tie = (tie_m[j] >> lane) & 1u;
-      if (((keep_m[j] >> lane) & 1u) || (tie && nt < left)) {
-        const unsigned at = nk + min(nt, left);
-        kept[at] = i0 + j * THREADS + tid;
+      if (j >= pe) break;
+      const unsigned is = (code >> (2 * j)) & 3u, under = (1u << lane) - 1u;
+      const unsigned km = __ballot_sync(0xffffffffu, is & 1u), tm = __ballot_sync(0xffffffffu, is & 2u);
+      const unsigned t = nt + __popc(tm & under);
+      if ((is & 1u) || ((is & 2u) && t < left)) {
+        const unsigned at = nk + __popc(km & under) + min(t, left);
+        kept[at] = i0 + own + 32 * j;
         ns[at] = v[j];
       }
+      nk += __popc(km);
+      nt += __popc(tm);
     }
     done_keep += all & 0xffffu;
     done_ties += all >> 16;
@@ -321,18 +344,19 @@ extern "C" int rw_paged_evict(const rw_paged_t* cache, const float* sums, long l
   p.dst_table = dst_table; p.dst_stride = dst_stride; p.dst_width = dst_width;
   p.status = status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // A short row needs few threads, and barriers cost less with few (evicting from 1000 rows 10.3 us, with 1024 threads
-  // 12.9; from 4000 rows 14.7 and 16.0).  A long one gets more CTAs while SMs are idle: 8 units of
-  // 32768 rows 56.0 -> 50.0 us, of 200000 rows 223 -> 81, 64 units of 32768 rows 212.8 -> 205.3; not one that a CTA
-  // holds in its registers (16 units of 10000 rows 25.7 -> 32.2 with four).
+  // Barriers cost less with few threads, and the work on a sum less with many: 600 rows 6.7 us with 256 threads, 7.2 with
+  // 1024; 1500 rows 7.7 and 8.0; 4000 rows 11.1 and 9.7.  A long row gets a cluster while SMs are idle: 1 unit of 32768
+  // rows 25 us with one CTA, 18.9 with eight, 8 units of 16384 rows 25.8 and 24.6, but of 10000 rows 18.4 and 20.6.
+  // Clusters of more than two leave some SMs of a group of SMs unused: 16 units of 32768 rows 74.9 us with eight CTAs,
+  // some of which then wait for others to leave, 62.4 with four.
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return RW_ERR_CUDA;
   const long long cap = (long long)cache->table_width * cache->page_size, units = (long long)p.pool.Hkv * cache->B;
-  const bool few = cap <= 4096;
   p.cs = 1;
-  while (cap > 16384 && p.cs < 8 && units * p.cs * 2 <= sms && cap >= 4096ll * p.cs) p.cs *= 2;
+  while (cap > 12288 && p.cs < 8 && units * p.cs * 2 <= (p.cs == 1 ? sms : sms * 3 / 4) && cap >= 4096ll * p.cs) p.cs *= 2;
+  const bool few = p.cs == 1 && cap <= 1536;
   {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(p.pool.Hkv * p.cs, cache->B);
