@@ -24,11 +24,18 @@
 // takes out what is not finite (paged.cuh) before the MMA warp gets them.
 //
 // Work: lengths are device data, so every CTA sums the key tiles of all units itself
-// (a few microseconds' latency, no host, no extra launch).  Pairs first take whole units
-// in waves (pairs at work at the same time then share heads, and k and v come from L2),
+// (a few microseconds' latency, no host, no extra launch).  Where it ends about as early, pairs take
+// whole units, in rounds, the longest first and every other round backwards.  Otherwise they first take
+// whole units in waves (pairs at work at the same time then share heads, and k and v come from L2),
 // if the units are about equal; what does not fill a wave, or all of it if they are not,
 // is one sequence of tiles of which every pair takes an equal share, and the parts of
 // units that more than one pair worked on are joined by join_kernel.
+//
+// The weights P are rounded to the values' 16-bit type (an MMA's operands have one type); totals are
+// sums of the unrounded ones, and O is fp32 until the output's one rounding.
+//
+// 2640 tokens over 34320 rows, 24 heads of 128: 0.88 ms (1.22 PFLOP/s) in a short run, 1.02 ms when the power
+// limit holds the clock down.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -56,6 +63,11 @@ constexpr int SOFTMAX_THREADS = 256;
 constexpr int REG_SOFTMAX = 208, REG_OTHER = 88;
 static_assert(NWG * 128 * REG_SOFTMAX + 128 * REG_OTHER <= NUM_THREADS * 168, "register split exceeds the launch's");
 constexpr float RESCALE_THRESHOLD = 8.0f;    // log2 units
+// What work dealt out in equal shares costs more than whole units: the starts of parts, and their joining.  Whole units
+// against shares: 8 units of 12 tiles 25.1 and 30.6 us, of 16 tiles 28.2 and 31.4, of 32 tiles 39.9 and 36.1 (74 pairs); 64
+// units of 35 tiles 46.5 and 56.5; head dim 64 (148 CTAs) 4 units of 8 tiles 20.3 and 22.2, of 20 tiles 26.9 and 23.8; 344
+// units of 1 to 12 tiles 41.8 and 51.2.
+template <int D> constexpr int JOIN_COST = D == 128 ? 17 : 13;
 constexpr int MIN_SHARE = 12;                // cost of a share, where there is little work
 // What a unit costs beside its key tiles, in tiles: filling and draining the pipeline (q and the first keys, the last
 // softmax, the output) takes 5 to 8 us, a tile 0.75 to 0.9.  4 ragged chunks of up to 701 tokens 140.5 us dealt out with
@@ -244,6 +256,55 @@ __device__ __forceinline__ Walk walk_to_unit(const Params& p, const Plan& pl, in
   w.n = tiles_of(p, w.s, w.rt, upt, &w.keys);
   return w;
 }
+// Row tiles of a sequence with at most n key tiles: they are its first ones.
+__device__ __forceinline__ int tiles_upto(const Params& p, const Seq& s, int nu, int n, int upt) {
+  if (n < 1) return 0;
+  if (s.kv <= (long long)n * BN) return nu;
+  return p.causal ? paged::clampi((int)((long long)n * BN - (s.kv - s.lq)) / upt, 0, nu) : 0;
+}
+// The units ordered by their key tiles, the longest first: lane b's sequence has the row tiles [from, upto) of n key
+// tiles, and `before` units are longer.
+struct Ranks {
+  Seq s;
+  int nu, n, from, upto, before;
+};
+__device__ __forceinline__ Ranks ranks(const Params& p, int longest, int upt, int lane) {
+  Ranks k{};
+  if (lane < p.pool.B) {
+    k.s = paged::load_seq(p.pool, lane, p.T, nullptr);
+    k.nu = units_of(p, k.s, upt);
+  }
+  k.n = longest;
+  k.upto = k.nu;
+  k.from = tiles_upto(p, k.s, k.nu, longest - 1, upt);
+  return k;
+}
+// Whole warp: the unit with index u in that order, no smaller than in the last call.
+__device__ __forceinline__ Walk walk_to_rank(const Params& p, Ranks& k, int u, int upt, int lane) {
+  for (int all; k.n > 1 && u >= k.before + (all = p.pool.Hkv * __reduce_add_sync(0xffffffffu, k.upto - k.from));) {
+    k.before += all;
+    --k.n;
+    k.upto = k.from;
+    k.from = tiles_upto(p, k.s, k.nu, k.n - 1, upt);
+  }
+  const int count = k.upto - k.from;
+  int x = count * p.pool.Hkv;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  const int f = __ffs(__ballot_sync(0xffffffffu, k.before + x > u)) - 1;
+  const int r = u - k.before - __shfl_sync(0xffffffffu, x - count * p.pool.Hkv, f);
+  const int each = __shfl_sync(0xffffffffu, count, f);
+  Walk w;
+  w.b = f;
+  enter(p, w, upt);
+  w.hk = r / each;
+  w.rt = __shfl_sync(0xffffffffu, k.from, f) + r - w.hk * each;
+  w.n = tiles_of(p, w.s, w.rt, upt, &w.keys);
+  return w;
+}
 // Whole warp: cost of the units before that one.
 __device__ __forceinline__ long long cost_before(const Params& p, const Plan& pl, const Walk& w, int upt, int lane) {
   long long sum = 0, all = paged::div_count(pl.cost[w.b + 1] - pl.cost[w.b], p.pool.Hkv);
@@ -382,10 +443,20 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   long long t = 0, t1 = 0, before = 0, t_base = 0, share = 1;  // pair c has [t_base + c share, t_base + (c + 1) share)
   int waves = 0, wave = 0, C = p.C;
   Walk wk{};
-  bool in_tail = false;
+  Ranks rk{};
+  bool in_tail = false, whole = false, sorted = false;
   auto plan_next = [&](int i) {
     Seg s{};
-    if (wave < waves) {
+    if (whole) {
+      // every other wave backwards: who has had a long unit gets a short one
+      const int u = wave * C + ((wave & 1) ? C - 1 - pid : pid);
+      if (wave < waves && u < pl.units[p.pool.B]) {
+        wk = sorted ? walk_to_rank(p, rk, u, upt, lane) : walk_to_unit(p, pl, u, upt);
+        ++wave;
+        s.n = wk.n;
+        s.slot = -1;
+      }
+    } else if (wave < waves) {
       wk = walk_to_unit(p, pl, wave * C + pid, upt);
       ++wave;
       s.n = wk.n;
@@ -433,11 +504,25 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const long long U = plan_sum(p, pl, lane);
     const long long N = pl.cost[p.pool.B];       // of all work
     if (even && lane == 0) p.header[pid] = make_int4(0, 0, 0, 0);
-    if (N < (long long)C * MIN_SHARE)
+    // about equal: no unit is over 1/8 longer than their mean
+    const bool equal = (long long)pl.longest * U * 8 <= N * 9;
+    int rounds = 1;
+    if (U > 0 && U <= 0x7fffffffll) {
+      if (U > C) rounds = ((unsigned)U + C - 1) / (unsigned)C;
+      const float all = (float)N;            // (estimates: no division of integers for them)
+      whole = fmaxf((float)pl.longest, rounds * __fdividef(all, (float)U)) <=
+              fmaxf((float)MIN_SHARE, __fdividef(all, (float)C)) + JOIN_COST<D>;
+      sorted = rounds > 1 && !equal && p.pool.B <= 32;
+      if (sorted) rk = ranks(p, pl.longest - UNIT_COST, upt, lane);
+    }
+    if (whole)
+      C = (int)min((long long)C, U);
+    else if (N < (long long)C * MIN_SHARE)
       C = (int)min((long long)C, max(U, paged::div_count(N + MIN_SHARE - 1, MIN_SHARE)));
-    if (pid < C && U <= 0x7fffffffll) {
-      // about equal: no unit is over 1/8 longer than their mean
-      if ((long long)pl.longest * U * 8 <= N * 9) waves = (int)paged::div_count(U, C);
+    if (whole) {
+      if (pid < C) waves = rounds;
+    } else if (pid < C && U <= 0x7fffffffll) {
+      if (equal) waves = (int)paged::div_count(U, C);
       if (waves > 0 && waves * C < U) {
         const Walk f = walk_to_unit(p, pl, waves * C, upt);
         t_base = cost_before(p, pl, f, upt, lane);

@@ -345,8 +345,8 @@ extern "C" int rw_paged_evict(const rw_paged_t* cache, const float* sums, long l
   p.status = status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // Barriers cost less with few threads, and the work on a sum less with many: 600 rows 6.7 us with 256 threads, 7.2 with
-  // 1024; 1500 rows 7.7 and 8.0; 4000 rows 11.1 and 9.7.  A long row gets a cluster while SMs are idle: 1 unit of 32768
-  // rows 25 us with one CTA, 18.9 with eight, 8 units of 16384 rows 25.8 and 24.6, but of 10000 rows 18.4 and 20.6.
+  // 1024; 1500 rows 7.7 and 8.0; 4000 rows 11.1 and 9.7.  A long row gets a cluster while SMs are idle: 1 unit of 16384
+  // rows 17.9 us with one CTA, 16.4 with eight, 8 units 25.8 and 24.6, but of 10000 rows 18.4 and 20.6.
   // Clusters of more than two leave some SMs of a group of SMs unused: 16 units of 32768 rows 74.9 us with eight CTAs,
   // some of which then wait for others to leave, 62.4 with four.
   int dev = 0, sms = 0;

@@ -180,6 +180,18 @@ def test_chunks_pages_and_layouts(cuda, page, layout):
     _run(cuda, [150, 31], [333, 500], 4, 2, 128, BF, page=page, layout=layout)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lqs,lens,hq,hkv,D,dtype", [
+    ([1501, 900, 0, 300], [1501, 900, 70, 300], 12, 4, 64, FP),    # more units than CTAs, of many lengths
+    ([1300, 700, 90], [1500, 600, 2000], 16, 16, 128, BF),         # (rows that see nothing among them)
+    ([300, 20, 150], [2000, 1500, 900], 32, 8, 128, BF),
+    ([600], [1000], 32, 8, 128, BF),                               # of about one length
+    ([150 + 20 * (i % 5) for i in range(35)], [400 + 90 * (i % 7) for i in range(35)], 6, 2, 128, FP),
+])
+def test_chunks_by_whole_units(cuda, causal, lqs, lens, hq, hkv, D, dtype):
+    _run(cuda, lqs, lens, hq, hkv, D, dtype, causal=causal)
+
+
 def test_chunks_of_many_sequences(cuda):
     _run(cuda, [(i % 3) + 3 for i in range(1100)], [(13 * i) % 90 + 5 for i in range(1100)], 4, 1, 64, BF, max_q=5)
 
