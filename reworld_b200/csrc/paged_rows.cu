@@ -101,12 +101,13 @@ struct Entry {
   int keys;   // keys that any of the rows sees
 };
 
-__device__ __forceinline__ Entry load_entry(const Params& p, int b, int* status) {
+// (of the rows from row0 on, 16 at most)
+__device__ __forceinline__ Entry load_entry(const Params& p, int b, int* status, int row0 = 0) {
   Entry n;
   n.s = paged::load_seq(p.pool, b, p.T, status);
-  n.rows = (int)min((long long)p.rows_most, (long long)n.s.lq * p.G);
+  n.rows = max(0, min(RT, (int)min((long long)p.rows_most, (long long)n.s.lq * p.G) - row0));
   n.keys = 0;
-  if (n.rows > 0) n.keys = p.causal ? max(0, n.s.kv - n.s.lq + (n.rows - 1) / p.G + 1) : n.s.kv;
+  if (n.rows > 0) n.keys = p.causal ? max(0, n.s.kv - n.s.lq + (row0 + n.rows - 1) / p.G + 1) : n.s.kv;
   return n;
 }
 
@@ -117,9 +118,9 @@ struct Seg {
   long long u0;
 };
 
-// Keys that every row sees: tiles behind them are looked through for values that are not finite.
-__device__ __forceinline__ int keys_of_all(const Params& p, const Entry& n) {
-  return p.causal ? min(n.keys, max(0, n.s.kv - n.s.lq + 1)) : n.keys;
+// Keys that every row from row0 on sees: tiles behind them are looked through for values that are not finite.
+__device__ __forceinline__ int keys_of_all(const Params& p, const Entry& n, int row0) {
+  return p.causal ? min(n.keys, max(0, n.s.kv - n.s.lq + row0 / p.G + 1)) : n.keys;
 }
 
 // Tiles of an entry: at least one while it has rows, so that rows that see nothing are written too.
@@ -183,19 +184,21 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
 
   const int cta = blockIdx.x;
   const int rank = CLUSTER ? cta % p.cs : 0;
+  int row0 = 0;         // CLUSTER: the unit's first row
   long long share = 1, t1 = 0;
   if constexpr (CLUSTER) {
-    const int unit = cta / p.cs;
+    const int head = cta / p.cs;
+    row0 = RT * blockIdx.y;
     Seg s;
-    s.b = unit / p.pool.Hkv;
-    s.hk = unit - s.b * p.pool.Hkv;
-    s.en = load_entry(p, s.b, cta % (p.cs * p.pool.Hkv) == 0 && tid == 0 ? p.status : nullptr);
+    s.b = head / p.pool.Hkv;
+    s.hk = head - s.b * p.pool.Hkv;
+    s.en = load_entry(p, s.b, blockIdx.y == 0 && cta % (p.cs * p.pool.Hkv) == 0 && tid == 0 ? p.status : nullptr, row0);
     if (s.en.rows == 0) return;              // (with the whole cluster)
     s.n_tiles = tiles_of(s.en);
     const int per = (s.n_tiles + p.cs - 1) / p.cs;
     s.k0 = min(rank * per, s.n_tiles);
     s.n = min(per, s.n_tiles - s.k0);
-    s.all = keys_of_all(p, s.en);
+    s.all = keys_of_all(p, s.en, row0);
     s.u0 = 0;
     if (tid == 0) {
       seg[0] = s;
@@ -247,7 +250,7 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
       s.u0 = plan.ebase + (long long)s.hk * s.n_tiles;
       s.k0 = (int)(plan.t - s.u0);
       s.n = (int)(min(t1, s.u0 + s.n_tiles) - plan.t);
-      s.all = keys_of_all(p, s.en);
+      s.all = keys_of_all(p, s.en, 0);
       plan.t += s.n;
     }
     seg[i & 1] = s;
@@ -316,9 +319,9 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
     int lim[2];          // keys that the thread's two rows see
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int r = grp + 8 * i;
+      const int r = row0 + grp + 8 * i;
       const int tok = r / p.G, g = r - tok * p.G;
-      const bool there = r < en.rows;
+      const bool there = grp + 8 * i < en.rows;
       lim[i] = there ? (p.causal ? max(0, s.kv - s.lq + tok + 1) : s.kv) : 0;
       const uint8_t* src = p.q + (long long)(s.s0 + tok) * p.q_sl + (long long)(hk * p.G + g) * p.q_sh;
 #pragma unroll
@@ -490,7 +493,7 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
       p.header[(long long)b * p.pool.Hkv + hk] = make_int2(my_slot, parts);
     }
     float* slot = CLUSTER ? reinterpret_cast<float*>(smem + STAGE) : p.part + (long long)my_slot * SLOT;
-    auto put = [&](int r, int c, float2 v, float mm, float ll) { put_row<HALF>(p, en, b, hk, r, c, v, mm, ll); };
+    auto put = [&](int r, int c, float2 v, float mm, float ll) { put_row<HALF>(p, en, b, hk, row0 + r, c, v, mm, ll); };
     // 2 channels of a row a thread and step
     for (int i = tid; i < en.rows * (D / 2); i += THREADS) {
       const int r = i / (D / 2), c = 2 * (i % (D / 2));
@@ -510,7 +513,7 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
       }
       if (dirty) {
         // taken-out values go to the rows that see them
-        const int lim = p.causal ? max(0, s.kv - s.lq + r / p.G + 1) : s.kv;
+        const int lim = p.causal ? max(0, s.kv - s.lq + (row0 + r) / p.G + 1) : s.kv;
         paged::for_nonfinite<HALF>(p.pool, b, hk, max(all / TILE, k0) * TILE, min(lim, (k0 + n) * TILE), c, 2,
                                    [&](int ch, float x) { (ch == c ? v.x : v.y) += x; });
       }
@@ -808,20 +811,32 @@ inline Layout layout(int D, int C, int B, int Hkv, long long rows, long long cap
 // rows 14.9 and 19.2; 32 ragged sequences x 8 heads, up to 500 rows 15.4 and 26.5, up to 1000 rows 23.9 and 31.9; 128
 // of them 68.8 and 79.5, with equal lengths 104 and 98.  With weights: 8 heads, 500 rows 7.2 and 17.2, 8000 rows 17.9
 // and 21.3, 16000 rows 27.7 and 26.9.
+//
+// More than 16 rows are so many blocks of 16, which read the keys from L2 at the same time: while all CTAs are
+// resident that is over before the tiles of chunk_kernel have filled their pipeline.  A tile takes a CTA 0.9 us, with two
+// CTAs on an SM 1.6.  By blocks and by chunk_kernel, us: 8 heads x 20 rows over 505 keys 8.7 and 18.1, over 6005 20.3 and
+// 38.9; x 64 rows over 516 keys 9.9 and 19.3; x 256 rows over 564 keys 15.2 and 20.0, over 2064 (2 CTAs an SM, 17 tiles
+// each) 28.3 and 29.2; x 512 rows over 628 keys (10 tiles) 23.7 and 20.1.  Their weights would meet in one key's sum
+// in no fixed order: with weights they are chunk_kernel's.
 struct Clusters {
   int cs, pitch, bytes;
 };
-inline Clusters clusters_for(int D, long long units, long long rows, long long cap, bool sums) {
-  const long long tiles = std::max(1ll, (cap + TILE - 1) / TILE);
-  const int all = grid_size(D), sm = D == 128 ? 2 : 4;
+inline Clusters clusters_for(int D, long long heads, long long rows, long long cap, bool sums) {
+  const long long tiles = std::max(1ll, (cap + TILE - 1) / TILE), blocks = (rows + RT - 1) / RT, units = heads * blocks;
+  const int all = grid_size(D), sm = D == 128 ? 2 : 4, half = 128 / D;
+  if (units >= (1 << 30) || (blocks > 1 && (sums || units > all))) return {0, 0, 0};
   for (int cs = MAX_CLUSTER; cs >= 1; cs /= 2) {
     const long long per = (tiles + cs - 1) / cs;
-    if (per > CLUSTER_TILES) break;
     const long long bytes = STAGES * 4 * TILE * D + (sums ? 4 * rows * per * TILE : 0);
-    // as many CTAs as are resident together, by shared memory (4 KB of it is static, or the system's)
-    const long long most = std::min((long long)sm, (220 << 10) / (bytes + 4096)) * (all / sm);
-    if (cs > 1 && (cs / 2 >= tiles || units * cs > most)) continue;
-    if (per <= 1024 / D + units * tiles / all && units < (1 << 30)) return {cs, (int)per * TILE, (int)bytes};
+    // as many CTAs as are resident together, by shared memory (4 KB of it is static, or the system's); not all
+    // clusters of 16 fit that the SMs would hold (16 of them, two CTAs an SM, took two rounds)
+    const long long fit = std::min((long long)sm, (220 << 10) / (bytes + 4096)) * (all / sm);
+    if (cs > 1 && (cs / 2 >= tiles || per > CLUSTER_TILES * (sums ? 1 : 4) || units * cs > (cs > 8 ? fit * 3 / 4 : fit)))
+      continue;
+    long long most;
+    if (blocks > 1) most = half * (units * cs * 2 > all ? std::min(20, 8 * cs) : 20);
+    else most = std::min((long long)CLUSTER_TILES, half * 8 + units * tiles / all);
+    if (per <= most) return {cs, (int)per * TILE, (int)bytes};
     break;
   }
   return {0, 0, 0};
@@ -834,7 +849,7 @@ int launch_cluster(const Params& p, int bytes, cudaStream_t stream) {
   const void* kernel = reinterpret_cast<const void*>(rows_kernel<HALF, D, true>);
   if (!ensure_smem_attr(kernel, MOST, &done) || !ensure_cluster_attr(kernel, &done_size)) return RW_ERR_CUDA;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(p.pool.B * p.pool.Hkv * p.cs));
+  cfg.gridDim = dim3((unsigned)(p.pool.B * p.pool.Hkv * p.cs), (unsigned)((p.rows_most + RT - 1) / RT));
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = stream;
@@ -947,8 +962,10 @@ extern "C" int rw_paged_attn(const rw_paged_t* cache, const void* q, void* out, 
   const chunk::Call c{q, out, lse, nullptr, T, Hq, longest, causal != 0, q_sl, q_sh, o_sl, o_sh,
                       softmax_scale * 1.4426950408889634f, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return rows::few_rows(rows)
-             ? rows::run_rows(cache, pool, c, rows, sums, sums_sb, sums_sh, workspace, workspace_bytes, st)
+  const bool few = rows::few_rows(rows) ||
+                   rows::clusters_for(cache->D, (long long)cache->B * pool.Hkv, rows,
+                                      (long long)cache->table_width * cache->page_size, sums != nullptr).cs != 0;
+  return few ? rows::run_rows(cache, pool, c, rows, sums, sums_sb, sums_sh, workspace, workspace_bytes, st)
              : rows::run_tiles(cache, pool, c, sums, sums_sb, sums_sh, workspace, workspace_bytes, st);
 }
 
@@ -958,7 +975,7 @@ extern "C" long long rw_paged_attn_workspace_bytes(int T, int Hq, int Hkv, int D
   if (T < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || B < 1 || max_q_len < 1 || (D != 64 && D != 128) || cache_rows < 0)
     return 0;
   const long long rows = (long long)std::min(max_q_len, T) * (Hq / Hkv);
-  if (rows::few_rows(rows) && rows::clusters_for(D, (long long)B * Hkv, rows, cache_rows, with_sums != 0).cs) return 0;
+  if (rows::clusters_for(D, (long long)B * Hkv, rows, cache_rows, with_sums != 0).cs) return 0;
   if (rows::few_rows(rows)) return rows::layout(D, rows::grid_size(D), B, Hkv, rows, cache_rows, with_sums != 0).total;
   return chunk::workspace_bytes(D) + (with_sums ? 4LL * T * Hq : 0);
 }

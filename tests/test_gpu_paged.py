@@ -181,6 +181,19 @@ def test_chunks_pages_and_layouts(cuda, page, layout):
 
 
 @pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("lqs,lens,hq,hkv,D", [
+    ([17], [1000], 1, 1, 64),
+    ([64], [2000], 8, 8, 128),                           # four blocks of rows, several CTAs each
+    ([40, 0, 7, 100], [600, 30, 3, 350], 6, 2, 128),
+    ([33, 5], [6000, 100], 4, 2, 64),
+    ([9], [130], 40, 2, 128),                            # blocks that end inside a token's heads
+])
+def test_chunks_by_blocks_and_by_tiles(cuda, causal, wide, lqs, lens, hq, hkv, D):
+    _run(cuda, lqs, lens, hq, hkv, D, BF, causal=causal, width=1250 if wide else None, sums=not wide)
+
+
+@pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("lqs,lens,hq,hkv,D,dtype", [
     ([1501, 900, 0, 300], [1501, 900, 70, 300], 12, 4, 64, FP),    # more units than CTAs, of many lengths
     ([1300, 700, 90], [1500, 600, 2000], 16, 16, 128, BF),         # (rows that see nothing among them)
@@ -213,7 +226,7 @@ def test_max_q_len_is_a_bound_and_may_be_left_out(cuda):
     assert torch.equal(a, b)
 
 
-@pytest.mark.parametrize("lq,wide", [(1, False), (1, True), (40, False)])
+@pytest.mark.parametrize("lq,wide", [(1, False), (1, True), (40, False), (40, True)])
 def test_large_and_infinite_scores(cuda, lq, wide):
     """Scores far apart (one weight is 1), masked rows of the largest finite values."""
     from reworld_b200 import paged_attention
@@ -233,7 +246,8 @@ def test_large_and_infinite_scores(cuda, lq, wide):
 @pytest.mark.parametrize("dtype,D,hq,hkv", [(BF, 128, 4, 4), (FP, 64, 6, 2), (BF, 128, 8, 1)])
 @pytest.mark.parametrize("lqs,lens,wide", [([5, 3], [40, 200], False), ([5, 3], [40, 200], True), ([2, 2], [700, 1900], False),
                                            ([2, 2], [700, 1900], True), ([300, 17], [300, 900], False),
-                                           ([2, 260], [1500, 2000], False)])
+                                           ([300, 17], [300, 900], True), ([2, 260], [1500, 2000], False),
+                                           ([2, 260], [1500, 2000], True)])
 def test_values_of_later_tokens_that_are_not_finite(cuda, dtype, D, hq, hkv, lqs, lens, wide):
     """Infinities and NaN in a token's key and value reach that token and those behind it, no other."""
     from reworld_b200 import paged_attention
