@@ -1,6 +1,6 @@
 // Attention of few new tokens over a paged cache: o = softmax(q k^T * scale) v for the
-// rows of a sequence that share a key head (tokens x heads of the group), 16 at most, with
-// the keys split over the whole device.
+// rows of a sequence that share a key head (tokens x heads of the group), 16 at most (over
+// short tables blocks of 16), with the keys split over the whole device.
 //
 // Such a call is bound by memory: every cached row of k and v is read once for 4 * 16
 // products an element at most.  What decides is that all SMs read all the time, however
@@ -26,6 +26,9 @@
 // Keys and values come through a ring of 3 stages
 // of 16-byte cp.async; rows behind the last visible one are filled with zeros, never
 // read, so what a page holds there (NaN included) does not matter.
+//
+// 32 tokens over up to 8191 rows (ragged), 8 key heads of 128: 105 us, 5.7 TB/s, start and join included; 2 tokens over
+// up to 131072 rows, 2 key heads: 48.6 us, 5.0 TB/s; 1 token over 511 rows, by clusters: 5.1 us.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -608,9 +611,8 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
 
 // Joins the parts of the units that more than one CTA worked on: a block takes one row of
 // one unit, its 8 groups of D / 4 threads every eighth part each.  (Joined by the last CTA
-// that comes to a unit instead, without another launch, single-token calls were slower
-// throughout: one of 511 rows 13.3 us against 9.2, 32 of 2000 rows 54.3 and 54.0, 2 of
-// 131072 rows 86 and 74.)
+// that comes to a unit instead, without another launch, calls were slower
+// throughout: 32 tokens of 2000 rows 54.3 us and 54.0, 2 of 131072 rows 86 and 74.)
 constexpr int JOIN_GROUPS = 8;
 constexpr int MAX_PARTS = 1024;  // CTAs of a launch: checked by the host
 

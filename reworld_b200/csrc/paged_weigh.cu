@@ -13,7 +13,10 @@
 // shared memory while the rows' tiles pass by.  Rows are packed as in paged_chunk.cu
 // (token * G + head).  Four warpgroups take 32 columns each.  Bound by the exponentials
 // (128 x 128 of them against 128 x 128 x D products): the S buffers, four, keep the
-// tensor pipe ahead.
+// tensor pipe ahead.  (A share of the exponentials on the FMA pipe, or the next tile's scores fetched into registers
+// ahead, made it 1 and 10 % slower.)
+//
+// 880 tokens over 13200 rows, 24 heads of 128: 109 us of the call's 250 to 290, the exponentials' unit 71 % busy.
 #include "paged_chunk.h"
 #include "paged_tiles.cuh"
 
