@@ -785,7 +785,7 @@ inline int grid_size(int D) {
 }
 
 // Which kernel: 16 rows of a sequence and key head are all that rows_kernel can use of a
-// key tile it has read; where there may be more, the tiles of chunk_kernel.
+// key tile it has read; where there may be more, the tiles of chunk_kernel, or blocks of 16 (clusters_for).
 inline bool few_rows(long long rows) { return rows <= RT; }
 
 struct Layout {
@@ -826,7 +826,7 @@ struct Clusters {
 inline Clusters clusters_for(int D, long long heads, long long rows, long long cap, bool sums) {
   const long long tiles = std::max(1ll, (cap + TILE - 1) / TILE), blocks = (rows + RT - 1) / RT, units = heads * blocks;
   const int all = grid_size(D), sm = D == 128 ? 2 : 4, half = 128 / D;
-  if (units >= (1 << 30) || (blocks > 1 && (sums || units > all))) return {0, 0, 0};
+  if (all == 0 || units >= (1 << 30) || (blocks > 1 && (sums || units > all))) return {0, 0, 0};
   for (int cs = MAX_CLUSTER; cs >= 1; cs /= 2) {
     const long long per = (tiles + cs - 1) / cs;
     const long long bytes = STAGES * 4 * TILE * D + (sums ? 4 * rows * per * TILE : 0);
