@@ -65,6 +65,7 @@ struct Params {
   float* sums;
   long long sums_sb, sums_sh;
   long long cap;
+  float* block_sums;            // [blocks of 16 rows][B * Hkv][cap]: what each block adds, if there are several
   int* status;
 };
 
@@ -532,12 +533,15 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
     }
     if constexpr (CLUSTER) {
       constexpr int KEYS = CLUSTER_TILES * TILE / THREADS;   // of a thread, whose sums are read meanwhile
-      float* dst = p.sums + b * p.sums_sb + hk * p.sums_sh + k0 * TILE + tid;
+      float* dst = nullptr;
       const int keys = min(n * TILE, en.keys - k0 * TILE) - tid;
       float old[KEYS];
       if (p.sums) {
+        dst = p.sums + b * p.sums_sb + hk * p.sums_sh;
+        if (p.block_sums) dst = p.block_sums + (((long long)blockIdx.y * p.pool.B + b) * p.pool.Hkv + hk) * p.cap;
+        dst += k0 * TILE + tid;
 #pragma unroll
-        for (int i = 0; i < KEYS; ++i) old[i] = i * THREADS < keys ? dst[i * THREADS] : 0.f;
+        for (int i = 0; i < KEYS; ++i) old[i] = !p.block_sums && i * THREADS < keys ? dst[i * THREADS] : 0.f;
       }
       cluster_sync();
       auto part = [&](int i, int at) { return mapa_shared(sbase + STAGE + 4 * at, (uint32_t)i); };
@@ -607,6 +611,29 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
     __syncthreads();                         // the warps' states are read
     if (tid == 0) dirty = 0;
   }
+}
+
+// sums[b, hk, j] += what the blocks of rows added up, in their order.
+constexpr int ADD_THREADS = 128;
+__global__ void __launch_bounds__(ADD_THREADS) add_blocks_kernel(const __grid_constant__ Params p) {
+  griddep_launch_dependents();
+  griddep_wait();
+  const int head = blockIdx.y, b = head / p.pool.Hkv, j = blockIdx.x * ADD_THREADS + threadIdx.x;
+  const Seq s = paged::load_seq(p.pool, b, p.T, nullptr);
+  const long long rows = min((long long)p.rows_most, (long long)s.lq * p.G), step = (long long)p.pool.B * p.pool.Hkv * p.cap;
+  const float* src = p.block_sums + head * p.cap + j;
+  float add = 0.f;
+  for (int r0 = 0; r0 < rows; r0 += 16 * RT) {
+    float x[16];                             // all under way at once
+#pragma unroll
+    for (int i = 0; i < 16; ++i, src += step) {
+      const int first = r0 + i * RT, last = (int)min(rows, (long long)first + RT) - 1;
+      x[i] = first < rows && j < (p.causal ? s.kv - s.lq + last / p.G + 1 : s.kv) ? __ldcg(src) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) add += x[i];
+  }
+  if (j < s.kv && rows > 0) p.sums[b * p.sums_sb + (head - b * p.pool.Hkv) * p.sums_sh + j] += add;
 }
 
 // Joins the parts of the units that more than one CTA worked on: a block takes one row of
@@ -818,18 +845,19 @@ inline Layout layout(int D, int C, int B, int Hkv, long long rows, long long cap
 // resident that is over before the tiles of chunk_kernel have filled their pipeline.  A tile takes a CTA 0.9 us, with two
 // CTAs on an SM 1.6.  By blocks and by chunk_kernel, us: 8 heads x 20 rows over 505 keys 8.7 and 18.1, over 6005 20.3 and
 // 38.9; x 64 rows over 516 keys 9.9 and 19.3; x 256 rows over 564 keys 15.2 and 20.0, over 2064 (2 CTAs an SM, 17 tiles
-// each) 28.3 and 29.2; x 512 rows over 628 keys (10 tiles) 23.7 and 20.1.  Their weights would meet in one key's sum
-// in no fixed order: with weights they are chunk_kernel's.
+// each) 28.3 and 29.2; x 512 rows over 628 keys (10 tiles) 23.7 and 20.1. 
+// What each block adds to the sums goes to scratch; add_blocks_kernel adds it up in the blocks' order: 8 heads x 64 rows
+// over 516 keys with weights 13.6 us, by chunk_kernel and weigh_kernel 25.5; x 256 rows 25.2 and 27.4.
 struct Clusters {
   int cs, pitch, bytes;
 };
 inline Clusters clusters_for(int D, long long heads, long long rows, long long cap, bool sums) {
   const long long tiles = std::max(1ll, (cap + TILE - 1) / TILE), blocks = (rows + RT - 1) / RT, units = heads * blocks;
   const int all = grid_size(D), sm = D == 128 ? 2 : 4, half = 128 / D;
-  if (all == 0 || units >= (1 << 30) || (blocks > 1 && (sums || units > all))) return {0, 0, 0};
+  if (all == 0 || units >= (1 << 30)) return {0, 0, 0};
   for (int cs = MAX_CLUSTER; cs >= 1; cs /= 2) {
     const long long per = (tiles + cs - 1) / cs;
-    const long long bytes = STAGES * 4 * TILE * D + (sums ? 4 * rows * per * TILE : 0);
+    const long long bytes = STAGES * 4 * TILE * D + (sums ? 4 * std::min(rows, (long long)RT) * per * TILE : 0);
     // as many CTAs as are resident together, by shared memory (4 KB of it is static, or the system's); not all
     // clusters of 16 fit that the SMs would hold (16 of them, two CTAs an SM, took two rounds)
     const long long fit = std::min((long long)sm, (220 << 10) / (bytes + 4096)) * (all / sm);
@@ -838,10 +866,15 @@ inline Clusters clusters_for(int D, long long heads, long long rows, long long c
     long long most;
     if (blocks > 1) most = half * (units * cs * 2 > all ? std::min(20, 8 * cs) : 20);
     else most = std::min((long long)CLUSTER_TILES, half * 8 + units * tiles / all);
+    if (sums) most = std::min(most, (long long)CLUSTER_TILES);
+    if (blocks > 1 && units > fit) break;    // (with weights, 256 units of 6 tiles 40 us, by chunk_kernel 27)
     if (per <= most) return {cs, (int)per * TILE, (int)bytes};
     break;
   }
   return {0, 0, 0};
+}
+inline long long block_sums_bytes(long long heads, long long rows, long long cap, bool sums) {
+  return sums && rows > RT ? 4 * ((rows + RT - 1) / RT) * heads * cap : 0;
 }
 
 template <bool HALF, int D>
@@ -864,7 +897,10 @@ int launch_cluster(const Params& p, int bytes, cudaStream_t stream) {
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, rows_kernel<HALF, D, true>, p) == cudaSuccess ? RW_OK : RW_ERR_CUDA;
+  if (cudaLaunchKernelEx(&cfg, rows_kernel<HALF, D, true>, p) != cudaSuccess) return RW_ERR_CUDA;
+  if (!p.block_sums) return RW_OK;
+  return launch_dependent(add_blocks_kernel, dim3((unsigned)((p.cap + ADD_THREADS - 1) / ADD_THREADS), p.pool.B * p.pool.Hkv),
+                          dim3(ADD_THREADS), 0, stream, p) == cudaSuccess ? RW_OK : RW_ERR_CUDA;
 }
 
 template <bool HALF, int D>
@@ -888,6 +924,8 @@ int run_rows(const rw_paged_t* cache, const Pool& pool, const chunk::Call& c, lo
   if (C == 0 || C > MAX_PARTS) return RW_ERR_CUDA;
   const Clusters cl = clusters_for(cache->D, (long long)cache->B * pool.Hkv, rows, cap, sums != nullptr);
   if (cap == 0) sums = nullptr;
+  const long long need = cl.cs ? block_sums_bytes((long long)cache->B * pool.Hkv, rows, cap, sums != nullptr) : 0;
+  if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return RW_ERR_INVALID_ARG;
   const Layout lay = layout(cache->D, C, cache->B, pool.Hkv, rows, cap, sums != nullptr);
   if (cl.cs == 0 && (!workspace || !aligned16(workspace) || workspace_bytes < lay.total)) return RW_ERR_INVALID_ARG;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -902,6 +940,7 @@ int run_rows(const rw_paged_t* cache, const Pool& pool, const chunk::Call& c, lo
   p.cs = cl.cs;
   p.pitch = cl.pitch;
   p.scale_log2 = c.scale_log2;
+  if (need) p.block_sums = static_cast<float*>(workspace);
   if (cl.cs == 0) {
     p.part = reinterpret_cast<float*>(ws + lay.part);
     p.header = reinterpret_cast<int2*>(ws + lay.header);
@@ -977,7 +1016,8 @@ extern "C" long long rw_paged_attn_workspace_bytes(int T, int Hq, int Hkv, int D
   if (T < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || B < 1 || max_q_len < 1 || (D != 64 && D != 128) || cache_rows < 0)
     return 0;
   const long long rows = (long long)std::min(max_q_len, T) * (Hq / Hkv);
-  if (rows::clusters_for(D, (long long)B * Hkv, rows, cache_rows, with_sums != 0).cs) return 0;
+  if (rows::clusters_for(D, (long long)B * Hkv, rows, cache_rows, with_sums != 0).cs)
+    return rows::block_sums_bytes((long long)B * Hkv, rows, cache_rows, with_sums != 0);
   if (rows::few_rows(rows)) return rows::layout(D, rows::grid_size(D), B, Hkv, rows, cache_rows, with_sums != 0).total;
   return chunk::workspace_bytes(D) + (with_sums ? 4LL * T * Hq : 0);
 }

@@ -190,7 +190,7 @@ def test_chunks_pages_and_layouts(cuda, page, layout):
     ([9], [130], 40, 2, 128),                            # blocks that end inside a token's heads
 ])
 def test_chunks_by_blocks_and_by_tiles(cuda, causal, wide, lqs, lens, hq, hkv, D):
-    _run(cuda, lqs, lens, hq, hkv, D, BF, causal=causal, width=1250 if wide else None, sums=not wide)
+    _run(cuda, lqs, lens, hq, hkv, D, BF, causal=causal, width=1250 if wide else None)
 
 
 @pytest.mark.parametrize("causal", [True, False])
