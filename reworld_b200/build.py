@@ -55,7 +55,7 @@ def _compile_bind(obj):
            "-o", obj, "-isystem", inc, "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"), "-isystem", cuda,
            "-isystem", sysconfig.get_paths()["include"]]
     _run(cmd)
-    return [CXX, "-shared", "-o", bind_path() + ".tmp", obj, "-L" + lib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+    return [CXX, "-shared", "-o", bind_path() + ".tmp", obj, "-L" + lib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
            "-L" + OUT_DIR, "-lreworld_b200",
            # the C++ and CUDA runtimes that torch loads: a second, static C++ runtime (a compiler that comes with
            # libstdc++.a alone takes that) is mixed with torch's, and the first formatted message ends the process

@@ -10,6 +10,7 @@
 // graphs share nothing.  The interpreter lock is held throughout, so that two host threads
 // that use one stream cannot put their launches between each other's.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -38,6 +39,11 @@ void check_code(int code, const char* what) {
 }
 
 int dtype_code(at::ScalarType t) { return t == at::kBFloat16 ? RW_DTYPE_BF16 : (t == at::kHalf ? RW_DTYPE_FP16 : -1); }
+
+// A new tensor beside `like` (at::empty's dispatch costs as much again as the allocation: 0.4 us a tensor).
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
 
 struct Heads {
   void* ptr;
@@ -188,14 +194,13 @@ int* status_word(int device) {
 }
 
 Tensor scratch_for(const Tensor& like, cudaStream_t stream, int64_t bytes) {
-  const auto opt = like.options().requires_grad(false).dtype(at::kByte);
   // (a large one is not worth keeping: its allocation is nothing beside the call)
   if (bytes > (64 << 20) || c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
-    return at::empty({bytes}, opt);
+    return fresh({bytes}, at::kByte, like);
   // never destroyed: at exit the device may be gone before it
   static auto* kept = new std::map<std::pair<int, cudaStream_t>, Tensor>();
   Tensor& s = (*kept)[{like.device().index(), stream}];
-  if (!s.defined() || s.numel() < bytes) s = at::empty({bytes}, opt);
+  if (!s.defined() || s.numel() < bytes) s = fresh({bytes}, at::kByte, like);
   return s;
 }
 
@@ -211,7 +216,7 @@ Tensor rotary(const Tensor& x, const Tensor& table, const Tensor& positions, boo
   const c10::cuda::CUDAGuard guard(x.device());
   Tensor copy;
   const Heads in = input(x, "x", x, copy);
-  const Tensor y = out ? *out : at::empty({T, H, D}, x.options());
+  const Tensor y = out ? *out : fresh({T, H, D}, x.scalar_type(), x);
   const Heads o = out ? output(y, "out", x, x.sizes(), x) : heads_of(y);
   if (T && H)
     check_code(rw_rotary(in.ptr, o.ptr, count(T, "tokens"), count(H, "heads"), (int)D, code, in.sl, in.sh, o.sl, o.sh,
@@ -245,7 +250,7 @@ optional<Tensor> store(const Tensor& k, const Tensor& v, const Tensor& k_pages, 
       ho = output(*y, "q_out", k_pages, q->sizes(), *q);
       CHECK_VALUE(!meet(*y, k) && !meet(*y, v), "q_out overlaps k or v");
     } else {
-      y = at::empty({T, Hq, (int64_t)c.D}, k_pages.options());
+      y = fresh({T, Hq, (int64_t)c.D}, k_pages.scalar_type(), k_pages);
       ho = heads_of(*y);
     }
     if (Hq == 0) hq.ptr = ho.ptr = nullptr;
@@ -297,7 +302,7 @@ py::object attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pag
     ho = output(y, "out", k_pages, q.sizes(), q);
     CHECK_VALUE(y.numel() == 0 || y.data_ptr() != q.data_ptr(), "out overlaps q");
   } else {
-    y = at::empty({T, Hq, D}, k_pages.options());
+    y = fresh({T, Hq, D}, k_pages.scalar_type(), k_pages);
     ho = heads_of(y);
   }
   const double scale = softmax_scale ? *softmax_scale : 1.0 / std::sqrt((double)D);
@@ -307,7 +312,7 @@ py::object attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pag
   Sums w{nullptr, 0, 0, 0};
   if (weight_sums) w = sums_of(*weight_sums, c, rows, k_pages);
   Tensor lse;
-  if (return_lse) lse = at::empty({T, Hq}, k_pages.options().dtype(at::kFloat));
+  if (return_lse) lse = fresh({T, Hq}, at::kFloat, k_pages);
   if (T && c.B && longest) {
     const int dev = k_pages.device().index();
     cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev).stream();
@@ -335,9 +340,8 @@ py::tuple evict(const Tensor& k_pages, const Tensor& v_pages, const Tensor& bloc
   CHECK_VALUE(dst.width * c.page_size >= keep, "dst_table holds ", dst.width * c.page_size, " rows, ", keep,
               " are kept");
   const c10::cuda::CUDAGuard guard(k_pages.device());
-  const auto opt = k_pages.options().requires_grad(false);
-  const Tensor kept = at::empty({c.B, c.Hkv, keep}, opt.dtype(at::kInt)), lens = at::empty({c.B}, opt.dtype(at::kInt)),
-               sums = at::empty({c.B, c.Hkv, w.cap}, opt.dtype(at::kFloat));
+  const Tensor kept = fresh({c.B, c.Hkv, keep}, at::kInt, k_pages), lens = fresh({c.B}, at::kInt, k_pages),
+               sums = fresh({c.B, c.Hkv, w.cap}, at::kFloat, k_pages);
   const int dev = k_pages.device().index();
   if (c.B)
     check_code(rw_paged_evict(&c, w.ptr, w.sb, w.sh, sums.data_ptr<float>(), w.cap, kept.data_ptr<int>(),
