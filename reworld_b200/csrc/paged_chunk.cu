@@ -789,7 +789,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         if (!pwait_warp(&sb.v_land[st], (phases >> st) & 1u, cx, RW_STATUS_TIMEOUT_LOAD)) break;
         phases ^= 1u << st;
         uint8_t* v = stages + st * STAGE_BYTES;
-        const int rows = max(0, sg.kv - (sg.kv0 + j) * BN), r0 = lane >> 3;
+        // rows of the tile that the sequence has (a checked tile need not be its last)
+        const int rows = min(BN, max(0, sg.kv - (sg.kv0 + j) * BN)), r0 = lane >> 3;
         auto at = [&](int r) { return reinterpret_cast<uint4*>(v + r * 128 + (((lane & 7) ^ (r & 7)) << 4)); };
 #pragma unroll 1
         for (int r = r0 + (max(0, rows - r0) + 3) / 4 * 4; r < BN; r += 4) *at(r) = make_uint4(0, 0, 0, 0);
