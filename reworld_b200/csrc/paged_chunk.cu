@@ -63,6 +63,11 @@ constexpr int SOFTMAX_THREADS = 256;
 constexpr int REG_SOFTMAX = 208, REG_OTHER = 88;
 static_assert(NWG * 128 * REG_SOFTMAX + 128 * REG_OTHER <= NUM_THREADS * 168, "register split exceeds the launch's");
 constexpr float RESCALE_THRESHOLD = 8.0f;    // log2 units
+// fp16 weights are exp2(s - base + 7), 2^15 at most: a row that gives one key nearly everything still has weights of
+// 2^-14 to 2^-24 of that one, which fp16 would hold to a few bits or none, and a long cache has enough of them to be
+// seen (4.5 * 2^-24 from each of 60000 keys is 1.6 % of a row, 11 % of it lost).  Totals have the factor too.
+template <bool HALF> constexpr float UP_LOG2 = HALF ? 7.0f : 0.0f;
+template <bool HALF> constexpr float DOWN = HALF ? 1.0f / 128 : 1.0f;
 // What work dealt out in equal shares costs more than whole units: the starts of parts, and their joining.  Whole units
 // against shares: 8 units of 12 tiles 25.1 and 30.6 us, of 16 tiles 28.2 and 31.4, of 32 tiles 39.9 and 36.1 (74 pairs); 64
 // units of 35 tiles 46.5 and 56.5; head dim 64 (148 CTAs) 4 units of 8 tiles 20.3 and 22.2, of 20 tiles 26.9 and 23.8; 344
@@ -905,7 +910,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         if (one_pass) {
           uint32_t pk[2][32];
           uint64_t l2f = l2;
-          const float nm0 = -m_base * sl2;
+          const float nm0 = UP_LOG2<HALF> - m_base * sl2;
           const uint64_t nm02 = f2_pack(nm0, nm0);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -980,7 +985,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             l2 = f2_pack(lo * f, hi * f);
             m_base = m_use;
           }
-          const float nm = m_use == -INFINITY ? 0.f : -m_use * sl2;  // nothing seen yet: weights of exp2(-inf) = 0
+          const float nm = m_use == -INFINITY ? 0.f : UP_LOG2<HALF> - m_use * sl2;  // nothing seen yet: weights of exp2(-inf) = 0
           const uint64_t nm2 = f2_pack(nm, nm);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -1069,8 +1074,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                              : nullptr;
         if (ok && w == 0 && there) {
           const long long at = (long long)(sg.s0 + tok) * p.Hq + sg.hk * p.G + rg;
-          if (p.lse) p.lse[at] = l_row != 0.f ? (m_fin * sl2 + log2f(l_row)) * 0.6931471805599453f : -INFINITY;
-          if (p.row_b) p.row_b[at] = l_row != 0.f ? -(m_fin * sl2 + log2f(l_row)) : -INFINITY;
+          const float l = l_row * DOWN<HALF>;
+          if (p.lse) p.lse[at] = l != 0.f ? (m_fin * sl2 + log2f(l)) * 0.6931471805599453f : -INFINITY;
+          if (p.row_b) p.row_b[at] = l != 0.f ? -(m_fin * sl2 + log2f(l)) : -INFINITY;
         }
         named_bar_sync(1, SOFTMAX_THREADS);
         constexpr int CH = D / 8;
@@ -1196,6 +1202,7 @@ __global__ void __launch_bounds__(BM) join_kernel(const __grid_constant__ Params
   }
   if (c0 == 0) {
     const long long at = (long long)(sq.s0 + tok) * p.Hq + head;
+    l *= DOWN<HALF>;
     if (p.lse) p.lse[at] = l != 0.f ? (m * p.scale_log2 + log2f(l)) * 0.6931471805599453f : -INFINITY;
     if (p.row_b) p.row_b[at] = l != 0.f ? -(m * p.scale_log2 + log2f(l)) : -INFINITY;
   }

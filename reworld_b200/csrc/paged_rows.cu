@@ -174,6 +174,7 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
   constexpr int SLOT = RT * D + 2 * RT;      // floats of a part
   constexpr int LOADS = TILE * CH / THREADS; // cp.async of k (and of v) a thread
   constexpr int RSTEP = THREADS / CH;        // rows between two of them
+  constexpr float UP = HALF ? 32768.f : 1.f; // factor of the weights in the second product
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ long long base[THREADS + 1];
   __shared__ Seg seg[2];
@@ -435,7 +436,8 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
         m[0] = mx[0];
         m[1] = mx[1];
       }
-      // weights in fp32 for the sum, rounded to the values' type for the product (its operands' type)
+      // weights in fp32 for the sum, rounded to the values' type for the product (its operands' type); fp16 ones 2^15 times
+      // as large, so that a key with 2^-24 of the largest weight still has all its bits
       uint32_t pf[4];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -443,8 +445,8 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
         const float b0 = fast_exp2(sc[i][2] - base_[1]), b1 = fast_exp2(sc[i][3] - base_[1]);
         l[0] += a0 + a1;
         l[1] += b0 + b1;
-        pf[2 * i] = Num<HALF>::pack(a0, a1);
-        pf[2 * i + 1] = Num<HALF>::pack(b0, b1);
+        pf[2 * i] = Num<HALF>::pack(UP * a0, UP * a1);
+        pf[2 * i + 1] = Num<HALF>::pack(UP * b0, UP * b1);
       }
 #pragma unroll
       for (int dd = 0; dd < D / 16; ++dd) {
@@ -480,7 +482,8 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
     for (int i = 0; i < D / 8; ++i)
 #pragma unroll
       for (int x = 0; x < 2; ++x)
-        *reinterpret_cast<float2*>(at(warp, grp + 8 * x, 8 * i + 2 * quad)) = make_float2(o[i][2 * x], o[i][2 * x + 1]);
+        *reinterpret_cast<float2*>(at(warp, grp + 8 * x, 8 * i + 2 * quad)) =
+            make_float2(o[i][2 * x] * (1.f / UP), o[i][2 * x + 1] * (1.f / UP));
     __syncthreads();
 
     const bool whole = !CLUSTER && n == sg.n_tiles;

@@ -291,34 +291,43 @@ def test_values_of_later_tokens_that_are_not_finite(cuda, dtype, D, hq, hkv, lqs
     assert torch.equal(lse[rows], lref[rows])
 
 
-@pytest.mark.parametrize("dtype,D,hq,hkv,lqs,lens", [
-    (BF, 128, 4, 4, [1501], [1501]),                     # a prompt: from its first tile on not every row sees all
-    (FP, 64, 6, 2, [1501], [1501]),
-    (BF, 128, 8, 1, [1501, 400], [1501, 900]),
-    (FP, 128, 2, 2, [1501], [4000]),                     # units in parts
-    (BF, 64, 1, 1, [2600], [2600]),
-])
-@pytest.mark.parametrize("early", [(3,), (130, 700), (3, 131, 702, 1100)])
-def test_values_early_in_a_prompt_that_are_not_finite(cuda, dtype, D, hq, hkv, lqs, lens, early):
-    """Infinities in the values of early tokens, with hundreds of the chunk's rows behind them: the tokens before are
-    what they were bit for bit, those behind have them in the channels they are in and what they had elsewhere."""
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("first", [0.0, 1.0])
+@pytest.mark.parametrize("D,batch,lq,n", [(64, 160, 130, 60000), (128, 80, 260, 60000), (64, 600, 1, 400000),
+                                          (128, 300, 1, 400000)])
+def test_many_small_weights_beside_a_large_one(cuda, dtype, first, D, batch, lq, n):
+    """Row 0 takes nearly everything and every other row 4.49 * 2^-24 of that, together 1.6 or 10 % of it; their values
+    are 1, row 0's is 0 (what such a row usually has: the others are all that is seen) or 1.  As many sequences (of the
+    same pages) as a CTA each has whole units.
+
+    Off by at most: the output's rounding; the weights', the same relative to what the small ones give; what is cut off
+    where a product is aligned with an fp32 accumulator, less than the accumulator's last place for every key (which is
+    large only beside first = 1; of 64 keys a warp of the kernel for few rows sees 16, so that its accumulator has a
+    quarter); and the total's additions, n / 32 of them at most, half a step of a number below 2 each."""
     from reworld_b200 import paged_attention
-    k, v, table, kv, g = _cache(cuda, lens, 16, hkv, D, dtype, 21)
-    s = _starts(cuda, lqs)
-    q = torch.randn(sum(lqs), hq, D, generator=g, device=cuda).to(dtype)
-    w0, w1 = (torch.zeros(len(lens), hkv, table.shape[1] * 16, device=cuda) for _ in range(2))
-    ref, lref = paged_attention(q, k, v, table, s, kv, max_q_len=max(lqs), weight_sums=w0, return_lse=True)
-    want = ref.float()
-    base = lens[0] - lqs[0]
-    for i, tok in enumerate(early):                      # channel 5 + i, one sign each
-        x = -math.inf if i & 1 else math.inf
-        v[int(table[0, (base + tok) // 16]), (base + tok) % 16, :, 5 + i] = x
-        want[tok:lqs[0], :, 5 + i] = x
-    out, lse = paged_attention(q, k, v, table, s, kv, max_q_len=max(lqs), weight_sums=w1, return_lse=True)
+    page = 64
+    pages = -(-n // page)
+    k = torch.zeros(pages, page, 1, D, dtype=dtype, device=cuda)
+    k[0, 0, 0, 0] = 1.0
+    v = torch.ones_like(k)
+    v[0, 0] = first
+    table = torch.arange(pages, dtype=torch.int32, device=cuda).expand(batch, pages).contiguous()
+    q = torch.zeros(batch * lq, 1, D, dtype=dtype, device=cuda)
+    q[..., 0] = 1.0
+    w = 4.49 * 2.0 ** -24
+    kv = torch.full((batch,), n, dtype=torch.int32, device=cuda)
+    out, lse = paged_attention(q, k, v, table, _starts(cuda, [lq] * batch), kv, max_q_len=lq, causal=False,
+                               softmax_scale=-math.log(w), return_lse=True)
     torch.cuda.synchronize()
     _status_clean()
-    assert torch.equal(out.float(), want)
-    assert torch.equal(lse, lref) and torch.equal(w0, w1)
+    small = (n - 1) * w
+    want = (first + small) / (1 + small)
+    half = torch.finfo(dtype).eps / 2
+    last = 2.0 ** (math.floor(math.log2(first + small / (1 if lq > 1 else 4))) - 23)
+    total = n / 32 * 2.0 ** -24
+    tol = half * want + half * small + n * last + total
+    assert (out.double() - want).abs().max().item() <= tol
+    assert (lse.double() - math.log1p(small) + math.log(w)).abs().max().item() <= total + 2.0 ** -18
 
 
 def test_strided_inputs_and_output(cuda):
