@@ -428,8 +428,9 @@ int rw_rotary(const void* x, void* out, int T, int H, int D, int dtype, long lon
  * of sequence b is row kv_lens[b] - lq + i), and q_out = rotated q when q != NULL,
  * in one launch.  k, v: [T, Hkv, D], q, q_out: [T, Hq, D] (q_out may be q).
  * positions [T] or NULL (then a token's row is its position); table NULL: no
- * rotation.  Tokens behind the last sequence, and rows of the pools that no new
- * token has, stay as they were. */
+ * rotation.  Tokens of no sequence (behind the last one, before the first; with
+ * starts that fall there may be others), and rows of the pools that no new token
+ * has, stay as they were. */
 int rw_paged_rotary_store(const rw_paged_t* cache, const void* k, const void* v, const void* q, void* q_out, int T,
                           int Hq, long long k_sl, long long k_sh, long long v_sl, long long v_sh, long long q_sl,
                           long long q_sh, long long qo_sl, long long qo_sh, const float* table, int max_pos, int rot,

@@ -76,6 +76,11 @@ template <bool HALF>
 __global__ void __launch_bounds__(THREADS) rotary_kernel(const __grid_constant__ Params p) {
   griddep_launch_dependents();
   griddep_wait();
+  if (p.with_pool && blockIdx.x == gridDim.x - 1) {
+    // The last CTA has no token: it looks at every sequence's start and length, also of those that no token finds.
+    for (int b = threadIdx.x; b < p.pool.B; b += THREADS) paged::load_seq(p.pool, b, p.T, p.status);
+    return;
+  }
   const int ipt = p.D / 16;              // items of a head
   const int item = threadIdx.x % ipt;
   const int h0 = threadIdx.x / ipt, hstep = THREADS / ipt;
@@ -100,7 +105,6 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(const __grid_constant__
     int pos = p.positions ? __ldg(p.positions + t) : 0;
     const uint8_t* kd = nullptr;
     const uint8_t* vd = nullptr;
-    bool in_seq = true;
     if (p.with_pool) {
       if (b < 0 || t >= sq.s0 + sq.lq) {
         // sequences that end at or before t; the sequence of t follows them
@@ -109,13 +113,13 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(const __grid_constant__
           const int e = i + lane <= p.pool.B ? __ldg(p.pool.q_starts + i + lane) : 0x7fffffff;
           b += __popc(__ballot_sync(0xffffffffu, e <= t));
         }
-        if (b >= p.pool.B) break;        // tokens behind the last sequence stay as they were
-        sq = paged::load_seq(p.pool, b, p.T, p.status);
+        if (b >= p.pool.B) break;        // tokens behind the last sequence stay as they were,
+        sq = paged::load_seq(p.pool, b, p.T, nullptr);
       }
-      in_seq = t >= sq.s0 && t < sq.s0 + sq.lq;
+      if (t < sq.s0 || t >= sq.s0 + sq.lq) continue;   // and those before the first one or where starts fall
       const int row = sq.kv - sq.lq + (t - sq.s0);
       if (!p.positions) pos = row;
-      if (in_seq && row >= 0) {
+      if (row >= 0) {
         const int pg = __ldg(p.pool.table + b * p.pool.table_stride + (row >> p.pool.page_shift));
         const int slot = row & ((1 << p.pool.page_shift) - 1);
         if ((unsigned)pg < (unsigned)p.pool.num_pages) {
@@ -182,7 +186,7 @@ inline int launch(Params& p, int dtype, void* stream) {
   // 65.9 us with 1, 65.3 with 2, 65.6 with 3, 70.0 with 4 (72 with one wave of CTAs), of 24 + 8 heads 37.2, 34.6,
   // 32.9, 35.9; 4 x 700 tokens of 24 + 48 heads 20.5, 23.1, 21.6, 25.7.
   p.run = std::min(3, std::max(1, p.T / (sms * 16)));
-  const int grid = (p.T + p.run - 1) / p.run;
+  const int grid = (p.T + p.run - 1) / p.run + (p.with_pool ? 1 : 0);
   auto kernel = dtype == RW_DTYPE_FP16 ? rotary_kernel<true> : rotary_kernel<false>;
   return launch_dependent(kernel, dim3(grid), dim3(THREADS), 0, static_cast<cudaStream_t>(stream), p) == cudaSuccess
              ? RW_OK : RW_ERR_CUDA;

@@ -113,7 +113,8 @@ def paged_rotary_store(k, v, k_pages, v_pages, block_table, q_starts, kv_lens, t
     kv_lens[b] - lq + i.  With q [T, Hq, D], the rotated q is returned (q_out, which may be q).
     table, interleaved: as rotary(); without a table nothing is rotated.  positions: int32 [T], by
     default a token's row (an evicted cache needs them: its rows are fewer than its positions).
-    Tokens behind the last sequence are not written; their rows of q_out stay as they were.
+    Tokens of no sequence (behind the last one, before the first) are not written; their rows of q_out stay
+    as they were.
     Replaces the cache write of wan_5b/modules/action_model.py:265-292."""
     return _bind.store(k, v, k_pages, v_pages, block_table, q_starts, kv_lens, table, positions, q, q_out, interleaved)
 

@@ -576,6 +576,145 @@ def test_bad_pages_and_lengths_are_reported_and_stay_in_bounds(cuda, wide):
     _status_clean()
 
 
+BAD = ["page high", "page low", "length beyond", "length negative", "start falls", "start passes", "start negative"]
+
+
+def _three(cuda, lq, width, hkv=2, D=64, page=16):
+    """Three sequences of lq new tokens with `width` pages each, all of them there."""
+    g = torch.Generator(device=cuda).manual_seed(31)
+    total = 3 * width + 6
+    k, v = (torch.randn(total, page, hkv, D, generator=g, device=cuda).to(BF) for _ in range(2))
+    table = torch.randperm(total, generator=g, device=cuda)[:3 * width].to(torch.int32).view(3, width).contiguous()
+    kv = torch.tensor([500, 390, 450], dtype=torch.int32, device=cuda)
+    return k, v, table, _starts(cuda, [lq] * 3), kv, g
+
+
+def _spoil(kind, lq, table, s, kv, page=16):
+    """(table, starts, lengths) with one value out of range, and what they are brought to."""
+    bad, good = [table.clone(), s.clone(), kv.clone()], [table.clone(), s.clone(), kv.clone()]
+    if kind.startswith("page"):
+        bad[0][1] = 2 ** 31 - 1 if kind == "page high" else -1
+        good[0][1] = 0
+    elif kind.startswith("length"):
+        bad[2][1] = 2 ** 31 - 1 if kind == "length beyond" else -5
+        good[2][1] = table.shape[1] * page if kind == "length beyond" else 0
+    elif kind == "start falls":
+        bad[1][0], good[1][0] = 2 * lq, lq               # the first sequence ends before it starts: it has no token
+    elif kind == "start passes":
+        bad[1][3] = 9 * lq + 1
+    else:
+        bad[1][0] = -3
+    return bad, good
+
+
+def _bits(*tensors):
+    return [t.view(torch.int16 if t.element_size() == 2 else torch.int32) for t in tensors]
+
+
+@pytest.mark.parametrize("sums", [False, True])
+@pytest.mark.parametrize("width", [32, 1250])
+@pytest.mark.parametrize("lq", [1, 60, 300])
+@pytest.mark.parametrize("kind", BAD)
+def test_attention_brings_values_into_range_and_reports_them(cuda, kind, lq, width, sums):
+    """Bit for bit what the call gives with the values that they are brought to, for all sequences, and a report."""
+    from reworld_b200 import _native, paged_attention
+    k, v, table, s, kv, g = _three(cuda, lq, width)
+    q = torch.randn(3 * lq, 8, 64, generator=g, device=cuda).to(BF)
+    got = []
+    for t, st, n in _spoil(kind, lq, table, s, kv):
+        out, w = torch.full_like(q, 7.0), torch.full((3, 2, 16 * width), 0.5, device=cuda) if sums else None
+        _, lse = paged_attention(q, k, v, t, st, n, max_q_len=lq, weight_sums=w, return_lse=True, out=out)
+        torch.cuda.synchronize()
+        first = lq if kind == "start falls" else 0       # tokens before the first sequence have no lse
+        got.append(_bits(out, lse[first:], *([w] if sums else [])))
+        if len(got) == 1:
+            with pytest.raises(RuntimeError):
+                _native.check_status(cuda)
+    _status_clean()
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("lq", [1, 60, 300])
+@pytest.mark.parametrize("kind", BAD + ["idle length", "idle start"])
+def test_store_brings_values_into_range_and_reports_them(cuda, kind, lq):
+    from reworld_b200 import _native, paged_rotary_store
+    k, v, table, s, kv, g = _three(cuda, lq, 32)
+    kn, vn = (torch.randn(3 * lq, 2, 64, generator=g, device=cuda).to(BF) for _ in range(2))
+    q = torch.randn(3 * lq, 4, 64, generator=g, device=cuda).to(BF)
+    if kind == "idle length":                            # of a sequence without a token
+        s = torch.cat([s[:1], s[:3]])
+        bad, good = [table, s, kv.clone()], [table, s, kv]
+        bad[2][0] = -1
+    elif kind == "idle start":                           # no token's place says that the last sequence's is wrong
+        s = torch.cat([s[:3], s[2:3]])
+        bad, good = [table, s.clone(), kv], [table, s, kv]
+        bad[1][3] = 2 * lq - 1
+    else:
+        bad, good = _spoil(kind, lq, table, s, kv)
+        if kind.startswith("page"):                      # (rows without a page are not written)
+            good = [table, s, kv]
+    got = []
+    for t, st, n in (bad, good):
+        kp, vp, qo = k.clone(), v.clone(), torch.full_like(q, 7.0)
+        paged_rotary_store(kn, vn, kp, vp, t, st, n, q=q, q_out=qo)
+        torch.cuda.synchronize()
+        if len(got) == 0:
+            with pytest.raises(RuntimeError):
+                _native.check_status(cuda)
+        got.append((kp, vp, qo))
+    if kind == "length negative":                        # (more new tokens than rows, here too)
+        with pytest.raises(RuntimeError):
+            _native.check_status(cuda)
+    if kind.startswith("page"):
+        for pool, old in zip(got[1][:2], (k, v)):
+            pool[table[1].long()] = old[table[1].long()]
+    if kind == "idle start":                             # the token at the place that the start fell to is nobody's
+        row = int(kv[1]) - 1
+        for pool, old in zip(got[1][:2], (k, v)):
+            pool[int(table[1, row // 16]), row % 16] = old[int(table[1, row // 16]), row % 16]
+        got[1][2][2 * lq - 1] = 7.0
+    if kind == "start falls":                            # tokens before the first sequence
+        assert (got[0][2][:lq] == 7.0).all() and (got[1][2][:lq] == 7.0).all()
+    for a, b in zip(_bits(*got[0]), _bits(*got[1])):
+        assert torch.equal(a, b)
+    _status_clean()
+
+
+@pytest.mark.parametrize("width", [32, 1250])
+@pytest.mark.parametrize("kind", ["page high", "page low", "length beyond", "length negative", "new page high",
+                                  "new page low"])
+def test_evict_brings_values_into_range_and_reports_them(cuda, kind, width):
+    from reworld_b200 import _native, paged_evict
+    k, v, table, s, kv, g = _three(cuda, 1, width)
+    keep = 40
+    spare = [i for i in range(k.shape[0]) if i not in set(table.flatten().tolist())]
+    dst = torch.tensor(spare[:6] + table[2, -3:].tolist(), dtype=torch.int32, device=cuda).view(3, 3)
+    table[2, -3:] = table[2, 0]                          # (behind the last row)
+    w = torch.rand(3, 2, 16 * width, generator=g, device=cuda)
+    if kind.startswith("new"):
+        bad, good = [table, dst.clone(), kv], [table, dst, kv]
+        bad[1][1] = 2 ** 31 - 1 if kind == "new page high" else -1
+    else:
+        (t0, _, n0), (t1, _, n1) = _spoil(kind, 1, table, s, kv)
+        bad, good = [t0, dst, n0], [t1, dst, n1]
+    got = []
+    for t, d, n in (bad, good):
+        kp, vp = k.clone(), v.clone()
+        kept, lens, sums = paged_evict(kp, vp, t, n, w, keep, d, n_sink=2, n_recent=5)
+        torch.cuda.synchronize()
+        got.append((kp, vp, kept, lens, sums))
+        if len(got) == 1:
+            with pytest.raises(RuntimeError):
+                _native.check_status(cuda)
+    if kind.startswith("new"):                           # rows without a page are not written
+        for pool, old in zip(got[1][:2], (k, v)):
+            pool[dst[1].long()] = old[dst[1].long()]
+    for a, b in zip(_bits(*got[0]), _bits(*got[1])):
+        assert torch.equal(a, b)
+    _status_clean()
+
+
 # ------------------------------------------------------------------ rotary positions and the page write
 
 def _freq(rot, theta=10000.0):
