@@ -450,7 +450,8 @@ int rw_paged_rotary_store(const rw_paged_t* cache, const void* k, const void* v,
  * gave to cached row j.  The order of the additions is fixed.
  * workspace: device memory, 16-byte aligned, rw_paged_attn_workspace_bytes(...)
  * bytes (0: it may be null), contents of no matter; calls that overlap on the GPU need workspaces of
- * their own.  (cache_rows: table_width * page_size; with_sums: sums != NULL.) */
+ * their own.  With sums, and up to 16 rows (tokens x Hq / Hkv) a sequence and key head, it holds the scores: 4 *
+ * Hkv * rows * cache_rows bytes a sequence, of as many sequences as fit 1 GiB (one at least).  (cache_rows: table_width * page_size; with_sums: sums != NULL.) */
 int rw_paged_attn(const rw_paged_t* cache, const void* q, void* out, float* lse, int T, int Hq, int max_q_len,
                   long long q_sl, long long q_sh, long long o_sl, long long o_sh, int causal, float softmax_scale,
                   float* sums, long long sums_sb, long long sums_sh, void* workspace, long long workspace_bytes,

@@ -833,6 +833,17 @@ inline Layout layout(int D, int C, int B, int Hkv, long long rows, long long cap
   return l;
 }
 
+// Sequences of a launch by shares.  With weights every row's scores are kept for the second kernel, for as many keys as
+// the table has room for: a batch whose scores would take more than SCORE_BYTES goes in slices that take no more (one
+// sequence's, if that is more), so that a wide table cannot make a decoding step run out of memory.  A slice more is
+// a start and a joining more: 256 sequences of 2154 rows on average, 32 heads, a table of 32768 (1 GB of scores) 549 us
+// in one, 572 in two, 696 in eight slices; 64 of 2141 rows, 64 heads, a table of 131072 (2.1 GB) 312, 389 in four.
+constexpr long long SCORE_BYTES = 1ll << 30;
+inline int slice_of(int B, int Hkv, long long rows, long long cap, bool sums) {
+  const long long each = 4 * Hkv * rows * cap;
+  return sums && each > 0 ? (int)std::min((long long)B, std::max(1ll, SCORE_BYTES / each)) : B;
+}
+
 // A launch of the CLUSTER kernel: CTAs of a unit (0: units are shared out among all CTAs instead), keys of a CTA at most,
 // dynamic shared memory.
 //
@@ -929,7 +940,8 @@ int run_rows(const rw_paged_t* cache, const Pool& pool, const chunk::Call& c, lo
   if (cap == 0) sums = nullptr;
   const long long need = cl.cs ? block_sums_bytes((long long)cache->B * pool.Hkv, rows, cap, sums != nullptr) : 0;
   if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return RW_ERR_INVALID_ARG;
-  const Layout lay = layout(cache->D, C, cache->B, pool.Hkv, rows, cap, sums != nullptr);
+  const int slice = cl.cs ? cache->B : slice_of(cache->B, pool.Hkv, rows, cap, sums != nullptr);
+  const Layout lay = layout(cache->D, C, slice, pool.Hkv, rows, cap, sums != nullptr);
   if (cl.cs == 0 && (!workspace || !aligned16(workspace) || workspace_bytes < lay.total)) return RW_ERR_INVALID_ARG;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   Params p{};
@@ -950,16 +962,22 @@ int run_rows(const rw_paged_t* cache, const Pool& pool, const chunk::Call& c, lo
     p.scores = sums ? reinterpret_cast<float*>(ws + lay.scores) : nullptr;
     p.row_ml = sums ? reinterpret_cast<float2*>(ws + lay.ml) : nullptr;
   }
-  p.sums = sums;
   p.sums_sb = sums_sb; p.sums_sh = sums_sh;
   p.cap = cap;
   p.status = c.status;
-  // no more CTAs than there can be tiles: the others would only cost their launch
-  const long long most = (long long)cache->B * pool.Hkv * std::max(1ll, (cap + TILE - 1) / TILE);
-  const int ctas = (int)std::min((long long)C, most);
-  if (cache->dtype == RW_DTYPE_FP16)
-    return cache->D == 128 ? launch_rows<true, 128>(p, ctas, cl.bytes, st) : launch_rows<true, 64>(p, ctas, cl.bytes, st);
-  return cache->D == 128 ? launch_rows<false, 128>(p, ctas, cl.bytes, st) : launch_rows<false, 64>(p, ctas, cl.bytes, st);
+  const auto launch = cache->dtype == RW_DTYPE_FP16 ? (cache->D == 128 ? launch_rows<true, 128> : launch_rows<true, 64>)
+                                                    : (cache->D == 128 ? launch_rows<false, 128> : launch_rows<false, 64>);
+  for (int b = 0; b < cache->B; b += slice) {
+    p.pool.B = std::min(slice, cache->B - b);
+    p.pool.table = pool.table + b * pool.table_stride;
+    p.pool.q_starts = pool.q_starts + b;
+    p.pool.kv_lens = pool.kv_lens + b;
+    p.sums = sums ? sums + b * sums_sb : nullptr;
+    // no more CTAs than there can be tiles: the others would only cost their launch
+    const long long most = (long long)p.pool.B * pool.Hkv * std::max(1ll, (cap + TILE - 1) / TILE);
+    if (int e = launch(p, (int)std::min((long long)C, most), cl.bytes, st)) return e;
+  }
+  return RW_OK;
 }
 
 // The chunk kernels plan MAX_BATCH sequences a launch.
@@ -1021,6 +1039,8 @@ extern "C" long long rw_paged_attn_workspace_bytes(int T, int Hq, int Hkv, int D
   const long long rows = (long long)std::min(max_q_len, T) * (Hq / Hkv);
   if (rows::clusters_for(D, (long long)B * Hkv, rows, cache_rows, with_sums != 0).cs)
     return rows::block_sums_bytes((long long)B * Hkv, rows, cache_rows, with_sums != 0);
-  if (rows::few_rows(rows)) return rows::layout(D, rows::grid_size(D), B, Hkv, rows, cache_rows, with_sums != 0).total;
+  if (rows::few_rows(rows))
+    return rows::layout(D, rows::grid_size(D), rows::slice_of(B, Hkv, rows, cache_rows, with_sums != 0), Hkv, rows,
+                        cache_rows, with_sums != 0).total;
   return chunk::workspace_bytes(D) + (with_sums ? 4LL * T * Hq : 0);
 }

@@ -132,6 +132,8 @@ def paged_attention(q, k_pages, v_pages, block_table, q_starts, kv_lens, max_q_l
     decoding step) is what lets the call choose its kernel.
     weight_sums: fp32 [B, Hkv, cap], cap >= block_table's rows, contiguous last dim; the weight that
     every cached row received from the new tokens (all query heads of the group) is added to it.
+    (Few tokens' weights take scratch memory for their scores by the table's width: 4 bytes for every head, token and
+    row of block_table, up to 1 GiB, or one sequence's if that is more.)
     Returns out [T, Hq, D] in q's dtype, or (out, lse [T, Hq] fp32).  Rows behind the last sequence
     stay as they were in a given `out` and are undefined in a new one, as are those of a sequence
     with more than max_q_len tokens.

@@ -136,6 +136,14 @@ def test_single_tokens_batches(cuda, batch):
     _run(cuda, [1] * batch, [(37 * i) % 211 + 1 for i in range(batch)], 4, 2, 64, FP, sums=batch < 200)
 
 
+@pytest.mark.parametrize("lqs,hq", [([1] * 5, 128), ([2, 1, 2, 0, 2], 64)])
+def test_weights_of_single_tokens_over_a_very_wide_table(cuda, lqs, hq):
+    """512 MiB of scores a sequence: the batch goes in slices of two."""
+    from reworld_b200 import _native
+    assert _native.lib().rw_paged_attn_workspace_bytes(sum(lqs) + 2, hq, 8, 64, 5, max(lqs), 1 << 20, 1) < 1.1 * 2 ** 30
+    _run(cuda, lqs, [700, 3000, 64, 90, 1], hq, 8, 64, BF, page=64, width=16384)
+
+
 def _widen(table, wide):
     """Few rows over a long table are shared out among all CTAs, over a short one they are a cluster's."""
     return torch.nn.functional.pad(table, (0, 1250 - table.shape[1])) if wide else table

@@ -111,6 +111,18 @@ def test_workspace_of_odd_questions():
     assert fn(1, 8, 2, 128, 1, 1, 64, 0) >= 0
 
 
+def test_workspace_of_weight_sums_is_bounded():
+    """Few rows' scores go by the table's width; a batch of any size takes 1 GiB, or one sequence's."""
+    fn = _native.lib().rw_paged_attn_workspace_bytes
+    small = fn(16, 512, 8, 128, 1, 1, 4096, 1)
+    for B in (64, 256, 4000):
+        for cap in (131072, 1 << 20, 1 << 22):
+            one = 4 * 8 * 16 * cap
+            lines = max(1, (1 << 30) // one) * 8 * 16
+            got = fn(B, 128, 8, 128, B, 1, cap, 1)
+            assert min(B * one, max(1 << 30, one)) - one <= got <= max(1 << 30, one) + 16 * lines + 8 * 8 * B + 1024 + small
+
+
 def test_python_calls_reject_cpu_tensors():
     z = torch.zeros(1, 8, 2, 128, dtype=torch.bfloat16)
     t = torch.zeros(1, 1, dtype=torch.int32)
