@@ -10,7 +10,8 @@ attention, with the reference's plugin points as the API:
                                 positions, page writes, attention, eviction by attention weight
   ulysses                       sequence-parallel (head-sharded) chunk attention
 All compute runs in the package's CUDA library (reworld_b200/_lib); importing
-the compute modules fails if it is missing.
+the compute modules fails if it is missing.  The paged calls also need
+_lib/paged_bind.so and fail without it.
 """
 from . import _native
 

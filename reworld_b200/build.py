@@ -94,14 +94,14 @@ def build(force=False, verbose=False):
         bind_obj = os.path.join(OUT_DIR, "paged_bind.o")
         bind = ex.submit(_compile_bind, bind_obj)
         objs = list(ex.map(compile_one, _sources()))
-        link_bind = bind.result()
     tmp = out + ".tmp"
     cmd = [NVCC, *ARCH, "-shared", "-o", tmp, *objs, "-cudart=static"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, out)
-    _run(link_bind)
+    # (behind the library, which is there whatever becomes of this: it needs no C++ compiler and no torch with CUDA)
+    _run(bind.result())
     os.replace(bind_path() + ".tmp", bind_path())
     for o in objs + [bind_obj]:
         os.remove(o)

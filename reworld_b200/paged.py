@@ -28,6 +28,7 @@ attention weight instead of pose.
 import importlib.util
 import math
 import os
+import threading
 
 import torch
 
@@ -48,7 +49,20 @@ def _load_bind():
     return mod
 
 
-_bind = _load_bind()
+class _Unloaded:
+    """Stands for the module until the first paged call: the rest of the package needs the CUDA library alone, and is
+    imported where the module is not built too."""
+    _lock = threading.Lock()
+
+    def __getattr__(self, name):
+        global _bind
+        with self._lock:
+            if _bind is self:
+                _bind = _load_bind()
+        return getattr(_bind, name)
+
+
+_bind = _Unloaded()
 
 
 # ------------------------------------------------------------------ rotary positions

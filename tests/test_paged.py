@@ -1,6 +1,10 @@
 """The paged-cache entry points' refusals and host logic: nothing here reaches a GPU."""
 import ctypes
 import math
+import os
+import shutil
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -174,3 +178,46 @@ def test_refusals_say_what_was_given():
         paged.paged_attention(z[0], z, z, n[None], n, n)
     with pytest.raises(ValueError, match=r"BFloat16 \[8, 2, 128\] on cpu"):
         paged.rotary(z[0], torch.zeros(4, 64, 2), n)
+
+
+def _in_a_copy(tmp_path, code, **env):
+    """Runs `code` where a copy of the package without its built binding is imported."""
+    pkg = tmp_path / "reworld_b200"
+    shutil.copytree(os.path.dirname(_native.__file__), pkg, ignore=shutil.ignore_patterns("__pycache__", "paged_bind*"))
+    shutil.copytree(os.path.join(os.path.dirname(os.path.dirname(_native.__file__)), "include"), tmp_path / "include")
+    return subprocess.run([sys.executable, "-c", code], cwd=tmp_path, capture_output=True, text=True,
+                          env={**os.environ, "PYTHONPATH": str(tmp_path), **env})
+
+
+def test_without_the_binding_everything_else_is_imported_and_paged_calls_fail(tmp_path):
+    r = _in_a_copy(tmp_path, """
+import torch, reworld_b200
+from reworld_b200 import attention, paged, self_attn, landmark, ulysses
+assert reworld_b200.__file__.startswith({!r})
+assert paged.rotary_table(4, 16, device="cpu").shape == (4, 8, 2)
+try:
+    reworld_b200.rotary(None, None, None)
+except ImportError as e:
+    print("refused:", e)
+""".format(str(tmp_path)))
+    assert r.returncode == 0, r.stderr
+    assert "refused:" in r.stdout and "build.py" in r.stdout
+
+
+def test_the_library_is_built_where_the_binding_cannot_be(tmp_path):
+    """With a C++ compiler that fails, build() says so, and the library is there."""
+    r = _in_a_copy(tmp_path, """
+import importlib.util, os
+spec = importlib.util.spec_from_file_location("b", "reworld_b200/build.py")
+b = importlib.util.module_from_spec(spec)
+spec.loader.exec_module(b)
+os.remove(b.lib_path())
+b._sources = lambda: [os.path.join(b.CSRC, "api.cu")]
+try:
+    b.build()
+except RuntimeError as e:
+    print("refused:", e)
+assert os.path.exists(b.lib_path()) and not os.path.exists(b.bind_path())
+""", CXX="false")
+    assert r.returncode == 0, r.stderr
+    assert "refused:" in r.stdout
