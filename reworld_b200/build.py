@@ -44,10 +44,35 @@ def bind_path():
     return os.path.join(OUT_DIR, BIND_NAME)
 
 
+def bind_stamp_path():
+    return bind_path() + ".for"
+
+
+def _torch_dir():
+    # found, not imported: a build needs torch's headers and libraries only
+    return list(importlib.util.find_spec("torch").submodule_search_locations)[0]
+
+
+def bind_stamp():
+    """What paged_bind.so is made for: torch's C++ interface and Python's differ from one version to the next."""
+    version = {}
+    with open(os.path.join(_torch_dir(), "version.py")) as f:
+        exec(f.read(), version)
+    return f"torch {version['__version__']} {sysconfig.get_config_var('SOABI')}"
+
+
+def bind_made_for():
+    """The stamp beside paged_bind.so, or None."""
+    try:
+        with open(bind_stamp_path()) as f:
+            return f.read()
+    except OSError:
+        return None
+
+
 def _compile_bind(obj):
     """Compiles paged_bind.cpp to `obj` and returns the command that links it."""
-    # found, not imported: a build needs torch's headers and libraries only
-    torch_dir = list(importlib.util.find_spec("torch").submodule_search_locations)[0]
+    torch_dir = _torch_dir()
     inc = os.path.join(torch_dir, "include")
     lib = os.path.join(torch_dir, "lib")
     cuda = os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")
@@ -70,11 +95,13 @@ def _run(cmd):
 
 def build(force=False, verbose=False):
     """Compiles csrc/*.cu into _lib/libreworld_b200.so and csrc/paged_bind.cpp into
-    _lib/paged_bind.so (skipped when up to date)."""
+    _lib/paged_bind.so (skipped when up to date: newer than the sources, and the second
+    one made for this torch and Python)."""
     os.makedirs(OUT_DIR, exist_ok=True)
     out = lib_path()
     newest = _newest_input_mtime()
-    if not force and all(os.path.exists(f) and os.path.getmtime(f) >= newest for f in (out, bind_path())):
+    if (not force and all(os.path.exists(f) and os.path.getmtime(f) >= newest for f in (out, bind_path()))
+            and bind_made_for() == bind_stamp()):
         return out
     objs = []
 
@@ -102,7 +129,11 @@ def build(force=False, verbose=False):
     os.replace(tmp, out)
     # (behind the library, which is there whatever becomes of this: it needs no C++ compiler and no torch with CUDA)
     _run(bind.result())
+    if os.path.exists(bind_stamp_path()):
+        os.remove(bind_stamp_path())
     os.replace(bind_path() + ".tmp", bind_path())
+    with open(bind_stamp_path(), "w") as f:
+        f.write(bind_stamp())
     for o in objs + [bind_obj]:
         os.remove(o)
     return out

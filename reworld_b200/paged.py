@@ -32,15 +32,17 @@ import threading
 
 import torch
 
-from . import _native
-from .build import bind_path
+from . import _native, build
 
 
 def _load_bind():
     """The module with the calls' checks (csrc/paged_bind.cpp); there is no other path."""
-    path = bind_path()
+    path = build.bind_path()
     if not os.path.exists(path):
         raise ImportError(f"reworld_b200 is not built ({path} missing); run `python reworld_b200/build.py`")
+    if build.bind_made_for() != build.bind_stamp():
+        raise ImportError(f"{path} is built for {build.bind_made_for()}, this is {build.bind_stamp()}; run `python "
+                          "reworld_b200/build.py`")
     spec = importlib.util.spec_from_file_location("paged_bind", path)
     mod = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(mod)

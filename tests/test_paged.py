@@ -221,3 +221,27 @@ assert os.path.exists(b.lib_path()) and not os.path.exists(b.bind_path())
 """, CXX="false")
     assert r.returncode == 0, r.stderr
     assert "refused:" in r.stdout
+
+
+def test_a_binding_for_another_torch_is_refused_and_built_again(tmp_path):
+    r = _in_a_copy(tmp_path, """
+import importlib.util, os
+spec = importlib.util.spec_from_file_location("b", "reworld_b200/build.py")
+b = importlib.util.module_from_spec(spec)
+spec.loader.exec_module(b)
+open(b.bind_path(), "w").close()
+open(b.bind_stamp_path(), "w").write("torch 1.0 another")
+b._sources = lambda: [os.path.join(b.CSRC, "api.cu")]
+b._compile_bind = lambda obj: open(obj, "w").close() or ["touch", b.bind_path() + ".tmp"]
+from reworld_b200 import paged
+try:
+    paged.rotary(None, None, None)
+except ImportError as e:
+    print("refused:", e)
+b.build()
+assert b.bind_made_for() == b.bind_stamp() and b.bind_stamp().startswith("torch 2")
+b._compile_bind = None
+b.build()                                                # up to date now
+""")
+    assert r.returncode == 0, r.stderr
+    assert "refused:" in r.stdout and "torch 1.0 another" in r.stdout
