@@ -76,7 +76,7 @@ def _compile_bind(obj):
     inc = os.path.join(torch_dir, "include")
     lib = os.path.join(torch_dir, "lib")
     cuda = os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")
-    cmd = [CXX, "-O2", "-std=c++20", "-fPIC", "-fvisibility=hidden", "-w", "-c", os.path.join(CSRC, "paged_bind.cpp"),
+    cmd = [CXX, "-O2", "-std=c++20", "-fPIC", "-fvisibility=hidden", "-Wall", "-Wextra", "-c", os.path.join(CSRC, "paged_bind.cpp"),
            "-o", obj, "-isystem", inc, "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"), "-isystem", cuda,
            "-isystem", sysconfig.get_paths()["include"]]
     _run(cmd)
@@ -91,6 +91,7 @@ def _run(cmd):
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"{' '.join(cmd)} failed:\n{r.stdout}\n{r.stderr}")
+    sys.stderr.write(r.stderr)                           # warnings
 
 
 def build(force=False, verbose=False):
