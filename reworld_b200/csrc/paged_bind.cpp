@@ -95,6 +95,18 @@ bool meet(const Tensor& a, const Tensor& b) {
   return true;
 }
 
+// Whether an output may lie among a pool's pages: between its first and its last byte.
+bool among(const Tensor& out, const Tensor& pool) {
+  if (out.numel() == 0) return false;
+  auto span = [](const Tensor& t) {
+    int64_t n = 1;
+    for (int64_t d = 0; d < t.dim(); ++d) n += (t.size(d) - 1) * t.stride(d);
+    return n * t.element_size();
+  };
+  const auto a = reinterpret_cast<uintptr_t>(out.data_ptr()), b = reinterpret_cast<uintptr_t>(pool.data_ptr());
+  return a < b + span(pool) && b < a + span(out);
+}
+
 // An output of the caller's: the input itself, or apart from it.
 Heads output(const Tensor& t, const char* name, const Tensor& like, at::IntArrayRef shape, const Tensor& given) {
   check_kind(t, name, like);
@@ -249,6 +261,7 @@ optional<Tensor> store(const Tensor& k, const Tensor& v, const Tensor& k_pages, 
       y = *q_out;
       ho = output(*y, "q_out", k_pages, q->sizes(), *q);
       CHECK_VALUE(!meet(*y, k) && !meet(*y, v), "q_out overlaps k or v");
+      CHECK_VALUE(!among(*y, k_pages) && !among(*y, v_pages), "q_out lies in the pools");
     } else {
       y = fresh({T, Hq, (int64_t)c.D}, k_pages.scalar_type(), k_pages);
       ho = heads_of(*y);
@@ -301,6 +314,7 @@ py::object attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pag
     y = *out;
     ho = output(y, "out", k_pages, q.sizes(), q);
     CHECK_VALUE(y.numel() == 0 || y.data_ptr() != q.data_ptr(), "out overlaps q");
+    CHECK_VALUE(!among(y, k_pages) && !among(y, v_pages), "out lies in the pools");
   } else {
     y = fresh({T, Hq, D}, k_pages.scalar_type(), k_pages);
     ho = heads_of(y);

@@ -126,7 +126,8 @@ def paged_rotary_store(k, v, k_pages, v_pages, block_table, q_starts, kv_lens, t
     """Writes the new tokens' keys, rotated, and values into their sequences' pages, in one launch.
 
     k, v: [T, Hkv, D] of the packed new tokens; token i of sequence b (of lq) becomes row
-    kv_lens[b] - lq + i.  With q [T, Hq, D], the rotated q is returned (q_out, which may be q).
+    kv_lens[b] - lq + i.  With q [T, Hq, D], the rotated q is returned (q_out, which may be q,
+    not in the pools).
     table, interleaved: as rotary(); without a table nothing is rotated.  positions: int32 [T], by
     default a token's row (an evicted cache needs them: its rows are fewer than its positions).
     Tokens of no sequence (behind the last one, before the first) are not written; their rows of q_out stay
@@ -150,6 +151,7 @@ def paged_attention(q, k_pages, v_pages, block_table, q_starts, kv_lens, max_q_l
     every cached row received from the new tokens (all query heads of the group) is added to it.
     (Few tokens' weights take scratch memory for their scores by the table's width: 4 bytes for every head, token and
     row of block_table, up to 1 GiB, or one sequence's if that is more.)
+    out must not lie in the pools.
     Returns out [T, Hq, D] in q's dtype, or (out, lse [T, Hq] fp32).  Rows behind the last sequence
     stay as they were in a given `out` and are undefined in a new one, as are those of a sequence
     with more than max_q_len tokens.

@@ -440,6 +440,30 @@ def test_nothing_to_do(cuda):
     _status_clean()
 
 
+def test_outputs_in_the_pools_are_refused(cuda):
+    from reworld_b200 import paged_attention, paged_rotary_store
+    k, v, table, kv, g = _cache(cuda, [30, 40], 16, 2, 64, BF, 16)
+    s = _starts(cuda, [3, 3])
+    q = torch.zeros(6, 2, 64, dtype=BF, device=cuda)
+    for pool in (k, v):
+        with pytest.raises(ValueError, match="pools"):
+            paged_attention(q, k, v, table, s, kv, out=pool[-1, :6])
+        with pytest.raises(ValueError, match="pools"):
+            paged_rotary_store(q, q, k, v, table, s, kv, q=q, q_out=pool[0, :6])
+        with pytest.raises(ValueError, match="pools"):
+            paged_rotary_store(q, q, k, v, table, s, kv, q=pool[0, :6], q_out=pool[0, :6])
+    # beside the pools in one tensor is well
+    page = k[0].numel()
+    arena = torch.zeros(2 * k.numel() + 2 * page, dtype=BF, device=cuda)
+    ka, va = arena[page:page + k.numel()].view_as(k), arena[page + k.numel():-page].view_as(k)
+    ka.copy_(k)
+    va.copy_(v)
+    for out in (arena[:6 * 128].view(6, 2, 64), arena[-6 * 128:].view(6, 2, 64)):
+        paged_attention(q, ka, va, table, s, kv, out=out)
+        assert torch.equal(out, paged_attention(q, k, v, table, s, kv))
+    _status_clean()
+
+
 def test_refusals_on_device_tensors(cuda):
     from reworld_b200 import paged_attention, paged_evict, paged_rotary_store, rotary, rotary_table
     k, v, table, kv, g = _cache(cuda, [30, 40], 16, 2, 64, BF, 16)
