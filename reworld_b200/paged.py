@@ -88,26 +88,34 @@ def rotary_table(max_pos, rotary_dim, theta=10000.0, scaling=None, device="cuda"
         raise ValueError("rotary_dim must be a positive multiple of 16")
     if max_pos < 1:
         raise ValueError("max_pos must be positive")
+    if not 0.0 < float(theta) < math.inf:
+        raise ValueError("theta must be positive and finite")
     i = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
     gain = 1.0
     freq = float(theta) ** (-i / rotary_dim)
     if scaling is not None:
-        kind, f = scaling[0], float(scaling[1])
-        if not f >= 1.0:
-            raise ValueError("the scaling factor must be >= 1")
+        kind = scaling[0]
+        if kind not in ("linear", "ntk", "bands"):
+            raise ValueError(f"unknown scaling {kind!r}")
+        if len(scaling) < (3 if kind == "bands" else 2) or (kind == "bands" and len(scaling) == 4):
+            raise ValueError(f"scaling {tuple(scaling)!r}: " + ("(kind, factor, trained) or (kind, factor, trained, slow, "
+                             "fast)" if kind == "bands" else "(kind, factor)") + " is needed")
+        f = float(scaling[1])
+        if not 1.0 <= f < math.inf:
+            raise ValueError("the scaling factor must be >= 1 and finite")
         if kind == "linear":
             freq = freq / f
         elif kind == "ntk":
             freq = (float(theta) * f ** (rotary_dim / (rotary_dim - 2))) ** (-i / rotary_dim)
-        elif kind == "bands":
+        else:
             trained = float(scaling[2])
             slow, fast = (float(scaling[3]), float(scaling[4])) if len(scaling) > 3 else (1.0, 32.0)
+            if not (0.0 < trained < math.inf and -math.inf < slow < fast < math.inf):
+                raise ValueError("bands: trained must be positive and slow below fast")
             turns = trained * freq / (2 * math.pi)
             keep = ((turns - slow) / (fast - slow)).clamp(0.0, 1.0)
             freq = freq * keep + freq / f * (1 - keep)
             gain = 0.1 * math.log(f) + 1.0
-        else:
-            raise ValueError(f"unknown scaling {kind!r}")
     angle = torch.outer(torch.arange(max_pos, dtype=torch.float64), freq)
     return (torch.stack([angle.cos(), angle.sin()], dim=-1) * gain).float().to(device).contiguous()
 

@@ -170,6 +170,33 @@ def test_rotary_table():
             paged.rotary_table(**{"max_pos": 8, "rotary_dim": 32, "device": "cpu", **bad})
 
 
+@pytest.mark.parametrize("kw", [
+    dict(scaling=("bands", 8.0, 64, 1.0)), dict(scaling=("bands", 8.0)), dict(scaling=("linear",)),
+    dict(scaling=("bands", 8.0, 64, 4.0, 4.0)), dict(scaling=("bands", 8.0, 64, 8.0, 1.0)), dict(scaling=("bands", 8.0, 0)),
+    dict(scaling=("bands", 8.0, -64)), dict(scaling=("linear", math.inf)), dict(scaling=("linear", math.nan)),
+    dict(theta=0.0), dict(theta=-10000.0), dict(theta=math.nan), dict(theta=math.inf)])
+def test_rotary_table_refuses_what_it_has_no_angles_for(kw):
+    with pytest.raises(ValueError):
+        paged.rotary_table(8, 32, device="cpu", **kw)
+
+
+def test_rotary_table_between_the_bands():
+    """Pairs that turn between `slow` and `fast` times are stretched in part, linear in their turns."""
+    f, theta, trained, slow, fast = 4.0, 1000.0, 300, 2.0, 20.0
+    t = paged.rotary_table(200, 64, theta=theta, scaling=("bands", f, trained, slow, fast), device="cpu")
+    g, between = 0.1 * math.log(f) + 1, 0
+    for i in range(32):
+        w = theta ** (-2 * i / 64)
+        keep = min(1.0, max(0.0, (trained * w / (2 * math.pi) - slow) / (fast - slow)))
+        between += 0.0 < keep < 1.0
+        for pos in (1, 57, 199):
+            a = pos * (keep * w + (1 - keep) * w / f)
+            # one rounding of a value of at most g < 2
+            assert abs(float(t[pos, i, 0]) - g * math.cos(a)) <= 2 ** -23
+            assert abs(float(t[pos, i, 1]) - g * math.sin(a)) <= 2 ** -23
+    assert between >= 8
+
+
 def test_refusals_say_what_was_given():
     """Messages are formatted in C++, which takes one C++ runtime in the process."""
     z = torch.zeros(1, 8, 2, 128, dtype=torch.bfloat16)
