@@ -608,6 +608,55 @@ def test_bad_pages_and_lengths_are_reported_and_stay_in_bounds(cuda, wide):
     _status_clean()
 
 
+@pytest.mark.parametrize("lq,width", [(1, 64), (1, 1250), (24, 64), (90, 64), (90, 1250)])
+def test_a_captured_step_replayed_with_other_lengths(cuda, lq, width):
+    """Store, attention with weights and eviction in one graph: replayed with other starts, lengths, pages and tokens it
+    gives what the calls give outside a graph, while eager calls of the same stream go on in between."""
+    from reworld_b200 import paged_attention, paged_evict, paged_rotary_store, rotary_table
+    g = torch.Generator(device=cuda).manual_seed(41)
+    B, hq, hkv, D, page, keep = 3, 8, 2, 64, 16, 100
+    dw = -(-keep // page)
+    pool = torch.randn(B * width + B * dw, page, hkv, D, generator=g, device=cuda).to(BF)
+    tab = rotary_table(width * page, D, device=cuda)
+    q, k, v = (torch.randn(B * lq, h, D, generator=g, device=cuda).to(BF) for h in (hq, hkv, hkv))
+    order = torch.randperm(pool.shape[0], generator=g, device=cuda).to(torch.int32)
+    table, dst = order[:B * width].view(B, width).clone(), order[B * width:].view(B, dw).clone()
+    s = _starts(cuda, [lq] * B)
+    kv = torch.tensor([500, 900, 101], dtype=torch.int32, device=cuda)
+    kp, vp = pool.clone(), pool.flip(0).contiguous()
+    w = torch.zeros(B, hkv, width * page, device=cuda)
+
+    def step(kp, vp, w):
+        qr = paged_rotary_store(k, v, kp, vp, table, s, kv, table=tab, q=q)
+        out, lse = paged_attention(qr, kp, vp, table, s, kv, max_q_len=lq, weight_sums=w, return_lse=True)
+        return qr, out, lse, *paged_evict(kp, vp, table, kv, w, keep, dst, n_sink=2, n_recent=9)
+
+    step(kp.clone(), vp.clone(), w.clone())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(kp, vp, w)
+    for lens, lqs in (([500, 900, 101], [lq] * B), ([120, 1000, 777], [lq, 0, lq]), ([1024, 91, 0], [1, lq, 0]),
+                      ([lq, 300, 1000], [lq] * B)):
+        order = torch.randperm(pool.shape[0], generator=g, device=cuda).to(torch.int32)
+        for to, of in ((table, order[:B * width].view(B, width)), (dst, order[B * width:].view(B, dw)),
+                       (s, _starts(cuda, lqs)), (kv, torch.tensor(lens, dtype=torch.int32, device=cuda)),
+                       (kp, pool), (vp, pool.flip(0)), (w, torch.full_like(w, 0.25)),
+                       (q, torch.randn(q.shape, generator=g, device=cuda).to(BF))):
+            to.copy_(of)
+        k2, v2, w2 = kp.clone(), vp.clone(), w.clone()
+        want = step(k2, v2, w2)
+        graph.replay()
+        step(pool.clone(), pool.clone(), w.clone())
+        torch.cuda.synchronize()
+        n = sum(lqs)
+        for i, (a, b) in enumerate(zip((*got, kp, vp, w), (*want, k2, v2, w2))):
+            if i < 3:                                    # (rows of no sequence are undefined)
+                a, b = a[:n], b[:n]
+            assert torch.equal(*_bits(a, b)), i
+    _status_clean()
+
+
 BAD = ["page high", "page low", "length beyond", "length negative", "start falls", "start passes", "start negative"]
 
 
