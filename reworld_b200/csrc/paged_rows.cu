@@ -162,6 +162,12 @@ __device__ __forceinline__ float2 ld_cluster2(uint32_t a) {
   return v;
 }
 
+// What a score weighs, by its row's m and 1 / l.  One of -inf (a key that the row does not see, above all) weighs nothing,
+// also where the row's total is NaN.
+__device__ __forceinline__ float weight_of(float score, float2 ml) {
+  return score == -INFINITY ? 0.f : fast_exp2(score - ml.x) * ml.y;
+}
+
 constexpr int MAX_CLUSTER = 16;
 constexpr int CLUSTER_TILES = 16;  // of a CTA at most
 
@@ -603,7 +609,7 @@ __global__ void __launch_bounds__(THREADS, 2) rows_kernel(const __grid_constant_
         for (int i = 0; i < KEYS; ++i)
           if (i * THREADS < keys) {
             float add = 0.f;
-            for (int r = 0; r < en.rows; ++r) add += fast_exp2(sc_sh[r * p.pitch + i * THREADS] - ml[r].x) * ml[r].y;
+            for (int r = 0; r < en.rows; ++r) add += weight_of(sc_sh[r * p.pitch + i * THREADS], ml[r]);
             dst[i * THREADS] = old[i] + add;
           }
       }
@@ -787,10 +793,10 @@ __global__ void __launch_bounds__(JOIN_GROUPS * D / 4) join_sums_kernel(const __
     for (int r = 0; r < rows; ++r) {
       const float4 x = __ldcs(reinterpret_cast<const float4*>(sc + r * p.cap + j));
       const float2 m = ml[r];
-      add.x += fast_exp2(x.x - m.x) * m.y;
-      add.y += fast_exp2(x.y - m.x) * m.y;
-      add.z += fast_exp2(x.z - m.x) * m.y;
-      add.w += fast_exp2(x.w - m.x) * m.y;
+      add.x += weight_of(x.x, m);
+      add.y += weight_of(x.y, m);
+      add.z += weight_of(x.z, m);
+      add.w += weight_of(x.w, m);
     }
     const float a[4] = {add.x, add.y, add.z, add.w};
 #pragma unroll

@@ -72,6 +72,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   __shared__ int3 seq[chunk::MAX_BATCH];         // s0, lq, kv
   __shared__ __align__(16) float par[NS][BM];    // -(m + log2 l) of the columns' rows
   __shared__ float part_sum[2][NWG - 1][BM];
+  __shared__ int unit_nan[2 * NS];               // whether a row of the unit has a total of NaN
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dsmem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ks = smem;
   uint8_t* qs = smem + NK * TILE_BYTES;
@@ -227,12 +228,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     if (ok)
       for (int t = max(0, k - NK); t < k; ++t) mbar_wait_drain(&sb.k_free[t % NK], (uint32_t)(t / NK) & 1u);
   } else if (warp == WARP_ROWS) {
-    // -(m + log2 l) of a row tile's rows, fetched one tile ahead; -inf (no weight) for a row that is none
-    int i = 0;
+    // -(m + log2 l) of a row tile's rows, fetched one tile ahead; -inf (no weight) for a row that is none.  Also for one
+    // whose total is NaN: that would reach keys that the row does not see (-inf + NaN), so such units are marked (this warp
+    // is at most NS units ahead of the sums) and the keys that do see it get their NaN behind the unit.
+    int i = 0, k = 0;
     bool ok = true;
     float next[4];
-    for (int u = blockIdx.x; u < U && ok; u += gridDim.x) {
+    for (int u = blockIdx.x; u < U && ok; u += gridDim.x, ++k) {
       const Unit x = unit(u);
+      bool nan = false;
       auto fetch = [&](int j) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -245,10 +249,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       fetch(0);
       for (int j = 0; j < x.n; ++j, ++i) {
         const int s = i % NS;
+        bool bad = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          bad = bad || next[e] != next[e];
+          next[e] = next[e] == next[e] ? next[e] : -INFINITY;
+        }
+        nan = __any_sync(0xffffffffu, bad) || nan;
         const float4 now = make_float4(next[0], next[1], next[2], next[3]);
         fetch(j + 1);
         if (i >= NS && !(ok = wait(&sb.s_free[s], (uint32_t)(i / NS - 1) & 1u, RW_STATUS_TIMEOUT_LOAD))) break;
         *reinterpret_cast<float4*>(par[s] + 4 * lane) = now;
+        if (lane == 0) unit_nan[k % (2 * NS)] = nan;
         mbar_arrive(&sb.r_full[s]);
       }
     }
@@ -320,6 +332,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 #pragma unroll
         for (int i = 0; i < NWG - 1; ++i) sum += part_sum[h][i][r];
         mbar_arrive(&sb.part_free[h]);
+        if (unit_nan[k % (2 * NS)]) {
+#pragma unroll 1
+          for (long long e = from; e < (long long)x.s.lq * p.G; ++e) {
+            const float y = __ldg(p.row_b + (x.s.s0 + e / p.G) * p.Hq + x.hk * p.G + e % p.G);
+            if (y != y) sum = y;
+          }
+        }
         // one thread of one CTA adds to a row's sum: an addition without a return value, whose order is no matter
         if (x.key0 + r < x.s.kv) atomicAdd(p.sums + x.b * p.sums_sb + x.hk * p.sums_sh + x.key0 + r, sum);
       }

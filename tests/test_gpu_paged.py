@@ -338,6 +338,42 @@ def test_many_small_weights_beside_a_large_one(cuda, dtype, first, D, batch, lq,
     assert (lse.double() - math.log1p(small) + math.log(w)).abs().max().item() <= total + 2.0 ** -18
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lqs,lens,hq,hkv,D,wide", [
+    ([5, 3], [40, 200], 8, 2, 128, False), ([5, 3], [40, 200], 8, 2, 128, True),       # a cluster; shares
+    ([64], [500], 4, 4, 64, False), ([64], [500], 4, 4, 64, True),                     # blocks of rows; tiles
+    ([300, 150], [300, 900], 6, 2, 128, False), ([400, 200], [500, 200], 4, 1, 64, False)])
+def test_weights_of_rows_whose_total_is_nan(cuda, causal, lqs, lens, hq, hkv, D, wide):
+    """A row with NaN in its query gives NaN to the rows that it sees and nothing to the others."""
+    from reworld_b200 import paged_attention
+    k, v, table, kv, g = _cache(cuda, lens, 16, hkv, D, BF, 33)
+    table = _widen(table, wide)
+    s = _starts(cuda, lqs)
+    q = torch.randn(sum(lqs), hq, D, generator=g, device=cuda).to(BF)
+    w = [torch.zeros(len(lens), hkv, table.shape[1] * 16, device=cuda) for _ in range(2)]
+    paged_attention(q, k, v, table, s, kv, max_q_len=max(lqs), causal=causal, weight_sums=w[0])
+    want = w[0].clone()
+    G, t = hq // hkv, 0
+    for b, (lq, n) in enumerate(zip(lqs, lens)):
+        tok = lq // 3
+        q[t + tok, G - 1, 7] = math.nan                  # of the first key head's group
+        sees = n - lq + tok + 1 if causal else n
+        want[b, 0, :sees] = math.nan
+        t += lq
+    out, lse = paged_attention(q, k, v, table, s, kv, max_q_len=max(lqs), causal=causal, weight_sums=w[1], return_lse=True)
+    torch.cuda.synchronize()
+    _status_clean()
+    assert int(torch.isnan(lse).sum()) == len(lqs)
+    assert torch.equal(torch.isnan(w[1]), torch.isnan(want))
+    # the NaN row gave the others at most 1, and nothing where it sees nothing
+    assert torch.equal(w[1][:, 1:], want[:, 1:])
+    t = 0
+    for b, (lq, n) in enumerate(zip(lqs, lens)):
+        if causal:
+            x, y = w[1][b, 0, n - lq + lq // 3 + 1:], w[0][b, 0, n - lq + lq // 3 + 1:]
+            assert torch.equal(x, y)
+
+
 def test_strided_inputs_and_output(cuda):
     from reworld_b200 import paged_attention
     k, v, table, kv, g = _cache(cuda, [100, 50], 16, 2, 128, BF, 4)
