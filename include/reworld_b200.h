@@ -438,7 +438,8 @@ int rw_paged_rotary_store(const rw_paged_t* cache, const void* k, const void* v,
 
 /* Attention of the new tokens over their sequences' cached rows: out[t, h] =
  * softmax(q[t, h] k^T * softmax_scale) v over key head h / (Hq / Hkv), fp32
- * statistics and accumulation, one rounding of the output.  causal != 0: token i
+ * statistics and accumulation; the weights are rounded to the pools' type for the
+ * product with v (the totals are of the unrounded ones), the output once more.  causal != 0: token i
  * of a sequence with lq new tokens sees rows 0 .. kv - lq + i, otherwise all kv.
  * A row that sees nothing gets zeros and lse -inf.  What a token does not see has
  * no effect on it, infinities and NaN in later rows included.  lse ([T, Hq] fp32,
@@ -447,7 +448,8 @@ int rw_paged_rotary_store(const rw_paged_t* cache, const void* k, const void* v,
  * undefined).  Rows of out and lse behind the last sequence stay as they were.
  * sums (may be NULL): fp32 [B, Hkv, >= table_width * page_size] with element strides
  * sums_sb, sums_sh; sums[b, g, j] += the weights that the rows of key head g's group
- * gave to cached row j.  The order of the additions is fixed.
+ * gave to cached row j (NaN from a row whose total is NaN, for the rows that it sees).
+ * The order of the additions is fixed.
  * workspace: device memory, 16-byte aligned, rw_paged_attn_workspace_bytes(...)
  * bytes (0: it may be null), contents of no matter; calls that overlap on the GPU need workspaces of
  * their own.  With sums, and up to 16 rows (tokens x Hq / Hkv) a sequence and key head, it holds the scores: 4 *

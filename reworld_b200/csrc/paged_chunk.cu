@@ -34,8 +34,8 @@
 // The weights P are rounded to the values' 16-bit type (an MMA's operands have one type); totals are
 // sums of the unrounded ones, and O is fp32 until the output's one rounding.
 //
-// 2640 tokens over 34320 rows, 24 heads of 128: 0.88 ms (1.22 PFLOP/s) in a short run, 1.02 ms when the power
-// limit holds the clock down.
+// 2640 tokens over 34320 rows, 24 heads of 128: 0.88 ms (1.22 PFLOP/s) in a short run, 1.03 ms when the power
+// limit holds the clock down; without the causal mask, which has 4 % more to do, 1.06 (the contiguous kernel 1.00).
 #include <algorithm>
 
 #include "paged.cuh"
@@ -517,6 +517,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const float all = (float)N;            // (estimates: no division of integers for them)
       whole = fmaxf((float)pl.longest, rounds * __fdividef(all, (float)U)) <=
               fmaxf((float)MIN_SHARE, __fdividef(all, (float)C)) + JOIN_COST<D>;
+      // (a lane a sequence.  With 12 ragged sequences of up to 600 tokens the order takes 88 us to 65 with head dim 64
+      // and 99 to 96 with 128; with 32, when a CTA has many units, 177 to 175 and nothing: more go as they come)
       sorted = rounds > 1 && !equal && p.pool.B <= 32;
       if (sorted) rk = ranks(p, pl.longest - UNIT_COST, upt, lane);
     }

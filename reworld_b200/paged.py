@@ -154,9 +154,11 @@ def paged_attention(q, k_pages, v_pages, block_table, q_starts, kv_lens, max_q_l
     of a sequence with lq new tokens sees rows 0 .. kv_lens[b] - lq + i, else all kv_lens[b].  A row
     that sees nothing gets zeros (lse -inf); what a row does not see has no effect on it, infinities
     and NaN included.  max_q_len: the most new tokens of a sequence, by default T; passing it (1 for a
-    decoding step) is what lets the call choose its kernel.
+    decoding step) is what lets the call choose its kernel.  Statistics and accumulation are fp32; the
+    weights are rounded to q's type for the product with v, the output once more.
     weight_sums: fp32 [B, Hkv, cap], cap >= block_table's rows, contiguous last dim; the weight that
-    every cached row received from the new tokens (all query heads of the group) is added to it.
+    every cached row received from the new tokens (all query heads of the group) is added to it; a row
+    whose total is NaN gives NaN to the rows that it sees.
     (Few tokens' weights take scratch memory for their scores by the table's width: 4 bytes for every head, token and
     row of block_table, up to 1 GiB, or one sequence's if that is more.)
     out must not lie in the pools.

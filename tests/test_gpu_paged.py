@@ -866,6 +866,28 @@ def test_rotary(cuda, dtype, D, rot, interleaved):
     _status_clean()
 
 
+def test_rotary_of_a_grid(cuda):
+    """A table whose row is a token of the model's 3-D grid: what causal_rope_apply makes of a chunk."""
+    from oracle import rope as orope
+    from reworld_b200 import rotary
+    frames, h, w, start = 2, 4, 6, 5
+    freqs = orope.build_freqs(128, 12 / 22, 20 / 40)
+    st, sh, _ = orope.rope_split(128)
+    f, y, x = (i.flatten() for i in torch.meshgrid(torch.arange(start + frames), torch.arange(h), torch.arange(w),
+                                                   indexing="ij"))
+    z = torch.cat([freqs[f, :st], freqs[y, st:st + sh], freqs[x, st + sh:]], dim=1)      # [tokens, 64] complex
+    table = torch.view_as_real(z).float().contiguous().to(cuda)
+    g = torch.Generator(device=cuda).manual_seed(51)
+    q = torch.randn(frames * h * w, 3, 128, generator=g, device=cuda).to(BF)
+    at = torch.arange(start * h * w, (start + frames) * h * w, dtype=torch.int32, device=cuda)
+    got = rotary(q, table, at, interleaved=True).float().cpu()
+    want = torch.from_numpy(orope.causal_rope_apply(q.float().cpu().numpy()[None], [(frames, h, w)], freqs, start)[0])
+    # both are rounded once, from values an fp32 product apart: at most a step
+    pair = 4 * q.float().abs().max().item() * 2.0 ** -24
+    assert ((got - want).abs() <= torch.finfo(BF).eps * want.abs() + pair).all()
+    _status_clean()
+
+
 def test_rotary_position_outside_the_table(cuda):
     from reworld_b200 import _native, rotary, rotary_table
     tab = rotary_table(10, 64, device=cuda)
