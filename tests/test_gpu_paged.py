@@ -299,6 +299,36 @@ def test_values_of_later_tokens_that_are_not_finite(cuda, dtype, D, hq, hkv, lqs
     assert torch.equal(lse[rows], lref[rows])
 
 
+@pytest.mark.parametrize("dtype,D,hq,hkv,lqs,lens", [
+    (BF, 128, 4, 4, [1501], [1501]),                     # a prompt: from its first tile on not every row sees all
+    (FP, 64, 6, 2, [1501], [1501]),
+    (BF, 128, 8, 1, [1501, 400], [1501, 900]),
+    (FP, 128, 2, 2, [1501], [4000]),                     # units in parts
+    (BF, 64, 1, 1, [2600], [2600]),
+])
+@pytest.mark.parametrize("early", [(3,), (130, 700), (3, 131, 702, 1100)])
+def test_values_early_in_a_prompt_that_are_not_finite(cuda, dtype, D, hq, hkv, lqs, lens, early):
+    """Infinities in the values of early tokens, with hundreds of the chunk's rows behind them: the tokens before are
+    what they were bit for bit, those behind have them in the channels they are in and what they had elsewhere."""
+    from reworld_b200 import paged_attention
+    k, v, table, kv, g = _cache(cuda, lens, 16, hkv, D, dtype, 21)
+    s = _starts(cuda, lqs)
+    q = torch.randn(sum(lqs), hq, D, generator=g, device=cuda).to(dtype)
+    w0, w1 = (torch.zeros(len(lens), hkv, table.shape[1] * 16, device=cuda) for _ in range(2))
+    ref, lref = paged_attention(q, k, v, table, s, kv, max_q_len=max(lqs), weight_sums=w0, return_lse=True)
+    want = ref.float()
+    base = lens[0] - lqs[0]
+    for i, tok in enumerate(early):                      # channel 5 + i, one sign each
+        x = -math.inf if i & 1 else math.inf
+        v[int(table[0, (base + tok) // 16]), (base + tok) % 16, :, 5 + i] = x
+        want[tok:lqs[0], :, 5 + i] = x
+    out, lse = paged_attention(q, k, v, table, s, kv, max_q_len=max(lqs), weight_sums=w1, return_lse=True)
+    torch.cuda.synchronize()
+    _status_clean()
+    assert torch.equal(out.float(), want)
+    assert torch.equal(lse, lref) and torch.equal(w0, w1)
+
+
 @pytest.mark.parametrize("dtype", [BF, FP])
 @pytest.mark.parametrize("first", [0.0, 1.0])
 @pytest.mark.parametrize("D,batch,lq,n", [(64, 160, 130, 60000), (128, 80, 260, 60000), (64, 600, 1, 400000),
