@@ -68,6 +68,12 @@ constexpr float RESCALE_THRESHOLD = 8.0f;    // log2 units
 // seen (4.5 * 2^-24 from each of 60000 keys is 1.6 % of a row, 11 % of it lost).  Totals have the factor too.
 template <bool HALF> constexpr float UP_LOG2 = HALF ? 7.0f : 0.0f;
 template <bool HALF> constexpr float DOWN = HALF ? 1.0f / 128 : 1.0f;
+// What a score has added before the exponential.  For fp16 it is rounded down: scores of some 10^7 have it in steps of 2
+// and more, and half a step up would take weights of 2^15 out of fp16.
+template <bool HALF>
+__device__ __forceinline__ float minus_base(float m, float sl2) {
+  return HALF ? __fmaf_rd(-m, sl2, UP_LOG2<HALF>) : -m * sl2;
+}
 // What work dealt out in equal shares costs more than whole units: the starts of parts, and their joining.  Whole units
 // against shares: 8 units of 12 tiles 25.1 and 30.6 us, of 16 tiles 28.2 and 31.4, of 32 tiles 39.9 and 36.1 (74 pairs); 64
 // units of 35 tiles 46.5 and 56.5; head dim 64 (148 CTAs) 4 units of 8 tiles 20.3 and 22.2, of 20 tiles 26.9 and 23.8; 344
@@ -912,7 +918,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         if (one_pass) {
           uint32_t pk[2][32];
           uint64_t l2f = l2;
-          const float nm0 = UP_LOG2<HALF> - m_base * sl2;
+          const float nm0 = minus_base<HALF>(m_base, sl2);
           const uint64_t nm02 = f2_pack(nm0, nm0);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -987,7 +993,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             l2 = f2_pack(lo * f, hi * f);
             m_base = m_use;
           }
-          const float nm = m_use == -INFINITY ? 0.f : UP_LOG2<HALF> - m_use * sl2;  // nothing seen yet: weights of exp2(-inf) = 0
+          const float nm = m_use == -INFINITY ? 0.f : minus_base<HALF>(m_use, sl2);  // nothing seen yet: weights of exp2(-inf) = 0
           const uint64_t nm2 = f2_pack(nm, nm);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {

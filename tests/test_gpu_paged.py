@@ -299,6 +299,40 @@ def test_values_of_later_tokens_that_are_not_finite(cuda, dtype, D, hq, hkv, lqs
     assert torch.equal(lse[rows], lref[rows])
 
 
+@pytest.mark.parametrize("lq", [1, 300])
+@pytest.mark.parametrize("dtype,D", [(FP, 64), (FP, 128), (BF, 64)])
+def test_scores_of_ten_million(cuda, dtype, D, lq):
+    """Scores of 3.6e9 * scale = 2.6e7, where fp32 has steps of 2: the later keys are 7.98 (in powers of two) above the
+    first tile's, just what leaves its maximum the base of their weights; 2^7.98 * 2^7 still is an fp16 weight."""
+    from reworld_b200 import paged_attention
+    g = torch.Generator(device=cuda).manual_seed(61)
+    n, page, scale = 500, 16, 0.007203400135040283
+    k = torch.zeros(32, page, 1, D, dtype=dtype, device=cuda)
+    v = torch.randn(32, page, 1, D, generator=g, device=cuda).to(dtype)
+    table = _widen(torch.arange(32, dtype=torch.int32, device=cuda).view(1, 32), lq > 1)   # (by tiles)
+    # products and sums below are exact in fp32 (and 61440 and 60000 in their types)
+    big = 60000.0 if dtype == FP else 61440.0
+    k[..., 0] = big
+    k.view(-1, D)[128:, 1] = 48.0
+    q = torch.zeros(lq, 1, D, dtype=dtype, device=cuda)
+    q[..., 0], q[..., 1] = big, 16.0
+    kv = torch.tensor([n], dtype=torch.int32, device=cuda)
+    out = paged_attention(q, k, v, table, _starts(cuda, [lq]), kv, max_q_len=lq, causal=False, softmax_scale=scale)
+    torch.cuda.synchronize()
+    _status_clean()
+    if lq == 1:                                          # few rows round the scores themselves, to steps of 2
+        assert torch.isfinite(out.float()).all()
+        return
+    x = torch.where(torch.arange(n, device=cuda) < 128, 0.0, 768.0).double() * scale
+    w = torch.softmax(x, 0)
+    vals = v.view(-1, D)[:n].double()
+    want, wv = w @ vals, w @ vals.abs()
+    # the scores' difference is exact; times the scale's fp32 power-of-two form it is off by 2^-23 of 8
+    half = torch.finfo(dtype).eps / 2
+    tol = half * wv * 1.01 + half * want.abs() + 2.0 ** -17 * wv
+    assert ((out[:, 0].double() - want).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("dtype,D,hq,hkv,lqs,lens", [
     (BF, 128, 4, 4, [1501], [1501]),                     # a prompt: from its first tile on not every row sees all
     (FP, 64, 6, 2, [1501], [1501]),
