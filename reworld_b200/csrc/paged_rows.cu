@@ -866,10 +866,10 @@ inline int slice_of(int B, int Hkv, long long rows, long long cap, bool sums) {
 // More than 16 rows are so many blocks of 16, which read the keys from L2 at the same time: while all CTAs are
 // resident that is over before the tiles of chunk_kernel have filled their pipeline.  A tile takes a CTA 0.9 us, with two
 // CTAs on an SM 1.6.  By blocks and by chunk_kernel, us: 8 heads x 20 rows over 505 keys 8.7 and 18.1, over 6005 20.3 and
-// 38.9; x 64 rows over 516 keys 9.9 and 19.3; x 256 rows over 564 keys 15.2 and 20.0, over 2064 (2 CTAs an SM, 17 tiles
+// 38.9; x 64 rows over 516 keys 10.4 and 19.3; x 256 rows over 564 keys 14.9 and 20.0, over 2064 (2 CTAs an SM, 17 tiles
 // each) 28.3 and 29.2; x 512 rows over 628 keys (10 tiles) 23.7 and 20.1. 
 // What each block adds to the sums goes to scratch; add_blocks_kernel adds it up in the blocks' order: 8 heads x 64 rows
-// over 516 keys with weights 13.6 us, by chunk_kernel and weigh_kernel 25.5; x 256 rows 25.2 and 27.4.
+// over 516 keys with weights 14.1 us, by chunk_kernel and weigh_kernel 25.5; x 256 rows 26.1 and 27.4.
 struct Clusters {
   int cs, pitch, bytes;
 };
